@@ -464,6 +464,59 @@ int mam_select_result(void *workspace, int mode, float *out, void *stream);
 int mam_select_ranks(const float *w, int64_t ldw, int mode, const void *aux, const void *aux2, int64_t ld_aux, int64_t M, int64_t K,
                      const int64_t *ranks, int nranks, float *out, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * ---- Operators of an encoder layer around the MAM layers --------------------------------------------------------
+ * Layer norm, dropout whose mask is never stored, the join of both between a layer's halves, and differential
+ * attention.  Elements are fp32, bf16 or fp16 (`type`); sums, statistics and softmaxes are fp32, and a result is rounded
+ * to its type once.  Pointers need the alignment of their elements only.  No counterparts in the reference, whose ViT
+ * example (examples/vitb16_imagenet1k/utils.py) takes these parts from its model library.
+ */
+#define MAM_F32 0
+#define MAM_BF16 1
+#define MAM_F16 2
+
+/* A dropout: element i (of the contiguous order of the tensor's shape) is kept where word i % 4 of Philox4x32-10 with
+ * counter (i / 4, offset [+ *step]) and key `seed` is at least round(p * 2^32); a kept element is multiplied by `scale`, a
+ * dropped one is 0 whatever it holds.  `step`: NULL, or one DEVICE word that is added to offset when the kernel runs, so that a captured
+ * graph takes another mask on every replay.  The struct itself is HOST memory, read during the call. */
+typedef struct mam_dropout_t {
+    double p;
+    float scale;
+    uint64_t seed, offset;
+    const int64_t *step;
+} mam_dropout_t;
+
+/* y = dropout(x) (+ residual, may be NULL), n contiguous elements; y may be x or residual.  The gradient of x is the same
+ * call on the gradient of y (residual NULL). */
+int mam_dropout(const void *x, const void *residual, void *y, int64_t n, int type, const mam_dropout_t *drop, void *stream);
+
+/*
+ * y (N, C) contiguous = layer norm of the rows of x (row stride ldx) with biased variance; weight, bias (C), of type
+ * `weight_type` (x's or MAM_F32), or NULL; mean, rstd (N) fp32 for the backward, or NULL.
+ */
+int mam_layer_norm(const void *x, int64_t ldx, const void *weight, const void *bias, double eps, void *y, float *mean, float *rstd,
+                   int64_t N, int64_t C, int type, int weight_type, void *stream);
+/* Gradients from dy (N, C, row stride lddy): dx (N, C) contiguous, dw, db (C) of weight_type; each may be NULL.  The
+ * workspace (of N, C and type) is needed where dw or db is wanted.  Deterministic. */
+size_t mam_layer_norm_backward_workspace(int64_t N, int64_t C, int type);
+int mam_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *weight, const float *mean,
+                            const float *rstd, void *dx, void *dw, void *db, int64_t N, int64_t C, int type, int weight_type,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * s = residual + dropout(x), y = layer norm of s (as rounded to its type), both (N, C) contiguous: what stands between the halves of
+ * a pre-norm layer, as one pass.  The elements of the dropout are numbered row * C + column.
+ */
+int mam_add_dropout_layer_norm(const void *x, int64_t ldx, const void *residual, int64_t ldr, const mam_dropout_t *drop,
+                               const void *weight, const void *bias, double eps, void *y, void *s, float *mean, float *rstd,
+                               int64_t N, int64_t C, int type, int weight_type, void *stream);
+/* From dy and ds (gradient of s from elsewhere, or NULL): d_residual, dx (each may be NULL), dw, db; workspace as for
+ * mam_layer_norm_backward. */
+int mam_add_dropout_layer_norm_backward(const void *dy, int64_t lddy, const void *ds, int64_t ldds, const void *s, const void *weight,
+                                        const float *mean, const float *rstd, const mam_dropout_t *drop, void *d_residual, void *dx,
+                                        void *dw, void *db, int64_t N, int64_t C, int type, int weight_type, void *workspace,
+                                        size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

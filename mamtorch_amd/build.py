@@ -17,7 +17,8 @@ HIP_LIB = os.path.join(LIB_DIR, "libmam_hip.so")
 OPS_LIB = os.path.join(LIB_DIR, "mam_torch_ops.so")
 
 HIP_SOURCES = ["mam_common.hip", "mam_forward.hip", "mam_ordered.hip", "mam_backward.hip", "mam_selcount.hip", "mam_csr.hip",
-               "mam_spmm.hip", "mam_prune.hip", "mam_select.hip", "mam_module.hip"]
+               "mam_spmm.hip", "mam_prune.hip", "mam_select.hip", "mam_module.hip", "mam_dropout.hip",
+               "mam_norm.hip"]
 
 # -ffp-contract=off: a product that feeds an add must stay an fp32 multiply followed by an fp32
 # add (bit-exact forward).  Packed-FP32 instructions are disabled for the device pass.
@@ -66,7 +67,8 @@ def build_torch_ops(verbose=False):
     cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unknown-pragmas",
             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
-           + inc + [os.path.join(CSRC, "torch_binding.cpp"), os.path.join(CSRC, "torch_autograd.cpp"), "-o", OPS_LIB,
+           + inc + [os.path.join(CSRC, "torch_binding.cpp"), os.path.join(CSRC, "torch_autograd.cpp"),
+                   os.path.join(CSRC, "torch_encoder.cpp"), "-o", OPS_LIB,
                     "-L" + LIB_DIR, "-lmam_hip", "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-lc10",
                     "-ltorch_hip", "-lc10_hip", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib,
                     "-Wl,--no-as-needed"])

@@ -28,6 +28,9 @@ BACKWARD_FORK_AUTO = -1
 COUNT_REFERENCE = 0
 COUNT_HITS = 1
 COUNT_FLAGS = 2
+F32 = 0
+BF16 = 1
+F16 = 2
 
 EXPORTS = (
     "mam_version", "mam_error_string", "mam_last_error", "mam_init", "mam_set_option", "mam_device_info",
@@ -44,6 +47,8 @@ EXPORTS = (
     "mam_prune_row_offsets", "mam_prune_fill_csr", "mam_prune_apply",
     "mam_select_workspace", "mam_select_begin", "mam_select_accumulate", "mam_select_advance", "mam_select_result",
     "mam_select_ranks",
+    "mam_dropout", "mam_layer_norm", "mam_layer_norm_backward_workspace", "mam_layer_norm_backward",
+    "mam_add_dropout_layer_norm", "mam_add_dropout_layer_norm_backward",
 )
 
 _i64 = ctypes.c_int64
@@ -51,6 +56,12 @@ _int = ctypes.c_int
 _ptr = ctypes.c_void_p
 _size = ctypes.c_size_t
 _configured = False
+
+
+class Dropout(ctypes.Structure):
+    """mam_dropout_t"""
+    _fields_ = [("p", ctypes.c_double), ("scale", ctypes.c_float), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                ("step", ctypes.c_void_p)]
 
 
 def lib():
@@ -114,6 +125,16 @@ def lib():
         l.mam_coo_row_offsets.argtypes = [_ptr, _i64, _ptr, _i64, _ptr]
         l.mam_csr_to_dense.argtypes = [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr]
         l.mam_coo_to_dense.argtypes = [_ptr, _ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _ptr]
+        _d = ctypes.POINTER(Dropout)
+        l.mam_dropout.argtypes = [_ptr, _ptr, _ptr, _i64, _int, _d, _ptr]
+        l.mam_layer_norm.argtypes = [_ptr, _i64, _ptr, _ptr, ctypes.c_double, _ptr, _ptr, _ptr, _i64, _i64, _int, _int, _ptr]
+        l.mam_layer_norm_backward_workspace.argtypes = [_i64, _i64, _int]
+        l.mam_layer_norm_backward_workspace.restype = _size
+        l.mam_layer_norm_backward.argtypes = [_ptr, _i64, _ptr, _i64] + [_ptr] * 6 + [_i64, _i64, _int, _int, _ptr, _size, _ptr]
+        l.mam_add_dropout_layer_norm.argtypes = ([_ptr, _i64, _ptr, _i64, _d, _ptr, _ptr, ctypes.c_double] + [_ptr] * 4
+                                                 + [_i64, _i64, _int, _int, _ptr])
+        l.mam_add_dropout_layer_norm_backward.argtypes = ([_ptr, _i64, _ptr, _i64] + [_ptr] * 4 + [_d] + [_ptr] * 4
+                                                          + [_i64, _i64, _int, _int, _ptr, _size, _ptr])
         _f = ctypes.c_float
         l.mam_prune_row_offsets.argtypes = [_ptr, _i64, _int, _ptr, _ptr, _i64, _f, _ptr, _i64, _i64, _ptr]
         l.mam_prune_fill_csr.argtypes = [_ptr, _i64, _int, _ptr, _ptr, _i64, _f, _ptr, _ptr, _ptr, _i64, _i64, _ptr]
