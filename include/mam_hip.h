@@ -517,6 +517,42 @@ int mam_add_dropout_layer_norm_backward(const void *dy, int64_t lddy, const void
                                         void *dw, void *db, int64_t N, int64_t C, int type, int weight_type, void *workspace,
                                         size_t workspace_bytes, void *stream);
 
+/*
+ * Differential attention: out[b, i, h] = (P1 - lam[h] P2) V with Pm the softmax over the keys j of scale * q[b, i, h, m] . k[b, j, h', m],
+ * h' = h / (H / Hkv) the key head that query head h shares.  All pointers are DEVICE memory, the struct itself HOST memory read during the
+ * call; strides are in elements, the last dimension of q, k, v has stride 1.
+ *   q (B, Lq, H, 2, D), k (B, Lk, Hkv, 2, D), v (B, Lk, Hkv, Dv), lam (H) of `lam_type` (`type` or MAM_F32); D <= 128, Dv <= 256
+ *   lengths (B) int32 or NULL: keys of each request (clamped to 0 .. Lk), all where NULL
+ *   key_mask (B, Lk) bytes, batches mask_stride apart, or NULL: keys with 0 are not seen by any query
+ *   causal: query i sees keys j <= i + starts[b] (int32, B); starts NULL: i + Lk - Lq
+ * Keys and values that lengths, key_mask or the causal limit of all queries leave out are not used, whatever their memory holds.  A
+ * query that sees no key gives zeros, and no gradient.
+ */
+typedef struct mam_diff_attention_t {
+    const void *q, *k, *v, *lam;
+    int64_t q_stride[4], k_stride[4], v_stride[3];   /* q, k: batch, token, head, map; v: batch, token, head */
+    const int32_t *lengths, *starts;
+    const unsigned char *key_mask;
+    int64_t mask_stride;
+    int64_t B, Lq, Lk, H, Hkv, D, Dv;
+    double scale;
+    int causal, type, lam_type;
+} mam_diff_attention_t;
+
+/* out (B, Lq, H, Dv) contiguous; for the backward: out2 (like out, P2 V) and lse (2, B, H, Lq) fp32 (log2 of each row's sum of
+ * exponentials, +inf where it sees no key), or NULL.  The workspace (of the sizes; 0 for most calls) holds partial results where the keys of few
+ * queries are split over workgroups. */
+size_t mam_diff_attention_workspace(const mam_diff_attention_t *args);
+int mam_diff_attention(const mam_diff_attention_t *args, void *out, void *out2, float *lse, void *workspace, size_t workspace_bytes,
+                       void *stream);
+/* Gradients from dout (B, Lq, H, Dv; strides of batch, token, head in HOST memory, last dimension 1) and the forward's out, out2 and lse:
+ * dq (B, Lq, H, 2, D), dk (B, Lk, Hkv, 2, D), dv (B, Lk, Hkv, Dv), dlam (H, of lam_type), contiguous, fully written (zeros where a key is
+ * not seen); each may be NULL.  Deterministic. */
+size_t mam_diff_attention_backward_workspace(const mam_diff_attention_t *args);
+int mam_diff_attention_backward(const mam_diff_attention_t *args, const void *dout, const int64_t *dout_stride, const void *out,
+                                const void *out2, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -49,6 +49,7 @@ EXPORTS = (
     "mam_select_ranks",
     "mam_dropout", "mam_layer_norm", "mam_layer_norm_backward_workspace", "mam_layer_norm_backward",
     "mam_add_dropout_layer_norm", "mam_add_dropout_layer_norm_backward",
+    "mam_diff_attention_workspace", "mam_diff_attention", "mam_diff_attention_backward_workspace", "mam_diff_attention_backward",
 )
 
 _i64 = ctypes.c_int64
@@ -62,6 +63,14 @@ class Dropout(ctypes.Structure):
     """mam_dropout_t"""
     _fields_ = [("p", ctypes.c_double), ("scale", ctypes.c_float), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
                 ("step", ctypes.c_void_p)]
+
+
+class DiffAttention(ctypes.Structure):
+    """mam_diff_attention_t"""
+    _fields_ = [("q", _ptr), ("k", _ptr), ("v", _ptr), ("lam", _ptr), ("q_stride", _i64 * 4), ("k_stride", _i64 * 4), ("v_stride", _i64 * 3),
+                ("lengths", _ptr), ("starts", _ptr), ("key_mask", _ptr), ("mask_stride", _i64)] + [
+                (n, _i64) for n in ("B", "Lq", "Lk", "H", "Hkv", "D", "Dv")] + [
+                ("scale", ctypes.c_double), ("causal", _int), ("type", _int), ("lam_type", _int)]
 
 
 def lib():
@@ -135,6 +144,13 @@ def lib():
                                                  + [_i64, _i64, _int, _int, _ptr])
         l.mam_add_dropout_layer_norm_backward.argtypes = ([_ptr, _i64, _ptr, _i64] + [_ptr] * 4 + [_d] + [_ptr] * 4
                                                           + [_i64, _i64, _int, _int, _ptr, _size, _ptr])
+        _a = ctypes.POINTER(DiffAttention)
+        l.mam_diff_attention_workspace.argtypes = [_a]
+        l.mam_diff_attention_workspace.restype = _size
+        l.mam_diff_attention.argtypes = [_a, _ptr, _ptr, _ptr, _ptr, _size, _ptr]
+        l.mam_diff_attention_backward_workspace.argtypes = [_a]
+        l.mam_diff_attention_backward_workspace.restype = _size
+        l.mam_diff_attention_backward.argtypes = [_a, _ptr, ctypes.POINTER(_i64)] + [_ptr] * 8 + [_size, _ptr]
         _f = ctypes.c_float
         l.mam_prune_row_offsets.argtypes = [_ptr, _i64, _int, _ptr, _ptr, _i64, _f, _ptr, _i64, _i64, _ptr]
         l.mam_prune_fill_csr.argtypes = [_ptr, _i64, _int, _ptr, _ptr, _i64, _f, _ptr, _ptr, _ptr, _i64, _i64, _ptr]

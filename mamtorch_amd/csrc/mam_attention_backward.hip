@@ -1,0 +1,424 @@
+// Differential attention, backward. With A = P1 - lambda P2 (Pm formed again from the scores and the forward's sums):
+//
+//   dV = A^T dO,  dA = dO V^T,  d1 = rowsum(dO O1),  d2 = rowsum(dO O2)
+//   dS1 = P1 (dA - d1),  dS2 = -lambda P2 (dA - d2),  dQm = scale dSm Km,  dKm = scale dSm^T Qm,  dlambda = -sum d2
+//
+// Three kernels: what the rows need beside the scores (sums, d1, d2, lambda), dQ by workgroups that own rows and pass over the keys, dK and dV
+// by workgroups that own keys and pass over the rows of all heads that share them.  Scores and dA are formed in both, 7 parts of
+// work instead of 5, and nothing is added to memory by more than one workgroup: no atomics, the same bits on every call.  Bound by the
+// matrix cores and, in 16-bit types, the exponentials beside them.
+#include "mam_attention.h"
+
+namespace mam {
+namespace attention {
+
+constexpr int STEP = 32;        // keys (dQ) or rows (dK, dV) of a tile
+
+// What a row brings beside its query: five planes of B * Hkv * R floats.
+enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, PLANES };
+
+struct BackwardCall {
+    Call a;
+    const void *dout, *out, *out2;      // dout strided, out and out2 contiguous (B, Lq, H, dv)
+    int64_t gb, gl, gh;
+    const float *lse;
+    void *dq, *dk, *dv, *dlam;
+    float *rows;                        // PLANES planes
+};
+
+// A row's planes: 16 lanes a row.
+template <class T>
+__global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
+{
+    const Call &a = g.a;
+    const int64_t count = (int64_t)a.B * a.Hkv * a.R, id = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    if (id >= count) return;
+    const int lane = threadIdx.x & 15, row = (int)(id % a.R), bh = (int)(id / a.R), b = bh / a.Hkv;
+    const int query = row / a.G, head = bh % a.Hkv * a.G + row % a.G;
+    const T *grad = static_cast<const T *>(g.dout) + b * g.gb + query * g.gl + head * g.gh;
+    const int64_t at = (((int64_t)b * a.Lq + query) * a.H + head) * a.dv;
+    const T *out = static_cast<const T *>(g.out) + at, *out2 = static_cast<const T *>(g.out2) + at;
+    float dot = 0.0f, dot2 = 0.0f;
+    for (int c = lane * kPack<T>; c < a.dv; c += 16 * kPack<T>) {
+        float v[kPack<T>], o[kPack<T>], o2[kPack<T>];
+        load_pack<T>(grad + c, a.dv - c, v);
+        load_pack<T>(out + c, a.dv - c, o);
+        load_pack<T>(out2 + c, a.dv - c, o2);
+#pragma unroll
+        for (int u = 0; u < kPack<T>; ++u) {
+            dot = fmaf(v[u], o[u], dot);
+            dot2 = fmaf(v[u], o2[u], dot2);
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+        dot += __shfl_xor(dot, m);
+        dot2 += __shfl_xor(dot2, m);
+    }
+    if (lane) return;
+    const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
+    const int64_t sums = ((int64_t)b * a.H + head) * a.Lq + query;
+    g.rows[MINUS_SUM1 * count + id] = -g.lse[sums];
+    g.rows[MINUS_SUM2 * count + id] = -g.lse[(int64_t)a.B * a.H * a.Lq + sums];
+    g.rows[DOT1 * count + id] = fmaf(lam, dot2, dot);       // O1 = out + lambda O2
+    g.rows[DOT2 * count + id] = dot2;
+    g.rows[LAMBDA * count + id] = lam;
+}
+
+// dlambda of a head, a workgroup each.
+template <class T>
+__global__ __launch_bounds__(1024) void lambda_kernel(const BackwardCall g)
+{
+    __shared__ float part[16];
+    const Call &a = g.a;
+    const int head = blockIdx.x, hk = head / a.G, which = head % a.G;
+    const int64_t count = (int64_t)a.B * a.Hkv * a.R, terms = (int64_t)a.B * a.Lq;
+    const float *dots = g.rows + DOT2 * count;
+    float sum = 0.0f;
+    for (int64_t t = threadIdx.x; t < terms; t += 1024) {
+        const int64_t b = t / a.Lq, i = t % a.Lq;
+        sum -= dots[(b * a.Hkv + hk) * a.R + i * a.G + which];
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x) return;
+    sum = 0.0f;
+    for (int w = 0; w < 16; ++w) sum += part[w];
+    if (a.lam_same) static_cast<T *>(g.dlam)[head] = (T)sum;
+    else static_cast<float *>(g.dlam)[head] = sum;
+}
+
+template <int TR>
+__device__ __forceinline__ void clear(Acc<TR> &c)
+{
+#pragma unroll
+    for (int i = 0; i < TR * TR / 64; ++i) c[i] = 0.0f;
+}
+
+// A wave's accumulators (columns col .. of its lanes' rows) to memory, times `scale`.
+template <class T, int TR>
+__device__ __forceinline__ void store_columns(T *p, int left, const Acc<TR> &c, float scale)
+{
+#pragma unroll
+    for (int f = 0; f < TR * TR / 64; f += 4) {
+        const int col = (f / 4) * 4 * GROUPS<TR> + 4 * lane_group<TR>();
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = c[f + u] * scale;
+        if (col < left) store_pack<T, 4>(p + col, left - col, v);
+    }
+}
+
+template <class T, int TR, int D, int DV>
+__global__ __launch_bounds__(256, 1) void queries_kernel(const BackwardCall g, int row_tiles)
+{
+    constexpr int ROWS = 4 * TR;
+    typedef Stage<T, 256, STEP, 2, D> StageK;
+    typedef Stage<T, 256, STEP, 1, DV> StageV;
+    __shared__ __attribute__((aligned(16))) T k_tile[STEP * StageK::PITCH];
+    __shared__ __attribute__((aligned(16))) T v_tile[STEP * StageV::PITCH];
+    const Call &a = g.a;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int bh = id / row_tiles, tile = row_tiles - 1 - id % row_tiles;
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const Reach reach = reach_of(a, b);
+    const int wave = threadIdx.x >> 6;
+    const int first = tile * ROWS + wave * TR, row = first + lane_row<TR>();
+    const bool there = row < a.R;
+    const int query = there ? row / a.G : 0, head = hk * a.G + (there ? row - query * a.G : 0);
+    const int limit = there ? reach.of_query(query) : 0;
+    const int wave_last = first + TR - 1 < a.R ? first + TR - 1 : a.R - 1;
+    const int wave_all = first < a.R ? reach.of_query(first / a.G) : 0, wave_any = first < a.R ? reach.of_query(wave_last / a.G) : 0;
+    const int last = tile * ROWS + ROWS - 1 < a.R ? tile * ROWS + ROWS - 1 : a.R - 1;
+    const int end = reach.of_query(last / a.G);
+
+    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d};
+    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv};
+    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d};
+    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv};
+    Frag<T> q[2][D / KS<T, TR>], grad[DV / KS<T, TR>];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
+    load_rows<T, TR, DV>(gs, row, there, 0, grad);
+    const int64_t count = (int64_t)a.B * a.Hkv * a.R;
+    const float *plane = g.rows + (int64_t)bh * a.R + (there ? row : 0);
+    const float minus_sum[2] = {plane[MINUS_SUM1 * count], plane[MINUS_SUM2 * count]};
+    const float dot[2] = {plane[DOT1 * count], plane[DOT2 * count]}, weight[2] = {1.0f, -plane[LAMBDA * count]};
+    const float c = a.scale * LOG2E;
+
+    Acc<TR> dq[2][D / TR];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int blk = 0; blk < D / TR; ++blk) clear<TR>(dq[m][blk]);
+    const auto seen = [&](int key) { return key < end && (!a.mask || a.mask[b * a.mask_b + key] != 0); };
+    StageK k_stage;
+    StageV v_stage;
+    k_stage.load(ks, 0, seen);
+    v_stage.load(vs, 0, seen);
+    for (int key = 0; key < end; key += STEP) {
+        __syncthreads();
+        k_stage.store(k_tile);
+        v_stage.store(v_tile);
+        __syncthreads();
+        if (key + STEP < end) {
+            k_stage.load(ks, key + STEP, seen);
+            v_stage.load(vs, key + STEP, seen);
+        }
+        if (key >= wave_any) continue;
+        const bool limited = key + STEP > wave_all || a.mask;
+        const uint32_t word = a.mask ? mask_word(a, b, key) : 0xffffffffu;
+        Acc<TR> da[BLOCKS<TR>];
+#pragma unroll
+        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+            clear<TR>(da[blk]);
+#pragma unroll
+            for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
+                mma<TR>(row_frag<T, TR>(v_tile, StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float ds[REGS<TR>];
+#pragma unroll
+            for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+                Acc<TR> s;
+                clear<TR>(s);
+#pragma unroll
+                for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+                    mma<TR>(row_frag<T, TR>(k_tile + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
+#pragma unroll
+                for (int i = 0; i < TR * TR / 64; ++i) {
+                    const int f = blk * (TR * TR / 64) + i, at = index_of<TR>(f);
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
+                    if (limited && !(at < limit - key && (word >> at & 1))) p = 0.0f;
+                    ds[f] = weight[m] * p * (da[blk][i] - dot[m]);
+                }
+            }
+            Frag<T> frag[FRAGS<T, TR>];
+            to_frags<T, TR>(ds, frag);
+#pragma unroll
+            for (int blk = 0; blk < D / TR; ++blk)
+#pragma unroll
+                for (int j = 0; j < FRAGS<T, TR>; ++j)
+                    mma<TR>(column_frag<TR>(k_tile + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
+        }
+    }
+    if (!there) return;
+    T *out = static_cast<T *>(g.dq) + (((int64_t)b * a.Lq + query) * a.H + head) * 2 * a.d;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dq[m][blk], a.scale);
+}
+
+template <class T, int TR, int D, int DV>
+__global__ __launch_bounds__(256, 1) void keys_kernel(const BackwardCall g, int key_tiles)
+{
+    constexpr int KEYS = 4 * TR;
+    typedef Stage<T, 256, STEP, 2, D> StageQ;
+    typedef Stage<T, 256, STEP, 1, DV> StageG;
+    __shared__ __attribute__((aligned(16))) T q_tile[STEP * StageQ::PITCH];
+    __shared__ __attribute__((aligned(16))) T g_tile[STEP * StageG::PITCH];
+    __shared__ __attribute__((aligned(16))) float planes[PLANES][STEP];
+    const Call &a = g.a;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int bh = id / key_tiles, tile = id % key_tiles;      // the first keys, which most rows of a causal call see, begin first
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const Reach reach = reach_of(a, b);
+    const int wave = threadIdx.x >> 6;
+    const int first = tile * KEYS + wave * TR, key = first + lane_row<TR>();
+    // rows that see a key begin at (key - reach.first) * G; past every row where none does
+    const auto from = [&](int k) {
+        const int64_t i = (int64_t)k - reach.first;
+        return i <= 0 ? 0 : i >= a.Lq ? a.R : (int)(i * a.G);
+    };
+    const bool seen = key < reach.keys && from(key) < a.R && (!a.mask || a.mask[b * a.mask_b + key] != 0);
+    const int lane_from = seen ? from(key) : a.R;
+    const bool wave_seen = first < reach.keys;
+    const int wave_any = wave_seen ? from(first) : a.R;
+    const int wave_all = first + TR <= reach.keys && !a.mask ? from(first + TR - 1) : a.R;    // from here on every lane's key is seen
+    const int begin = tile * KEYS < reach.keys ? from(tile * KEYS) / STEP * STEP : a.R;
+
+    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d};
+    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv};
+    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d};
+    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv};
+    Frag<T> k[2][D / KS<T, TR>], v[DV / KS<T, TR>];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(ks, key, seen, m, k[m]);
+    load_rows<T, TR, DV>(vs, key, seen, 0, v);
+    const int64_t count = (int64_t)a.B * a.Hkv * a.R;
+    const float *rows = g.rows + (int64_t)bh * a.R;
+    const float c = a.scale * LOG2E;
+
+    Acc<TR> dk[2][D / TR], dv[DV / TR];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int blk = 0; blk < D / TR; ++blk) clear<TR>(dk[m][blk]);
+#pragma unroll
+    for (int blk = 0; blk < DV / TR; ++blk) clear<TR>(dv[blk]);
+    const auto in = [&](int row) { return row < a.R; };
+    StageQ q_stage;
+    StageG g_stage;
+    float plane = 0.0f;
+    // a row past the last has a sum of +inf: its probabilities are 0
+    const auto load_planes = [&](int row0) {
+        const int p = threadIdx.x / STEP, row = row0 + threadIdx.x % STEP;
+        if (p < PLANES) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
+    };
+    if (begin < a.R) {
+        q_stage.load(qs, begin, in);
+        g_stage.load(gs, begin, in);
+        load_planes(begin);
+    }
+    for (int row = begin; row < a.R; row += STEP) {
+        __syncthreads();
+        q_stage.store(q_tile);
+        g_stage.store(g_tile);
+        if (threadIdx.x < PLANES * STEP) planes[threadIdx.x / STEP][threadIdx.x % STEP] = plane;
+        __syncthreads();
+        if (row + STEP < a.R) {
+            q_stage.load(qs, row + STEP, in);
+            g_stage.load(gs, row + STEP, in);
+            load_planes(row + STEP);
+        }
+        if (row + STEP <= wave_any) continue;
+        const bool limited = row < wave_all;
+        Acc<TR> da[BLOCKS<TR>];
+        float p[2][REGS<TR>];
+#pragma unroll
+        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+            clear<TR>(da[blk]);
+#pragma unroll
+            for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
+                mma<TR>(row_frag<T, TR>(g_tile, StageG::PITCH, blk * TR + lane_row<TR>(), kk), v[kk], da[blk]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+                Acc<TR> s;
+                clear<TR>(s);
+#pragma unroll
+                for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+                    mma<TR>(row_frag<T, TR>(q_tile + m * D, StageQ::PITCH, blk * TR + lane_row<TR>(), kk), k[m][kk], s);
+#pragma unroll
+                for (int i = 0; i < TR * TR / 64; ++i) {
+                    const int f = blk * (TR * TR / 64) + i, at = index_of<TR>(f);
+                    float t = __builtin_amdgcn_exp2f(fmaf(s[i], c, planes[m ? MINUS_SUM2 : MINUS_SUM1][at]));
+                    if (limited && row + at < lane_from) t = 0.0f;
+                    p[m][f] = m ? t * planes[LAMBDA][at] : t;       // the second map's with lambda
+                }
+            }
+        {
+            float diff[REGS<TR>];
+            Frag<T> frag[FRAGS<T, TR>];
+#pragma unroll
+            for (int f = 0; f < REGS<TR>; ++f) diff[f] = p[0][f] - p[1][f];
+            to_frags<T, TR>(diff, frag);
+#pragma unroll
+            for (int blk = 0; blk < DV / TR; ++blk)
+#pragma unroll
+                for (int j = 0; j < FRAGS<T, TR>; ++j) mma<TR>(column_frag<TR>(g_tile, StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float ds[REGS<TR>];
+            Frag<T> frag[FRAGS<T, TR>];
+#pragma unroll
+            for (int f = 0; f < REGS<TR>; ++f) {
+                const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[m ? DOT2 : DOT1][index_of<TR>(f)];
+                ds[f] = (m ? -p[m][f] : p[m][f]) * d;
+            }
+            to_frags<T, TR>(ds, frag);
+#pragma unroll
+            for (int blk = 0; blk < D / TR; ++blk)
+#pragma unroll
+                for (int j = 0; j < FRAGS<T, TR>; ++j)
+                    mma<TR>(column_frag<TR>(q_tile + m * D, StageQ::PITCH, blk * TR, j), frag[j], dk[m][blk]);
+        }
+    }
+    if (key >= a.Lk) return;
+    const int64_t at = ((int64_t)b * a.Lk + key) * a.Hkv + hk;
+    if (g.dk) {
+        T *out = static_cast<T *>(g.dk) + at * 2 * a.d;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dk[m][blk], a.scale);
+    }
+    if (g.dv) {
+        T *out = static_cast<T *>(g.dv) + at * a.dv;
+#pragma unroll
+        for (int blk = 0; blk < DV / TR; ++blk) store_columns<T, TR>(out + blk * TR, a.dv - blk * TR, dv[blk], 1.0f);
+    }
+}
+
+template <class T>
+struct Backward {
+    const BackwardCall &g;
+    hipStream_t st;
+    template <int D, int DV>
+    int operator()() const
+    {
+        constexpr int TR = TILE_ROWS<D, DV>;
+        const Call &a = g.a;
+        const int64_t rows = (int64_t)a.B * a.Hkv * a.R, row_tiles = ceil_div(a.R, 4 * TR), key_tiles = ceil_div(a.Lk, 4 * TR);
+        if (ceil_div(rows, 16) > INT32_MAX || key_tiles * a.B * a.Hkv > INT32_MAX) return fail(MAM_ERR_UNSUPPORTED, "too many tiles");
+        int rc = MAM_OK;
+        if (rows > 0) {
+            hipLaunchKernelGGL((rows_kernel<T>), dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, st, g);
+            rc = check_launch("attention::rows_kernel");
+        }
+        if (rc == MAM_OK && g.dq && rows > 0) {
+            hipLaunchKernelGGL((queries_kernel<T, TR, D, DV>), dim3((unsigned)(row_tiles * a.B * a.Hkv)), dim3(256), 0, st, g, (int)row_tiles);
+            rc = check_launch("attention::queries_kernel");
+        }
+        if (rc == MAM_OK && (g.dk || g.dv) && key_tiles * a.B * a.Hkv > 0) {
+            hipLaunchKernelGGL((keys_kernel<T, TR, D, DV>), dim3((unsigned)(key_tiles * a.B * a.Hkv)), dim3(256), 0, st, g, (int)key_tiles);
+            rc = check_launch("attention::keys_kernel");
+        }
+        if (rc == MAM_OK && g.dlam && a.H > 0) {
+            hipLaunchKernelGGL((lambda_kernel<T>), dim3((unsigned)a.H), dim3(1024), 0, st, g);
+            rc = check_launch("attention::lambda_kernel");
+        }
+        return rc;
+    }
+};
+
+}  // namespace attention
+}  // namespace mam
+
+extern "C" size_t mam_diff_attention_backward_workspace(const mam_diff_attention_t *args)
+{
+    if (!args || args->B <= 0 || args->Lq <= 0 || args->H <= 0) return 0;
+    return (size_t)mam::attention::PLANES * (size_t)args->B * (size_t)args->Lq * (size_t)args->H * sizeof(float);
+}
+
+extern "C" int mam_diff_attention_backward(const mam_diff_attention_t *args, const void *dout, const int64_t *dout_stride, const void *out,
+                                           const void *out2, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
+                                           size_t workspace_bytes, void *stream)
+{
+    using namespace mam;
+    attention::BackwardCall g{};
+    const int rc = attention::fill_call(args, g.a);
+    if (rc != MAM_OK) return rc;
+    const attention::Call &a = g.a;
+    const bool rows = a.B > 0 && a.R > 0;
+    if (rows && (!a.q || !a.lam || !dout || !dout_stride || !out || !out2 || !lse)) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
+    if (a.B > 0 && a.Lk > 0 && a.H > 0 && (!a.k || !a.v)) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
+    const size_t need = mam_diff_attention_backward_workspace(args);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MAM_ERR_WORKSPACE, "the attention's backward needs %zu workspace bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+    g.dout = dout; g.out = out; g.out2 = out2; g.lse = lse;
+    if (dout_stride) { g.gb = dout_stride[0]; g.gl = dout_stride[1]; g.gh = dout_stride[2]; }
+    g.dq = dq; g.dk = dk; g.dv = dv; g.dlam = dlam;
+    g.rows = static_cast<float *>(workspace);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (args->type == MAM_F32) return attention::with_head_sizes(a.d, a.dv, attention::Backward<float>{g, st});
+    if (args->type == MAM_BF16) return attention::with_head_sizes(a.d, a.dv, attention::Backward<bf16>{g, st});
+    return attention::with_head_sizes(a.d, a.dv, attention::Backward<f16>{g, st});
+}

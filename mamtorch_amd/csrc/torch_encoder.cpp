@@ -230,6 +230,119 @@ Tensors add_dropout_layer_norm_backward_cuda(const Tensor &dy, const MaybeTensor
     return {or_empty(dx, s), or_empty(dr, s), or_empty(grads.dw, s), or_empty(grads.db, s)};
 }
 
+// A tensor with elements next to each other in its last dimension: itself, or a copy.
+Tensor unit_last(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+struct AttentionCall {
+    mam_diff_attention_t a;
+    Tensor q, k, v, mask;           // what the pointers belong to
+};
+
+AttentionCall attention_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, double scale, bool causal,
+                             const MaybeTensor &lengths, const MaybeTensor &starts, const MaybeTensor &key_mask)
+{
+    AttentionCall c{};
+    mam_diff_attention_t &a = c.a;
+    a.type = type_of(q, "q");
+    for (const Tensor *t : {&k, &v}) {
+        const char *name = t == &k ? "k" : "v";
+        TORCH_CHECK(t->device() == q.device(), name, " is on a different device");
+        TORCH_CHECK(t->scalar_type() == q.scalar_type(), name, " must have q's type ", q.scalar_type(), ", got ", t->scalar_type());
+    }
+    TORCH_CHECK(q.dim() == 5 && q.size(3) == 2, "q must be (batch, queries, heads, 2, head size), got ", q.sizes());
+    TORCH_CHECK(k.dim() == 5 && k.size(3) == 2, "k must be (batch, keys, key heads, 2, head size), got ", k.sizes());
+    TORCH_CHECK(v.dim() == 4, "v must be (batch, keys, key heads, value size), got ", v.sizes());
+    a.B = q.size(0); a.Lq = q.size(1); a.H = q.size(2); a.D = q.size(4);
+    a.Lk = k.size(1); a.Hkv = k.size(2); a.Dv = v.size(3);
+    TORCH_CHECK(k.size(0) == a.B && v.size(0) == a.B && v.size(1) == a.Lk && v.size(2) == a.Hkv && k.size(4) == a.D,
+                "q ", q.sizes(), ", k ", k.sizes(), " and v ", v.sizes(), " do not match");
+    TORCH_CHECK(a.H == 0 || (a.Hkv > 0 && a.H % a.Hkv == 0), "the ", a.Hkv, " key heads must divide the ", a.H, " query heads");
+    TORCH_CHECK(a.D >= 1 && a.D <= 128 && a.Dv >= 1 && a.Dv <= 256, "head sizes are 1 to 128 and value sizes 1 to 256, got ", a.D, " and ", a.Dv);
+    TORCH_CHECK(lam.device() == q.device(), "lam is on a different device");
+    a.lam_type = type_of(lam, "lam");
+    TORCH_CHECK(a.lam_type == a.type || a.lam_type == MAM_F32, "lam must be float32 or of q's type");
+    TORCH_CHECK(lam.dim() == 1 && lam.size(0) == a.H && lam.is_contiguous(), "lam must be a contiguous vector of ", a.H, " heads");
+    TORCH_CHECK(scale > 0 && scale <= 1e30, "scale must be positive and finite, got ", scale);
+    for (const MaybeTensor *t : {&lengths, &starts}) {
+        const char *name = t == &lengths ? "lengths" : "starts";
+        if (!has(*t)) continue;
+        TORCH_CHECK((*t)->device() == q.device(), name, " is on a different device");
+        TORCH_CHECK((*t)->scalar_type() == at::kInt && (*t)->dim() == 1 && (*t)->size(0) == a.B && (*t)->is_contiguous(), name,
+                    " must be a contiguous int32 vector of ", a.B, " requests");
+    }
+    TORCH_CHECK(!has(starts) || causal, "starts is for causal calls");
+    if (has(key_mask)) {
+        TORCH_CHECK(key_mask->device() == q.device(), "key_mask is on a different device");
+        TORCH_CHECK(key_mask->scalar_type() == at::kBool && key_mask->dim() == 2 && key_mask->size(0) == a.B && key_mask->size(1) == a.Lk,
+                    "key_mask must be a bool tensor of (", a.B, ", ", a.Lk, ")");
+        c.mask = unit_last(*key_mask);
+        a.key_mask = static_cast<const unsigned char *>(c.mask.data_ptr());
+        a.mask_stride = c.mask.stride(0);
+    }
+    c.q = unit_last(q);
+    c.k = unit_last(k);
+    c.v = unit_last(v);
+    a.q = c.q.data_ptr(); a.k = c.k.data_ptr(); a.v = c.v.data_ptr(); a.lam = lam.data_ptr();
+    for (int i = 0; i < 4; ++i) {
+        a.q_stride[i] = c.q.stride(i);
+        a.k_stride[i] = c.k.stride(i);
+        if (i < 3) a.v_stride[i] = c.v.stride(i);
+    }
+    a.lengths = has(lengths) ? lengths->data_ptr<int32_t>() : nullptr;
+    a.starts = has(starts) ? starts->data_ptr<int32_t>() : nullptr;
+    a.scale = scale;
+    a.causal = causal;
+    return c;
+}
+
+Tensors diff_attention_cuda(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, double scale, bool causal,
+                            const MaybeTensor &lengths, const MaybeTensor &starts, const MaybeTensor &key_mask, bool with_sums)
+{
+    const c10::DeviceGuard guard(q.device());
+    const AttentionCall c = attention_call(q, k, v, lam, scale, causal, lengths, starts, key_mask);
+    const mam_diff_attention_t &a = c.a;
+    Tensor out = at::empty({a.B, a.Lq, a.H, a.Dv}, q.options());
+    Tensor out2 = with_sums ? at::empty({a.B, a.Lq, a.H, a.Dv}, q.options()) : at::empty({0}, q.options());
+    Tensor lse = with_sums ? at::empty({2, a.B, a.H, a.Lq}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
+    const Tensor ws = workspace_for(mam_diff_attention_workspace(&a), q);
+    check_rc(mam_diff_attention(&a, out.data_ptr(), with_sums ? out2.data_ptr() : nullptr, with_sums ? lse.data_ptr<float>() : nullptr,
+                                out_ptr(ws), ws.defined() ? ws.numel() : 0, current_stream(q)),
+             "mam_diff_attention");
+    return {out, out2, lse};
+}
+
+// wanted: the gradients of q, of k and v, of lam
+Tensors diff_attention_backward_cuda(const Tensor &grad, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, const Tensor &out,
+                                     const Tensor &out2, const Tensor &lse, double scale, bool causal, const MaybeTensor &lengths,
+                                     const MaybeTensor &starts, const MaybeTensor &key_mask, bool want_q, bool want_kv, bool want_lam)
+{
+    const c10::DeviceGuard guard(q.device());
+    const AttentionCall c = attention_call(q, k, v, lam, scale, causal, lengths, starts, key_mask);
+    const mam_diff_attention_t &a = c.a;
+    TORCH_CHECK(out.sizes() == at::IntArrayRef({a.B, a.Lq, a.H, a.Dv}), "out has the wrong shape");
+    check_like(out, grad, "out");
+    check_like(out2, out, "out2");
+    TORCH_CHECK(out.device() == q.device() && out.scalar_type() == q.scalar_type(), "out must have q's type and device");
+    TORCH_CHECK(out.is_contiguous() && out2.is_contiguous(), "out and out2 must be contiguous");
+    TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                    lse.sizes() == at::IntArrayRef({2, a.B, a.H, a.Lq}),
+                "lse must be a contiguous float32 tensor of (2, batch, heads, queries)");
+    const Tensor g = unit_last(grad);
+    const int64_t strides[3] = {g.stride(0), g.stride(1), g.stride(2)};
+    Tensor dq, dk, dv, dlam;
+    if (want_q) dq = at::empty({a.B, a.Lq, a.H, 2, a.D}, q.options());
+    if (want_kv) {
+        dk = at::empty({a.B, a.Lk, a.Hkv, 2, a.D}, q.options());
+        dv = at::empty({a.B, a.Lk, a.Hkv, a.Dv}, q.options());
+    }
+    if (want_lam) dlam = at::empty({a.H}, lam.options());
+    const Tensor ws = workspace_for(mam_diff_attention_backward_workspace(&a), q);
+    check_rc(mam_diff_attention_backward(&a, g.data_ptr(), strides, out.data_ptr(), out2.data_ptr(), lse.data_ptr<float>(), out_ptr(dq),
+                                         out_ptr(dk), out_ptr(dv), out_ptr(dlam), out_ptr(ws), ws.defined() ? ws.numel() : 0, current_stream(q)),
+             "mam_diff_attention_backward");
+    return {or_empty(dq, q), or_empty(dk, q), or_empty(dv, q), or_empty(dlam, lam)};
+}
+
 // ---- autograd ----
 template <class Signature>
 c10::TypedOperatorHandle<Signature> find(const char *name)
@@ -401,6 +514,61 @@ Tensors add_dropout_layer_norm_autograd(const Tensor &x, const Tensor &residual,
                                                 : join_below(x, residual, weight, bias, p, scale, seed, offset, eps, step, with_stats);
 }
 
+typedef Tensors AttentionSignature(const Tensor &, const Tensor &, const Tensor &, const Tensor &, double, bool, const MaybeTensor &,
+                                   const MaybeTensor &, const MaybeTensor &, bool);
+typedef Tensors AttentionBackwardSignature(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                           const Tensor &, const Tensor &, double, bool, const MaybeTensor &, const MaybeTensor &,
+                                           const MaybeTensor &, bool, bool, bool);
+
+Tensors attention_below(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, double scale, bool causal,
+                        const MaybeTensor &lengths, const MaybeTensor &starts, const MaybeTensor &key_mask, bool with_sums)
+{
+    static const auto op = find<AttentionSignature>("mamtorch_kernel_encoder::diff_attention");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(q, k, v, lam, scale, causal, lengths, starts, key_mask, with_sums);
+}
+
+struct Attention : public Function<Attention> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, double scale,
+                                 bool causal, const MaybeTensor &lengths, const MaybeTensor &starts, const MaybeTensor &key_mask)
+    {
+        Tensors out = attention_below(q, k, v, lam, scale, causal, lengths, starts, key_mask, true);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["q"] = q.requires_grad();
+        ctx->saved_data["k"] = k.requires_grad();
+        ctx->saved_data["v"] = v.requires_grad();
+        ctx->saved_data["lam"] = lam.requires_grad();
+        ctx->save_for_backward({q, k, v, lam, out[0], out[1], out[2], or_none(lengths), or_none(starts), or_none(key_mask)});
+        ctx->mark_non_differentiable({out[1], out[2]});
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        static const auto op = find<AttentionBackwardSignature>("mamtorch_kernel_encoder::diff_attention_backward");
+        variable_list out(9);
+        if (!grads[0].defined()) return out;
+        const variable_list s = ctx->get_saved_variables();
+        const bool q = ctx->saved_data["q"].toBool(), k = ctx->saved_data["k"].toBool(), v = ctx->saved_data["v"].toBool();
+        const bool lam = ctx->saved_data["lam"].toBool();
+        const Tensors g = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(),
+                                  ctx->saved_data["causal"].toBool(), maybe(s[7]), maybe(s[8]), maybe(s[9]), q, k || v, lam);
+        if (q) out[0] = g[0];
+        if (k) out[1] = g[1];
+        if (v) out[2] = g[2];
+        if (lam) out[3] = g[3];
+        return out;
+    }
+};
+
+Tensors diff_attention_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, double scale, bool causal,
+                                const MaybeTensor &lengths, const MaybeTensor &starts, const MaybeTensor &key_mask, bool with_sums)
+{
+    return recording(q, k, v, lam) ? Attention::apply(q, k, v, lam, scale, causal, lengths, starts, key_mask)
+                                   : attention_below(q, k, v, lam, scale, causal, lengths, starts, key_mask, with_sums);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mamtorch_kernel_encoder, m)
@@ -414,10 +582,16 @@ TORCH_LIBRARY(mamtorch_kernel_encoder, m)
     m.def("add_dropout_layer_norm_backward(Tensor grad, Tensor? grad_sum, Tensor s, Tensor? weight, Tensor mean, Tensor rstd, float p, "
           "float scale, int seed, int offset, Tensor? step, bool want_x, bool want_residual, bool want_weight, bool want_bias, "
           "bool weight_is_float) -> Tensor[]");
+    m.def("diff_attention(Tensor q, Tensor k, Tensor v, Tensor lam, float scale, bool causal, Tensor? lengths, Tensor? starts, "
+          "Tensor? key_mask, bool with_sums) -> Tensor[]");
+    m.def("diff_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor lam, Tensor out, Tensor out2, Tensor lse, float scale, "
+          "bool causal, Tensor? lengths, Tensor? starts, Tensor? key_mask, bool want_q, bool want_kv, bool want_lam) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(mamtorch_kernel_encoder, CUDA, m)
 {
+    m.impl("diff_attention", &diff_attention_cuda);
+    m.impl("diff_attention_backward", &diff_attention_backward_cuda);
     m.impl("layer_norm", &layer_norm_cuda);
     m.impl("layer_norm_backward", &layer_norm_backward_cuda);
     m.impl("dropout", &dropout_cuda);
@@ -430,4 +604,5 @@ TORCH_LIBRARY_IMPL(mamtorch_kernel_encoder, Autograd, m)
     m.impl("layer_norm", &layer_norm_autograd);
     m.impl("dropout", &dropout_autograd);
     m.impl("add_dropout_layer_norm", &add_dropout_layer_norm_autograd);
+    m.impl("diff_attention", &diff_attention_autograd);
 }

@@ -3,5 +3,6 @@ halves, and differential attention.  No upstream names (the reference's ViT exam
 examples/vitb16_imagenet1k/utils.py)."""
 from .norm import layer_norm, add_dropout_layer_norm
 from .dropout import dropout
+from .attention import diff_attention
 
-__all__ = ["layer_norm", "add_dropout_layer_norm", "dropout"]
+__all__ = ["layer_norm", "add_dropout_layer_norm", "dropout", "diff_attention"]

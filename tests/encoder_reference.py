@@ -95,3 +95,88 @@ def assert_within(got, want, bound, what):
     assert not bad.any(), "%s: %d of %d outside, worst %.3g of its bound at %s: got %r want %r" % (
         what, int(bad.sum()), bad.numel(), float((off / bound).nan_to_num(nan=float("inf")).max()), bad.nonzero()[0].tolist(),
         got[tuple(bad.nonzero()[0])].item(), want[tuple(bad.nonzero()[0])].item())
+
+
+# ---- differential attention ----
+def seen_keys(batch, queries, keys, causal=False, lengths=None, starts=None, key_mask=None):
+    """bool (batch, queries, keys)"""
+    j, i = torch.arange(keys), torch.arange(queries)
+    seen = torch.ones(batch, queries, keys, dtype=torch.bool)
+    if lengths is not None:
+        seen &= (j[None] < lengths.long().clamp(0, keys)[:, None])[:, None]
+    if key_mask is not None:
+        seen &= key_mask[:, None]
+    if causal:
+        first = torch.full((batch,), keys - queries) if starts is None else starts.long()
+        seen &= j[None, None] <= i[None, :, None] + first[:, None, None]
+    return seen
+
+
+class Attention:
+    """Outputs, gradients and what rounding may cost them, in 64 bits.
+
+    Scores are sums of d products of the operands as they are, exponentials of them err by the scores' absolute error, and a row's
+    normaliser by as much again.  In 16-bit types probabilities, score gradients and the results handed to the backward are rounded to the type."""
+
+    def __init__(self, q, k, v, lam, seen, scale=None, dout=None):
+        dtype, group = q.dtype, q.shape[2] // max(1, k.shape[2])
+        unit = UNIT[dtype] if dtype != torch.float32 else 0.0
+        tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0    # half the spacing of its subnormal numbers
+        self.dtype = dtype
+        d, keys = q.shape[-1], k.shape[1]
+        scale = d ** -0.5 if scale is None else scale
+        live = seen.any(1)                                      # (batch, keys): what no query sees may hold anything
+        k = torch.where(live[:, :, None, None, None], k, torch.zeros((), dtype=dtype))
+        v = torch.where(live[:, :, None, None], v, torch.zeros((), dtype=dtype))
+        q, k, v = q.double().permute(3, 0, 2, 1, 4), k.double().permute(3, 0, 2, 1, 4), v.double().permute(0, 2, 1, 3)
+        k, v = k.repeat_interleave(group, 2), v.repeat_interleave(group, 1)
+        seen = seen[:, None]
+        w = lam.double()[None, :, None, None]
+        s = (q @ k.transpose(-1, -2)) * scale                   # (map, batch, head, query, key)
+        masked = torch.where(seen, s, torch.tensor(-float("inf"), dtype=torch.float64))
+        p = torch.nan_to_num(torch.softmax(masked, -1), nan=0.0) if keys else masked
+        o = p @ v
+        out = o[0] - w * o[1]
+        self.out = out.transpose(1, 2)
+        # errors
+        off = F32 * ((d + 8) * scale * (q.abs() @ k.abs().transpose(-1, -2)) + 8 * s.abs())
+        off = torch.where(seen, off, torch.zeros((), dtype=torch.float64))
+        worst = off.amax(-1, keepdim=True) if keys else off.sum(-1, keepdim=True)
+        share = off + worst + (keys / 16 + 64) * F32 + unit     # relative, of a probability
+        p_off = p * share + tiny * seen
+        o_off = p_off @ v.abs()
+        out_off = o_off[0] + w.abs() * o_off[1] + 8 * F32 * (o[0].abs() + (w * o[1]).abs())
+        self.out_bound = (UNIT[dtype] * out.abs() + out_off + TINY[dtype]).transpose(1, 2)
+        if dout is None:
+            return
+        g = dout.double().transpose(1, 2)
+        da = g @ v.transpose(-1, -2)
+        delta = (g[None] * o).sum(-1, keepdim=True)
+        dp = torch.stack((da, -w * da))
+        ds = torch.stack((p[0] * (da - delta[0]), -w * p[1] * (da - delta[1])))
+        dq, dk = ds @ k * scale, ds.transpose(-1, -2) @ q * scale
+        a = p[0] - w * p[1]
+        dv = a.transpose(-1, -2) @ g
+        del dp
+        dv_size = v.shape[-1]
+        da_off = F32 * (dv_size + 8) * (g.abs() @ v.abs().transpose(-1, -2))
+        # d1 and d2 from the results as they are kept: rounded to the type
+        kept = torch.stack((UNIT[dtype] * (out.abs() + 2 * (w * o[1]).abs()) + out_off + w.abs() * o_off[1], UNIT[dtype] * o[1].abs() + o_off[1]))
+        delta_off = (g.abs()[None] * (kept + F32 * (dv_size + 8) * (o.abs() + out.abs()[None]))).sum(-1, keepdim=True)
+        size = torch.stack((torch.ones_like(p[0]), w.abs() * torch.ones_like(p[0])))
+        diff = torch.stack((da - delta[0], da - delta[1]))
+        ds_off = size * (p_off * (diff.abs() + da_off + delta_off) + p * (da_off + delta_off)) + (unit + 16 * F32) * ds.abs() + tiny * seen
+        a_off = p_off[0] + w.abs() * p_off[1] + (unit + 4 * F32) * a.abs() + tiny * seen
+        rows = (q.shape[-2] * group / 16 + 64) * F32
+        dq_off = scale * ((ds_off + (keys / 16 + 64) * F32 * ds.abs()) @ k.abs())
+        dk_off = scale * ((ds_off + rows * ds.abs()).transpose(-1, -2) @ q.abs())
+        dv_off = (a_off + rows * a.abs()).transpose(-1, -2) @ g.abs()
+        heads = lambda t: t.unflatten(-3, (-1, group)).sum(-3) if t.shape[-3] else t        # noqa: E731  (shared heads' gradients)
+        final = lambda t, t_off: (t, UNIT[dtype] * t.abs() + t_off + TINY[dtype])           # noqa: E731
+        self.dq, self.dq_bound = (t.permute(1, 3, 2, 0, 4) for t in final(dq, dq_off))
+        self.dk, self.dk_bound = (t.permute(1, 3, 2, 0, 4) for t in final(heads(dk), heads(dk_off)))
+        self.dv, self.dv_bound = (t.transpose(1, 2) for t in final(heads(dv), heads(dv_off)))
+        self.dlam = -delta[1].sum((0, 2, 3))
+        count = q.shape[1] * q.shape[-2]
+        lam_off = delta_off[1].sum((0, 2, 3)) + (count / 1024 + 32) * F32 * delta[1].abs().sum((0, 2, 3))
+        self.dlam_bound = UNIT[lam.dtype] * self.dlam.abs() + lam_off + TINY[lam.dtype]

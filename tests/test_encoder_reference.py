@@ -82,3 +82,47 @@ def test_fake_kernels_propagate_shapes_and_types():
         assert ops.dropout(x, x, 0.1, 1.0, 1, 2, None).shape == x.shape
         y, s, mean, _ = ops.add_dropout_layer_norm(x, x, None, None, 0.1, 1.0, 1, 2, 1e-5, None, False)
         assert y.shape == s.shape == x.shape and mean.numel() == 0
+
+
+def test_attention_gradients_agree_with_differences():
+    g = torch.Generator().manual_seed(1)
+    q, k, v, lam, dout = (torch.randn(*s, generator=g).double() for s in ((2, 3, 4, 2, 5), (2, 6, 2, 2, 5), (2, 6, 2, 7), (4,), (2, 3, 4, 7)))
+    ref.UNIT[torch.float64], ref.TINY[torch.float64] = 2.0 ** -53, 0.0
+    seen = ref.seen_keys(2, 3, 6, causal=True, lengths=torch.tensor([6, 2]), starts=torch.tensor([2, -1]))
+    assert seen[1, 0].sum() == 0 and seen[0, 0].sum() == 3
+    want = ref.Attention(q, k, v, lam, seen, None, dout)
+    f = lambda: (ref.Attention(q, k, v, lam, seen).out * dout).sum().item()         # noqa: E731
+    h = 1e-6
+    for t, grad in ((q, want.dq), (k, want.dk), (v, want.dv), (lam, want.dlam)):
+        flat, grad = t.reshape(-1), grad.reshape(-1)
+        for i in range(0, t.numel(), 7):
+            at = flat[i].item()
+            flat[i] = at + h
+            up = f()
+            flat[i] = at - h
+            down = f()
+            flat[i] = at
+            assert abs((up - down) / (2 * h) - grad[i].item()) < 1e-7
+
+
+def test_the_attention_entry_points_refuse_what_they_do_not_cover():
+    l = capi.lib()
+
+    def call(**changes):
+        a = capi.DiffAttention(q=256, k=256, v=256, lam=256, B=1, Lq=2, Lk=2, H=2, Hkv=1, D=8, Dv=8, scale=1.0)
+        for n, v in changes.items():
+            setattr(a, n, v)
+        one = ctypes.c_void_p(256)
+        forward = l.mam_diff_attention(a, None if changes.get("no_out") else one, None, None, None, 0, None)
+        strides = (ctypes.c_int64 * 3)(16, 8, 8)
+        backward = l.mam_diff_attention_backward(a, one, strides, None if changes.get("no_out") else one, one, one, one, one, one, one, None, 0, None)
+        return forward, backward
+
+    assert call(B=-1) == call(Lk=-1) == call(Hkv=0) == call(H=3, Hkv=2) == call(type=9) == call(lam_type=1) == (-1, -1)
+    assert call(scale=0.0) == call(scale=float("nan")) == call(scale=float("inf")) == call(scale=-2.0) == (-1, -1)
+    assert call(D=129) == call(D=0) == call(Dv=257) == call(B=2 ** 31) == call(Lq=2 ** 30) == (-2, -2)
+    assert call(q=None) == call(k=None) == call(v=None) == call(lam=None) == call(no_out=True) == (-1, -1)
+    assert call(B=0)[0] == 0
+    a = capi.DiffAttention(q=256, k=256, v=256, lam=256, B=1, Lq=2, Lk=2, H=2, Hkv=1, D=8, Dv=8, scale=1.0)
+    assert l.mam_diff_attention_backward_workspace(a) == 5 * 4 * 4
+    assert l.mam_diff_attention(None, None, None, None, None, 0, None) == -1
