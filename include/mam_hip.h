@@ -539,18 +539,18 @@ typedef struct mam_diff_attention_t {
     int causal, type, lam_type;
 } mam_diff_attention_t;
 
-/* out (B, Lq, H, Dv) contiguous; for the backward: out2 (like out, P2 V) and lse (2, B, H, Lq) fp32 (log2 of each row's sum of
- * exponentials, +inf where it sees no key), or NULL.  The workspace (of the sizes; 0 for most calls) holds partial results where the keys of few
+/* out (B, Lq, H, Dv) contiguous; for the backward, or NULL: kept, fp32 planes of out's shape (one for fp32 operands, P2 V; two for 16-bit
+ * operands, P2 V and P1 V), and lse (2, B, H, Lq) fp32, log2 of each row's sum of exponentials, +inf where it sees no key.  The workspace (of the sizes; 0 for most calls) holds partial results where the keys of few
  * queries are split over workgroups. */
 size_t mam_diff_attention_workspace(const mam_diff_attention_t *args);
-int mam_diff_attention(const mam_diff_attention_t *args, void *out, void *out2, float *lse, void *workspace, size_t workspace_bytes,
+int mam_diff_attention(const mam_diff_attention_t *args, void *out, float *kept, float *lse, void *workspace, size_t workspace_bytes,
                        void *stream);
-/* Gradients from dout (B, Lq, H, Dv; strides of batch, token, head in HOST memory, last dimension 1) and the forward's out, out2 and lse:
+/* Gradients from dout (B, Lq, H, Dv; strides of batch, token, head in HOST memory, last dimension 1) and the forward's out, kept and lse:
  * dq (B, Lq, H, 2, D), dk (B, Lk, Hkv, 2, D), dv (B, Lk, Hkv, Dv), dlam (H, of lam_type), contiguous, fully written (zeros where a key is
  * not seen); each may be NULL.  Deterministic. */
 size_t mam_diff_attention_backward_workspace(const mam_diff_attention_t *args);
 int mam_diff_attention_backward(const mam_diff_attention_t *args, const void *dout, const int64_t *dout_stride, const void *out,
-                                const void *out2, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
+                                const float *kept, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
                                 size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

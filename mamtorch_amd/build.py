@@ -18,7 +18,8 @@ OPS_LIB = os.path.join(LIB_DIR, "mam_torch_ops.so")
 
 HIP_SOURCES = ["mam_common.hip", "mam_forward.hip", "mam_ordered.hip", "mam_backward.hip", "mam_selcount.hip", "mam_csr.hip",
                "mam_spmm.hip", "mam_prune.hip", "mam_select.hip", "mam_module.hip", "mam_dropout.hip",
-               "mam_norm.hip", "mam_attention.hip", "mam_attention_backward.hip"]
+               "mam_norm.hip", "mam_attention.hip", "mam_attention_backward.hip",
+               "mam_attention_split.hip"]
 
 # -ffp-contract=off: a product that feeds an add must stay an fp32 multiply followed by an fp32
 # add (bit-exact forward).  Packed-FP32 instructions are disabled for the device pass.

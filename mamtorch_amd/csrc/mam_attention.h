@@ -26,7 +26,8 @@ struct Call {
     int64_t mask_b;
     int B, Lq, Lk, H, Hkv, G, d, dv, causal, lam_same;
     int R;              // rows of a key head: Lq * G
-    float scale;
+    float scale, inverse;
+    bool fast;          // k and v may be read by Stage<..., FAST>, and q too; no mask
 };
 
 // What rows of batch b see: keys below `keys`, and with a causal limit those up to query + first.
@@ -57,6 +58,16 @@ template <class T>
 __device__ __forceinline__ float lambda_of(const Call &a, int head, const T *)
 {
     return a.lam_same ? (float)static_cast<const T *>(a.lam)[head] : static_cast<const float *>(a.lam)[head];
+}
+
+// The tile that a workgroup takes: workgroups of one turn are those of all (request, key head) pairs, which follow each other on the XCDs, so that where there are a
+// multiple of 8 of them a head's workgroups meet in one L2.  A causal call's tiles differ in length, from the last rows (the first keys) on;
+// the longest begin first.  Where the device holds all workgroups at once, two a CU, the second half takes the shortest first, so that a CU has a long and a short one.
+__device__ __forceinline__ int tile_of_turn(int turn, int tiles, bool last_first, int workgroups)
+{
+    const int half = (tiles + 1) / 2;
+    const int order = workgroups <= 2 * kNumCU && turn >= half ? tiles - 1 - (turn - half) : turn;
+    return last_first ? tiles - 1 - order : order;
 }
 
 // ---- matrix-core tiles ----
@@ -114,11 +125,20 @@ __device__ __forceinline__ int lane_group() { return (threadIdx.x & 63) / TR; }
 template <int TR>
 __device__ __forceinline__ int index_of(int f) { return (f / 4) * 4 * GROUPS<TR> + 4 * lane_group<TR>() + f % 4; }
 
+// Where row `row` of a tile stands in LDS.  A pitch is 4 words more than a multiple of 32, so rows that follow each other are 4 banks apart: right for
+// the 16-byte reads of 16 rows.  The transposing read takes 4 rows of 16 words at a time: 4 consecutive ones stand 4 rows, 16 banks, apart.  fp32 columns
+// are read a row a lane group and have their rows in order.  (Rows in order in all types: profiles count 3 cycles of conflicts for one of reads.)
+template <class T>
+__device__ __forceinline__ int place_of(int row)
+{
+    return sizeof(T) == 2 ? (row & ~15) | (row & 3) << 2 | (row >> 2 & 3) : row;
+}
+
 // Fragment of a row of LDS: terms kk * KS .. of row `row`.
 template <class T, int TR>
 __device__ __forceinline__ Frag<T> row_frag(const T *tile, int pitch, int row, int kk)
 {
-    return *reinterpret_cast<const Frag<T> *>(tile + row * pitch + kk * KS<T, TR> + FE<T> * lane_group<TR>());
+    return *reinterpret_cast<const Frag<T> *>(tile + place_of<T>(row) * pitch + kk * KS<T, TR> + FE<T> * lane_group<TR>());
 }
 
 // Fragment j of the columns col .. col + TR - 1 of 32 rows of LDS, taken as the contraction's terms in the accumulators' order.
@@ -131,9 +151,10 @@ __device__ __forceinline__ Frag<T> column_frag(const T *tile, int pitch, int col
         typedef short quad __attribute__((ext_vector_type(4)));
         typedef short octet __attribute__((ext_vector_type(8)));
         typedef __attribute__((address_space(3))) quad *lds_quad;
-        const T *p = tile + (8 * GROUPS<TR> * j + 4 * lane_group<TR>() + (lane % 16) / 4) * pitch + col + 16 * ((lane % TR) / 16) + 4 * (lane % 4);
+        const T *p = tile + place_of<T>(8 * GROUPS<TR> * j + 4 * lane_group<TR>() + (lane % 16) / 4) * pitch + col + 16 * ((lane % TR) / 16) + 4 * (lane % 4);
         const quad lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)p);
-        const quad hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(p + 4 * GROUPS<TR> * pitch));
+        // 4 * GROUPS rows on: 8 rows (two lane groups of 4) stand 2 rows on, 16 stand 16 rows on
+        const quad hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(p + (TR == 32 ? 2 : 16) * pitch));
         const octet all = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(Frag<T>, all);
     } else {
@@ -155,19 +176,63 @@ __device__ __forceinline__ void to_frags(const float (&p)[REGS<TR>], Frag<T> (&f
         for (int u = 0; u < FE<T>; ++u) f[j][u] = (T)p[j * FE<T> + u];
 }
 
-// Maximum and sum over the lane groups that hold a row's values.
+// Has elements u and u + 1 of a fragment made here and not where they are used, behind a later branch.
+template <class F>
+__device__ __forceinline__ void keep_here(F &f, int u)
+{
+    constexpr int SIZE = sizeof(f[0]);
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    words w = __builtin_bit_cast(words, f);
+#pragma unroll
+    for (int i = u * SIZE / 4; i < (u + 2) * SIZE / 4; ++i) {
+        uint32_t t = w[i];
+        asm volatile("" : "+v"(t));
+        w[i] = t;
+    }
+    f = __builtin_bit_cast(F, w);
+}
+
+// Element u of a fragment in fp32, from the words that hold it.
+__device__ __forceinline__ float element(const Frag<bf16> &f, int u)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    const words w = __builtin_bit_cast(words, f);
+    return __uint_as_float(u & 1 ? w[u / 2] & 0xffff0000u : w[u / 2] << 16);
+}
+__device__ __forceinline__ float element(const Frag<f16> &f, int u) { return (float)f[u]; }
+__device__ __forceinline__ float element(const Frag<float> &f, int u) { return f[u]; }
+
+// Maximum and sum over the lane groups that hold a row's values: the halves (quarters) of a wave meet by vector instructions that
+// swap them, not through LDS.  Of a value swapped with itself the two results are one half's and the other's.
+typedef uint32_t Halves __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ Halves halves(float v)
+{
+    return __builtin_bit_cast(Halves, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
+__device__ __forceinline__ Halves quarters(float v)
+{
+    return __builtin_bit_cast(Halves, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
 template <int TR>
 __device__ __forceinline__ float groups_max(float v)
 {
-    v = fmaxf(v, __shfl_xor(v, 32));
-    if constexpr (TR == 16) v = fmaxf(v, __shfl_xor(v, 16));
+    Halves t = halves(v);
+    v = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+    if constexpr (TR == 16) {
+        t = quarters(v);
+        v = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+    }
     return v;
 }
 template <int TR>
 __device__ __forceinline__ float groups_sum(float v)
 {
-    v += __shfl_xor(v, 32);
-    if constexpr (TR == 16) v += __shfl_xor(v, 16);
+    Halves t = halves(v);
+    v = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    if constexpr (TR == 16) {
+        t = quarters(v);
+        v = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    }
     return v;
 }
 
@@ -178,6 +243,7 @@ struct Source {
     const T *base;
     int64_t row, head, map;     // strides; a row's head is its number modulo G
     int G, width;
+    float inverse;              // 1 / G
     __device__ __forceinline__ const T *at(int r, int m) const
     {
         const int64_t off = G == 1 ? (int64_t)r * row : (int64_t)(r / G) * row + (int64_t)(r % G) * head;
@@ -201,36 +267,88 @@ __device__ __forceinline__ Frag<T> load_frag(const T *p, int left)
     return r;
 }
 
+// 16 bytes at a 32-bit offset from a uniform base; an offset of NOWHERE reads nothing and gives zeros (the buffer's own bounds check).
+constexpr uint32_t NOWHERE = 0x80000000u;
+template <class T>
+__device__ __forceinline__ Frag<T> buffer_frag(const T *base, uint32_t offset)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, 0x7fffffff, 0x00027000);
+    const words w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)offset, 0, 0);
+    return __builtin_bit_cast(Frag<T>, w);
+}
+
 // ROWS rows of MAPS segments of W elements between global memory and LDS by THREADS threads, in 16-byte pieces that stay in
-// registers between load() and store().
-template <class T, int THREADS, int ROWS, int MAPS, int W>
+// registers between load() and store().  FAST: widths are whole pieces, addresses and strides multiples of 16 bytes, a tile's rows
+// within 2^30 bytes and all rows below an end are there, so that a piece is one buffer load whatever of it is there; else element by element
+// where a row ends inside a piece, and rows that are there by a test of each.
+template <class T, int THREADS, int ROWS, int MAPS, int W, bool FAST>
 struct Stage {
-    static constexpr int PER = MAPS * W / FE<T>, PIECES = ROWS * PER, N = (PIECES + THREADS - 1) / THREADS;
+    static constexpr int PER = W / FE<T>, SEGMENT = ROWS * PER, PIECES = MAPS * SEGMENT, N = PIECES / THREADS;
     static constexpr int PITCH = MAPS * W + FE<T>;
+    static_assert(PIECES % THREADS == 0 && SEGMENT % 64 == 0, "whole pieces a thread, a segment a wave");
     Frag<T> piece[N];
 
-    // `there(row)`: whether a row is read or taken as zeros
+    static __device__ __forceinline__ uint32_t map_of(int i)
+    {
+        return MAPS == 1 ? 0 : (i * THREADS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64u) / SEGMENT;
+    }
+    static __device__ __forceinline__ int row_of(int i) { return (int)((i * THREADS + threadIdx.x) % SEGMENT / PER); }
+    static __device__ __forceinline__ int column_of(int i) { return (int)((i * THREADS + threadIdx.x) % SEGMENT % PER * FE<T>); }
+
+    // Rows first .. of the source; those from `end` on, and those that `there` denies (slow loads only), are zeros.
     template <class There>
-    __device__ __forceinline__ void load(const Source<T> &src, int first, const There &there)
+    __device__ __forceinline__ void load(const Source<T> &src, int first, int end, const There &there)
+    {
+        if constexpr (FAST) {
+            const int left = end - first;
+            if (src.G == 1) {
+                const T *base = src.base + (int64_t)first * src.row;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint32_t off = ((uint32_t)row_of(i) * (uint32_t)src.row + (uint32_t)column_of(i)) * (uint32_t)sizeof(T);
+                    piece[i] = buffer_frag<T>(base + map_of(i) * src.map, row_of(i) < left && column_of(i) < src.width ? off : NOWHERE);
+                }
+            } else {            // heads of a shared key head: rows of a token are its heads
+                const int token = first / src.G, turn = first - token * src.G;
+                const T *base = src.base + (int64_t)token * src.row;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int t = turn + row_of(i), more = (int)(((float)t + 0.5f) * src.inverse);
+                    const uint32_t off = (uint32_t)more * (uint32_t)src.row + (uint32_t)(t - more * src.G) * (uint32_t)src.head + (uint32_t)column_of(i);
+                    piece[i] = buffer_frag<T>(base + map_of(i) * src.map,
+                                              row_of(i) < left && column_of(i) < src.width ? off * (uint32_t)sizeof(T) : NOWHERE);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int row = first + row_of(i), c = column_of(i);
+#pragma unroll
+                for (int u = 0; u < FE<T>; ++u) piece[i][u] = (T)0.0f;
+                if (row < end && c < src.width && there(row)) piece[i] = load_frag<T>(src.at(row, map_of(i)) + c, src.width - c);
+            }
+        }
+    }
+    __device__ __forceinline__ void clear()
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * THREADS + threadIdx.x, row = id / PER, col = id % PER * FE<T>, c = col % W;
-            const bool ok = (PIECES % THREADS == 0 || id < PIECES) && c < src.width && there(first + row);
+        for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int u = 0; u < FE<T>; ++u) piece[i][u] = (T)0.0f;
-            if (ok) piece[i] = load_frag<T>(src.at(first + row, col / W) + c, src.width - c);
-        }
     }
     __device__ __forceinline__ void store(T *tile) const
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * THREADS + threadIdx.x, row = id / PER, col = id % PER * FE<T>;
-            if (PIECES % THREADS == 0 || id < PIECES) *reinterpret_cast<Frag<T> *>(tile + row * PITCH + col) = piece[i];
-        }
+        for (int i = 0; i < N; ++i) *reinterpret_cast<Frag<T> *>(tile + place_of<T>(row_of(i)) * PITCH + map_of(i) * W + column_of(i)) = piece[i];
     }
 };
+
+constexpr int KT = 32;          // rows of a tile in LDS
+
+// Tiles in LDS: two where two workgroups still fit a CU, so that a tile is written while the last one is read.
+template <class T, int D, int DV>
+constexpr int TILES = 2 * KT * (2 * D + DV + 2 * FE<T>) * (int)sizeof(T) + 2 * 5 * KT * 4 <= 80 * 1024 ? 2 : 1;
 
 // A wave's own TR rows as the fragments of a contraction over their W elements.
 template <class T, int TR, int W>
@@ -267,11 +385,30 @@ int with_head_sizes(int d, int dv, const F &f)
     return f.template operator()<128, 256>();
 }
 
-// Rows of a wave's tile.
-template <int D, int DV>
-constexpr int TILE_ROWS = D > 64 ? 16 : 32;
+// Rows of a wave's tile.  fp32 products take 8 times as long for the bytes that they read of LDS, so tiles of 16 rows keep the matrix cores as busy
+// and take half the registers; in 16-bit types 32 rows halve the reads, while the accumulators fit two waves a SIMD.
+template <class T, int D>
+constexpr int TILE_ROWS = sizeof(T) == 4 || D > 64 ? 16 : 32;
+
+// Whether every operand can be read in whole 16-byte pieces at 32-bit offsets from its tiles (Stage).
+inline bool fast_operand(const void *p, int64_t size, int width, int64_t batch, int64_t row, int64_t head, int64_t map, int64_t heads)
+{
+    const int64_t pack = 16 / size;
+    return (uintptr_t)p % 16 == 0 && width % pack == 0 && batch % pack == 0 && row % pack == 0 && head % pack == 0 && map % pack == 0 && row >= 0 &&
+           head >= 0 && map >= 0 && row <= (int64_t)1 << 22 && head * heads <= (int64_t)1 << 26;
+}
+
+// Planes of fp32 that the backward reads of the forward's products: the second map's, from which and the result the first's follows in fp32; in
+// 16-bit types the first's too, since the result's rounding would enter every score gradient of its row.
+template <class T>
+constexpr int KEPT = sizeof(T) == 2 ? 2 : 1;
 
 int fill_call(const mam_diff_attention_t *a, Call &c);
+
+// Few queries over many keys (mam_attention_split.hip): whether a call runs there, its workspace, and the call.
+bool use_split(const Call &a, bool keep);
+size_t split_workspace(const Call &a);
+int run_split(const Call &a, int type, void *out, void *workspace, size_t workspace_bytes, hipStream_t st);
 
 }  // namespace attention
 }  // namespace mam

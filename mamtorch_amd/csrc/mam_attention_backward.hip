@@ -12,16 +12,17 @@
 namespace mam {
 namespace attention {
 
-constexpr int STEP = 32;        // keys (dQ) or rows (dK, dV) of a tile
+constexpr int STEP = KT;        // keys (dQ) or rows (dK, dV) of a tile
 
 // What a row brings beside its query: five planes of B * Hkv * R floats.
 enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, PLANES };
 
 struct BackwardCall {
     Call a;
-    const void *dout, *out, *out2;      // dout strided, out and out2 contiguous (B, Lq, H, dv)
+    const void *dout, *out;             // dout strided, out contiguous (B, Lq, H, dv)
     int64_t gb, gl, gh;
-    const float *lse;
+    const float *kept, *lse;            // KEPT<T> planes like out
+    bool fast;                          // dout may be read by Stage<..., FAST> like the operands
     void *dq, *dk, *dv, *dlam;
     float *rows;                        // PLANES planes
 };
@@ -37,13 +38,14 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     const int query = row / a.G, head = bh % a.Hkv * a.G + row % a.G;
     const T *grad = static_cast<const T *>(g.dout) + b * g.gb + query * g.gl + head * g.gh;
     const int64_t at = (((int64_t)b * a.Lq + query) * a.H + head) * a.dv;
-    const T *out = static_cast<const T *>(g.out) + at, *out2 = static_cast<const T *>(g.out2) + at;
+    const int64_t plane = (int64_t)a.B * a.Lq * a.H * a.dv;
     float dot = 0.0f, dot2 = 0.0f;
     for (int c = lane * kPack<T>; c < a.dv; c += 16 * kPack<T>) {
         float v[kPack<T>], o[kPack<T>], o2[kPack<T>];
         load_pack<T>(grad + c, a.dv - c, v);
-        load_pack<T>(out + c, a.dv - c, o);
-        load_pack<T>(out2 + c, a.dv - c, o2);
+        if (KEPT<T> == 2) load_pack<float, kPack<T>>(g.kept + plane + at + c, a.dv - c, o);
+        else load_pack<T>(static_cast<const T *>(g.out) + at + c, a.dv - c, o);
+        load_pack<float, kPack<T>>(g.kept + at + c, a.dv - c, o2);
 #pragma unroll
         for (int u = 0; u < kPack<T>; ++u) {
             dot = fmaf(v[u], o[u], dot);
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     const int64_t sums = ((int64_t)b * a.H + head) * a.Lq + query;
     g.rows[MINUS_SUM1 * count + id] = -g.lse[sums];
     g.rows[MINUS_SUM2 * count + id] = -g.lse[(int64_t)a.B * a.H * a.Lq + sums];
-    g.rows[DOT1 * count + id] = fmaf(lam, dot2, dot);       // O1 = out + lambda O2
+    g.rows[DOT1 * count + id] = KEPT<T> == 2 ? dot : fmaf(lam, dot2, dot);      // O1 = out + lambda O2
     g.rows[DOT2 * count + id] = dot2;
     g.rows[LAMBDA * count + id] = lam;
 }
@@ -90,6 +92,14 @@ __global__ __launch_bounds__(1024) void lambda_kernel(const BackwardCall g)
     else static_cast<float *>(g.dlam)[head] = sum;
 }
 
+// Waves of a SIMD that the registers are shared between: a lane holds its wave's operands and gradients, and 48 of scores.
+template <class T, int TR, int D, int DV>
+constexpr int OPERANDS = (2 * D + DV) * TR * (int)sizeof(T) / 256;
+template <class T, int TR, int D, int DV>
+constexpr int QUERIES_WAVES = OPERANDS<T, TR, D, DV> + D * TR / 32 <= 128 ? 2 : 1;
+template <class T, int TR, int D, int DV>
+constexpr int KEYS_WAVES = OPERANDS<T, TR, D, DV> + D * TR / 32 + DV * TR / 64 <= 128 ? 2 : 1;
+
 template <int TR>
 __device__ __forceinline__ void clear(Acc<TR> &c)
 {
@@ -111,20 +121,19 @@ __device__ __forceinline__ void store_columns(T *p, int left, const Acc<TR> &c, 
     }
 }
 
-template <class T, int TR, int D, int DV>
-__global__ __launch_bounds__(256, 1) void queries_kernel(const BackwardCall g, int row_tiles)
+template <class T, int TR, int D, int DV, bool FAST>
+__global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_kernel(const BackwardCall g, int row_tiles)
 {
-    constexpr int ROWS = 4 * TR;
-    typedef Stage<T, 256, STEP, 2, D> StageK;
-    typedef Stage<T, 256, STEP, 1, DV> StageV;
-    __shared__ __attribute__((aligned(16))) T k_tile[STEP * StageK::PITCH];
-    __shared__ __attribute__((aligned(16))) T v_tile[STEP * StageV::PITCH];
+    constexpr int ROWS = 4 * TR, BUFFERS = TILES<T, D, DV>;
+    typedef Stage<T, 256, STEP, 2, D, FAST> StageK;
+    typedef Stage<T, 256, STEP, 1, DV, FAST> StageV;
+    __shared__ __attribute__((aligned(16))) T k_tile[BUFFERS][STEP * StageK::PITCH];
+    __shared__ __attribute__((aligned(16))) T v_tile[BUFFERS][STEP * StageV::PITCH];
     const Call &a = g.a;
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int bh = id / row_tiles, tile = row_tiles - 1 - id % row_tiles;
+    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, row_tiles, true, gridDim.x);
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
     const Reach reach = reach_of(a, b);
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = tile * ROWS + wave * TR, row = first + lane_row<TR>();
     const bool there = row < a.R;
     const int query = there ? row / a.G : 0, head = hk * a.G + (there ? row - query * a.G : 0);
@@ -134,10 +143,10 @@ __global__ __launch_bounds__(256, 1) void queries_kernel(const BackwardCall g, i
     const int last = tile * ROWS + ROWS - 1 < a.R ? tile * ROWS + ROWS - 1 : a.R - 1;
     const int end = reach.of_query(last / a.G);
 
-    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d};
-    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv};
-    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d};
-    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv};
+    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
+    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv, a.inverse};
+    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d, 1.0f};
+    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv, 1.0f};
     Frag<T> q[2][D / KS<T, TR>], grad[DV / KS<T, TR>];
 #pragma unroll
     for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
@@ -153,58 +162,79 @@ __global__ __launch_bounds__(256, 1) void queries_kernel(const BackwardCall g, i
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int blk = 0; blk < D / TR; ++blk) clear<TR>(dq[m][blk]);
-    const auto seen = [&](int key) { return key < end && (!a.mask || a.mask[b * a.mask_b + key] != 0); };
+    const auto seen = [&](int key) { return !a.mask || a.mask[b * a.mask_b + key] != 0; };
     StageK k_stage;
     StageV v_stage;
-    k_stage.load(ks, 0, seen);
-    v_stage.load(vs, 0, seen);
-    for (int key = 0; key < end; key += STEP) {
-        __syncthreads();
-        k_stage.store(k_tile);
-        v_stage.store(v_tile);
-        __syncthreads();
-        if (key + STEP < end) {
-            k_stage.load(ks, key + STEP, seen);
-            v_stage.load(vs, key + STEP, seen);
+    k_stage.load(ks, 0, end, seen);
+    v_stage.load(vs, 0, end, seen);
+    if (BUFFERS == 2) {
+        k_stage.store(k_tile[0]);
+        v_stage.store(v_tile[0]);
+    }
+    // a tile's part of the loop, and a wave that is past its keys in a loop of its own, as in the forward
+    int at = 0;
+    const auto tile_of = [&](int key, const auto &use) {
+        const bool more = key + STEP < end;
+        if (BUFFERS == 1) {
+            __syncthreads();
+            k_stage.store(k_tile[0]);
+            v_stage.store(v_tile[0]);
         }
-        if (key >= wave_any) continue;
-        const bool limited = key + STEP > wave_all || a.mask;
-        const uint32_t word = a.mask ? mask_word(a, b, key) : 0xffffffffu;
-        Acc<TR> da[BLOCKS<TR>];
-#pragma unroll
-        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-            clear<TR>(da[blk]);
-#pragma unroll
-            for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
-                mma<TR>(row_frag<T, TR>(v_tile, StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
+        if (more) {
+            k_stage.load(ks, key + STEP, end, seen);
+            v_stage.load(vs, key + STEP, end, seen);
         }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            float ds[REGS<TR>];
+        __syncthreads();
+        use();
+        if (BUFFERS == 2) {
+            at ^= 1;
+            if (more) {
+                k_stage.store(k_tile[at]);
+                v_stage.store(v_tile[at]);
+            }
+        }
+    };
+    int key = 0;
+    for (; key < wave_any; key += STEP)
+        tile_of(key, [&] {
+            const bool limited = key + STEP > wave_all || (!FAST && a.mask);
+            const uint32_t word = !FAST && a.mask ? mask_word(a, b, key) : 0xffffffffu;
+            Acc<TR> da[BLOCKS<TR>];
 #pragma unroll
             for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-                Acc<TR> s;
-                clear<TR>(s);
+                clear<TR>(da[blk]);
 #pragma unroll
-                for (int kk = 0; kk < D / KS<T, TR>; ++kk)
-                    mma<TR>(row_frag<T, TR>(k_tile + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
-#pragma unroll
-                for (int i = 0; i < TR * TR / 64; ++i) {
-                    const int f = blk * (TR * TR / 64) + i, at = index_of<TR>(f);
-                    float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
-                    if (limited && !(at < limit - key && (word >> at & 1))) p = 0.0f;
-                    ds[f] = weight[m] * p * (da[blk][i] - dot[m]);
-                }
+                for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
+                    mma<TR>(row_frag<T, TR>(v_tile[at], StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
             }
-            Frag<T> frag[FRAGS<T, TR>];
-            to_frags<T, TR>(ds, frag);
 #pragma unroll
-            for (int blk = 0; blk < D / TR; ++blk)
+            for (int m = 0; m < 2; ++m) {
+                float ds[REGS<TR>];
 #pragma unroll
-                for (int j = 0; j < FRAGS<T, TR>; ++j)
-                    mma<TR>(column_frag<TR>(k_tile + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
-        }
-    }
+                for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+                    Acc<TR> s;
+                    clear<TR>(s);
+#pragma unroll
+                    for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+                        mma<TR>(row_frag<T, TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
+#pragma unroll
+                    for (int i = 0; i < TR * TR / 64; ++i) {
+                        const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
+                        float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
+                        if (limited && !(n < limit - key && (FAST || (word >> n & 1)))) p = 0.0f;
+                        ds[f] = weight[m] * p * (da[blk][i] - dot[m]);
+                    }
+                }
+                Frag<T> frag[FRAGS<T, TR>];
+                to_frags<T, TR>(ds, frag);
+#pragma unroll
+                for (int blk = 0; blk < D / TR; ++blk)
+#pragma unroll
+                    for (int j = 0; j < FRAGS<T, TR>; ++j)
+                        mma<TR>(column_frag<TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
+            }
+        });
+    for (; key < end; key += STEP) tile_of(key, [] {});
     if (!there) return;
     T *out = static_cast<T *>(g.dq) + (((int64_t)b * a.Lq + query) * a.H + head) * 2 * a.d;
 #pragma unroll
@@ -213,21 +243,20 @@ __global__ __launch_bounds__(256, 1) void queries_kernel(const BackwardCall g, i
         for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dq[m][blk], a.scale);
 }
 
-template <class T, int TR, int D, int DV>
-__global__ __launch_bounds__(256, 1) void keys_kernel(const BackwardCall g, int key_tiles)
+template <class T, int TR, int D, int DV, bool FAST>
+__global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(const BackwardCall g, int key_tiles)
 {
-    constexpr int KEYS = 4 * TR;
-    typedef Stage<T, 256, STEP, 2, D> StageQ;
-    typedef Stage<T, 256, STEP, 1, DV> StageG;
-    __shared__ __attribute__((aligned(16))) T q_tile[STEP * StageQ::PITCH];
-    __shared__ __attribute__((aligned(16))) T g_tile[STEP * StageG::PITCH];
-    __shared__ __attribute__((aligned(16))) float planes[PLANES][STEP];
+    constexpr int KEYS = 4 * TR, BUFFERS = TILES<T, D, DV>;
+    typedef Stage<T, 256, STEP, 2, D, FAST> StageQ;
+    typedef Stage<T, 256, STEP, 1, DV, FAST> StageG;
+    __shared__ __attribute__((aligned(16))) T q_tile[BUFFERS][STEP * StageQ::PITCH];
+    __shared__ __attribute__((aligned(16))) T g_tile[BUFFERS][STEP * StageG::PITCH];
+    __shared__ __attribute__((aligned(16))) float planes[BUFFERS][PLANES][STEP];
     const Call &a = g.a;
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int bh = id / key_tiles, tile = id % key_tiles;      // the first keys, which most rows of a causal call see, begin first
+    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, gridDim.x);
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
     const Reach reach = reach_of(a, b);
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = tile * KEYS + wave * TR, key = first + lane_row<TR>();
     // rows that see a key begin at (key - reach.first) * G; past every row where none does
     const auto from = [&](int k) {
@@ -241,10 +270,10 @@ __global__ __launch_bounds__(256, 1) void keys_kernel(const BackwardCall g, int 
     const int wave_all = first + TR <= reach.keys && !a.mask ? from(first + TR - 1) : a.R;    // from here on every lane's key is seen
     const int begin = tile * KEYS < reach.keys ? from(tile * KEYS) / STEP * STEP : a.R;
 
-    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d};
-    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv};
-    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d};
-    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv};
+    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
+    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv, a.inverse};
+    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d, 1.0f};
+    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv, 1.0f};
     Frag<T> k[2][D / KS<T, TR>], v[DV / KS<T, TR>];
 #pragma unroll
     for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(ks, key, seen, m, k[m]);
@@ -260,7 +289,7 @@ __global__ __launch_bounds__(256, 1) void keys_kernel(const BackwardCall g, int 
         for (int blk = 0; blk < D / TR; ++blk) clear<TR>(dk[m][blk]);
 #pragma unroll
     for (int blk = 0; blk < DV / TR; ++blk) clear<TR>(dv[blk]);
-    const auto in = [&](int row) { return row < a.R; };
+    const auto in = [](int) { return true; };
     StageQ q_stage;
     StageG g_stage;
     float plane = 0.0f;
@@ -270,88 +299,105 @@ __global__ __launch_bounds__(256, 1) void keys_kernel(const BackwardCall g, int 
         if (p < PLANES) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
     };
     if (begin < a.R) {
-        q_stage.load(qs, begin, in);
-        g_stage.load(gs, begin, in);
+        q_stage.load(qs, begin, a.R, in);
+        g_stage.load(gs, begin, a.R, in);
         load_planes(begin);
     }
-    for (int row = begin; row < a.R; row += STEP) {
-        __syncthreads();
-        q_stage.store(q_tile);
-        g_stage.store(g_tile);
-        if (threadIdx.x < PLANES * STEP) planes[threadIdx.x / STEP][threadIdx.x % STEP] = plane;
-        __syncthreads();
-        if (row + STEP < a.R) {
-            q_stage.load(qs, row + STEP, in);
-            g_stage.load(gs, row + STEP, in);
+    const auto store = [&](int to) {
+        q_stage.store(q_tile[to]);
+        g_stage.store(g_tile[to]);
+        if (threadIdx.x < PLANES * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = plane;
+    };
+    if (BUFFERS == 2 && begin < a.R) store(0);
+    int at = 0;
+    const auto tile_of = [&](int row, const auto &use) {
+        const bool more = row + STEP < a.R;
+        if (BUFFERS == 1) {
+            __syncthreads();
+            store(0);
+        }
+        if (more) {
+            q_stage.load(qs, row + STEP, a.R, in);
+            g_stage.load(gs, row + STEP, a.R, in);
             load_planes(row + STEP);
         }
-        if (row + STEP <= wave_any) continue;
-        const bool limited = row < wave_all;
-        Acc<TR> da[BLOCKS<TR>];
-        float p[2][REGS<TR>];
-#pragma unroll
-        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-            clear<TR>(da[blk]);
-#pragma unroll
-            for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
-                mma<TR>(row_frag<T, TR>(g_tile, StageG::PITCH, blk * TR + lane_row<TR>(), kk), v[kk], da[blk]);
+        __syncthreads();
+        use();
+        if (BUFFERS == 2) {
+            at ^= 1;
+            if (more) store(at);
         }
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
+    };
+    int row = begin;
+    for (; row + STEP <= wave_any && row < a.R; row += STEP) tile_of(row, [] {});        // rows that see none of the wave's keys
+    for (; row < a.R; row += STEP)
+        tile_of(row, [&] {
+            const bool limited = row < wave_all;
+            Acc<TR> da[BLOCKS<TR>];
+            float p[2][REGS<TR>];
 #pragma unroll
             for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-                Acc<TR> s;
-                clear<TR>(s);
+                clear<TR>(da[blk]);
 #pragma unroll
-                for (int kk = 0; kk < D / KS<T, TR>; ++kk)
-                    mma<TR>(row_frag<T, TR>(q_tile + m * D, StageQ::PITCH, blk * TR + lane_row<TR>(), kk), k[m][kk], s);
+                for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
+                    mma<TR>(row_frag<T, TR>(g_tile[at], StageG::PITCH, blk * TR + lane_row<TR>(), kk), v[kk], da[blk]);
+            }
 #pragma unroll
-                for (int i = 0; i < TR * TR / 64; ++i) {
-                    const int f = blk * (TR * TR / 64) + i, at = index_of<TR>(f);
-                    float t = __builtin_amdgcn_exp2f(fmaf(s[i], c, planes[m ? MINUS_SUM2 : MINUS_SUM1][at]));
-                    if (limited && row + at < lane_from) t = 0.0f;
-                    p[m][f] = m ? t * planes[LAMBDA][at] : t;       // the second map's with lambda
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+                    Acc<TR> s;
+                    clear<TR>(s);
+#pragma unroll
+                    for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+                        mma<TR>(row_frag<T, TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR + lane_row<TR>(), kk), k[m][kk], s);
+#pragma unroll
+                    for (int i = 0; i < TR * TR / 64; ++i) {
+                        const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
+                        float t = __builtin_amdgcn_exp2f(fmaf(s[i], c, planes[at][m ? MINUS_SUM2 : MINUS_SUM1][n]));
+                        if (limited && row + n < lane_from) t = 0.0f;
+                        p[m][f] = m ? t * planes[at][LAMBDA][n] : t;       // the second map's with lambda
+                    }
                 }
+            {
+                float diff[REGS<TR>];
+                Frag<T> frag[FRAGS<T, TR>];
+#pragma unroll
+                for (int f = 0; f < REGS<TR>; ++f) diff[f] = p[0][f] - p[1][f];
+                to_frags<T, TR>(diff, frag);
+#pragma unroll
+                for (int blk = 0; blk < DV / TR; ++blk)
+#pragma unroll
+                    for (int j = 0; j < FRAGS<T, TR>; ++j) mma<TR>(column_frag<TR>(g_tile[at], StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
             }
-        {
-            float diff[REGS<TR>];
-            Frag<T> frag[FRAGS<T, TR>];
 #pragma unroll
-            for (int f = 0; f < REGS<TR>; ++f) diff[f] = p[0][f] - p[1][f];
-            to_frags<T, TR>(diff, frag);
+            for (int m = 0; m < 2; ++m) {
+                float ds[REGS<TR>];
+                Frag<T> frag[FRAGS<T, TR>];
 #pragma unroll
-            for (int blk = 0; blk < DV / TR; ++blk)
+                for (int f = 0; f < REGS<TR>; ++f) {
+                    const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[at][m ? DOT2 : DOT1][index_of<TR>(f)];
+                    ds[f] = (m ? -p[m][f] : p[m][f]) * d;
+                }
+                to_frags<T, TR>(ds, frag);
 #pragma unroll
-                for (int j = 0; j < FRAGS<T, TR>; ++j) mma<TR>(column_frag<TR>(g_tile, StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
-        }
+                for (int blk = 0; blk < D / TR; ++blk)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            float ds[REGS<TR>];
-            Frag<T> frag[FRAGS<T, TR>];
-#pragma unroll
-            for (int f = 0; f < REGS<TR>; ++f) {
-                const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[m ? DOT2 : DOT1][index_of<TR>(f)];
-                ds[f] = (m ? -p[m][f] : p[m][f]) * d;
+                    for (int j = 0; j < FRAGS<T, TR>; ++j)
+                        mma<TR>(column_frag<TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR, j), frag[j], dk[m][blk]);
             }
-            to_frags<T, TR>(ds, frag);
-#pragma unroll
-            for (int blk = 0; blk < D / TR; ++blk)
-#pragma unroll
-                for (int j = 0; j < FRAGS<T, TR>; ++j)
-                    mma<TR>(column_frag<TR>(q_tile + m * D, StageQ::PITCH, blk * TR, j), frag[j], dk[m][blk]);
-        }
-    }
+        });
     if (key >= a.Lk) return;
-    const int64_t at = ((int64_t)b * a.Lk + key) * a.Hkv + hk;
+    const int64_t place = ((int64_t)b * a.Lk + key) * a.Hkv + hk;
     if (g.dk) {
-        T *out = static_cast<T *>(g.dk) + at * 2 * a.d;
+        T *out = static_cast<T *>(g.dk) + place * 2 * a.d;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dk[m][blk], a.scale);
     }
     if (g.dv) {
-        T *out = static_cast<T *>(g.dv) + at * a.dv;
+        T *out = static_cast<T *>(g.dv) + place * a.dv;
 #pragma unroll
         for (int blk = 0; blk < DV / TR; ++blk) store_columns<T, TR>(out + blk * TR, a.dv - blk * TR, dv[blk], 1.0f);
     }
@@ -364,7 +410,7 @@ struct Backward {
     template <int D, int DV>
     int operator()() const
     {
-        constexpr int TR = TILE_ROWS<D, DV>;
+        constexpr int TR = TILE_ROWS<T, D>;
         const Call &a = g.a;
         const int64_t rows = (int64_t)a.B * a.Hkv * a.R, row_tiles = ceil_div(a.R, 4 * TR), key_tiles = ceil_div(a.Lk, 4 * TR);
         if (ceil_div(rows, 16) > INT32_MAX || key_tiles * a.B * a.Hkv > INT32_MAX) return fail(MAM_ERR_UNSUPPORTED, "too many tiles");
@@ -374,11 +420,15 @@ struct Backward {
             rc = check_launch("attention::rows_kernel");
         }
         if (rc == MAM_OK && g.dq && rows > 0) {
-            hipLaunchKernelGGL((queries_kernel<T, TR, D, DV>), dim3((unsigned)(row_tiles * a.B * a.Hkv)), dim3(256), 0, st, g, (int)row_tiles);
+            const dim3 grid((unsigned)(row_tiles * a.B * a.Hkv));
+            if (a.fast) hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, true>), grid, dim3(256), 0, st, g, (int)row_tiles);
+            else hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, false>), grid, dim3(256), 0, st, g, (int)row_tiles);
             rc = check_launch("attention::queries_kernel");
         }
         if (rc == MAM_OK && (g.dk || g.dv) && key_tiles * a.B * a.Hkv > 0) {
-            hipLaunchKernelGGL((keys_kernel<T, TR, D, DV>), dim3((unsigned)(key_tiles * a.B * a.Hkv)), dim3(256), 0, st, g, (int)key_tiles);
+            const dim3 grid((unsigned)(key_tiles * a.B * a.Hkv));
+            if (a.fast && g.fast) hipLaunchKernelGGL((keys_kernel<T, TR, D, DV, true>), grid, dim3(256), 0, st, g, (int)key_tiles);
+            else hipLaunchKernelGGL((keys_kernel<T, TR, D, DV, false>), grid, dim3(256), 0, st, g, (int)key_tiles);
             rc = check_launch("attention::keys_kernel");
         }
         if (rc == MAM_OK && g.dlam && a.H > 0) {
@@ -399,7 +449,7 @@ extern "C" size_t mam_diff_attention_backward_workspace(const mam_diff_attention
 }
 
 extern "C" int mam_diff_attention_backward(const mam_diff_attention_t *args, const void *dout, const int64_t *dout_stride, const void *out,
-                                           const void *out2, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
+                                           const float *kept, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
                                            size_t workspace_bytes, void *stream)
 {
     using namespace mam;
@@ -408,13 +458,14 @@ extern "C" int mam_diff_attention_backward(const mam_diff_attention_t *args, con
     if (rc != MAM_OK) return rc;
     const attention::Call &a = g.a;
     const bool rows = a.B > 0 && a.R > 0;
-    if (rows && (!a.q || !a.lam || !dout || !dout_stride || !out || !out2 || !lse)) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
+    if (rows && (!a.q || !a.lam || !dout || !dout_stride || !out || !kept || !lse)) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
     if (a.B > 0 && a.Lk > 0 && a.H > 0 && (!a.k || !a.v)) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
     const size_t need = mam_diff_attention_backward_workspace(args);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(MAM_ERR_WORKSPACE, "the attention's backward needs %zu workspace bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);
-    g.dout = dout; g.out = out; g.out2 = out2; g.lse = lse;
+    g.dout = dout; g.out = out; g.kept = kept; g.lse = lse;
     if (dout_stride) { g.gb = dout_stride[0]; g.gl = dout_stride[1]; g.gh = dout_stride[2]; }
+    g.fast = attention::fast_operand(dout, type_size(args->type), a.dv, g.gb, g.gl, g.gh, 0, a.G);
     g.dq = dq; g.dk = dk; g.dv = dv; g.dlam = dlam;
     g.rows = static_cast<float *>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -302,18 +302,19 @@ Tensors diff_attention_cuda(const Tensor &q, const Tensor &k, const Tensor &v, c
     const AttentionCall c = attention_call(q, k, v, lam, scale, causal, lengths, starts, key_mask);
     const mam_diff_attention_t &a = c.a;
     Tensor out = at::empty({a.B, a.Lq, a.H, a.Dv}, q.options());
-    Tensor out2 = with_sums ? at::empty({a.B, a.Lq, a.H, a.Dv}, q.options()) : at::empty({0}, q.options());
+    const int64_t planes = a.type == MAM_F32 ? 1 : 2;
+    Tensor kept = with_sums ? at::empty({planes, a.B, a.Lq, a.H, a.Dv}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
     Tensor lse = with_sums ? at::empty({2, a.B, a.H, a.Lq}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
     const Tensor ws = workspace_for(mam_diff_attention_workspace(&a), q);
-    check_rc(mam_diff_attention(&a, out.data_ptr(), with_sums ? out2.data_ptr() : nullptr, with_sums ? lse.data_ptr<float>() : nullptr,
+    check_rc(mam_diff_attention(&a, out.data_ptr(), with_sums ? kept.data_ptr<float>() : nullptr, with_sums ? lse.data_ptr<float>() : nullptr,
                                 out_ptr(ws), ws.defined() ? ws.numel() : 0, current_stream(q)),
              "mam_diff_attention");
-    return {out, out2, lse};
+    return {out, kept, lse};
 }
 
 // wanted: the gradients of q, of k and v, of lam
 Tensors diff_attention_backward_cuda(const Tensor &grad, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lam, const Tensor &out,
-                                     const Tensor &out2, const Tensor &lse, double scale, bool causal, const MaybeTensor &lengths,
+                                     const Tensor &kept, const Tensor &lse, double scale, bool causal, const MaybeTensor &lengths,
                                      const MaybeTensor &starts, const MaybeTensor &key_mask, bool want_q, bool want_kv, bool want_lam)
 {
     const c10::DeviceGuard guard(q.device());
@@ -321,9 +322,12 @@ Tensors diff_attention_backward_cuda(const Tensor &grad, const Tensor &q, const 
     const mam_diff_attention_t &a = c.a;
     TORCH_CHECK(out.sizes() == at::IntArrayRef({a.B, a.Lq, a.H, a.Dv}), "out has the wrong shape");
     check_like(out, grad, "out");
-    check_like(out2, out, "out2");
     TORCH_CHECK(out.device() == q.device() && out.scalar_type() == q.scalar_type(), "out must have q's type and device");
-    TORCH_CHECK(out.is_contiguous() && out2.is_contiguous(), "out and out2 must be contiguous");
+    TORCH_CHECK(out.is_contiguous(), "out must be contiguous");
+    const int64_t planes = a.type == MAM_F32 ? 1 : 2;
+    TORCH_CHECK(kept.device() == q.device() && kept.scalar_type() == at::kFloat && kept.is_contiguous() &&
+                    kept.sizes() == at::IntArrayRef({planes, a.B, a.Lq, a.H, a.Dv}),
+                "kept must be a contiguous float32 tensor of ", planes, " planes like out");
     TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
                     lse.sizes() == at::IntArrayRef({2, a.B, a.H, a.Lq}),
                 "lse must be a contiguous float32 tensor of (2, batch, heads, queries)");
@@ -337,7 +341,7 @@ Tensors diff_attention_backward_cuda(const Tensor &grad, const Tensor &q, const 
     }
     if (want_lam) dlam = at::empty({a.H}, lam.options());
     const Tensor ws = workspace_for(mam_diff_attention_backward_workspace(&a), q);
-    check_rc(mam_diff_attention_backward(&a, g.data_ptr(), strides, out.data_ptr(), out2.data_ptr(), lse.data_ptr<float>(), out_ptr(dq),
+    check_rc(mam_diff_attention_backward(&a, g.data_ptr(), strides, out.data_ptr(), kept.data_ptr<float>(), lse.data_ptr<float>(), out_ptr(dq),
                                          out_ptr(dk), out_ptr(dv), out_ptr(dlam), out_ptr(ws), ws.defined() ? ws.numel() : 0, current_stream(q)),
              "mam_diff_attention_backward");
     return {or_empty(dq, q), or_empty(dk, q), or_empty(dv, q), or_empty(dlam, lam)};
@@ -584,7 +588,7 @@ TORCH_LIBRARY(mamtorch_kernel_encoder, m)
           "bool weight_is_float) -> Tensor[]");
     m.def("diff_attention(Tensor q, Tensor k, Tensor v, Tensor lam, float scale, bool causal, Tensor? lengths, Tensor? starts, "
           "Tensor? key_mask, bool with_sums) -> Tensor[]");
-    m.def("diff_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor lam, Tensor out, Tensor out2, Tensor lse, float scale, "
+    m.def("diff_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor lam, Tensor out, Tensor kept, Tensor lse, float scale, "
           "bool causal, Tensor? lengths, Tensor? starts, Tensor? key_mask, bool want_q, bool want_kv, bool want_lam) -> Tensor[]");
 }
 

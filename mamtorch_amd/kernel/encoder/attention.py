@@ -39,13 +39,13 @@ def _(q, k, v, lam, scale, causal, lengths, starts, key_mask, with_sums):
     b, n, h = q.shape[:3]
     shape = (b, n, h, v.size(3))
     return [torch.empty(shape, dtype=q.dtype, device=q.device),
-            torch.empty(shape if with_sums else (0,), dtype=q.dtype, device=q.device),
+            torch.empty((1 if q.dtype == torch.float else 2,) + shape if with_sums else (0,), dtype=torch.float, device=q.device),
             torch.empty((2, b, h, n) if with_sums else (0,), dtype=torch.float, device=q.device)]
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::diff_attention_backward")
-def _(grad, q, k, v, lam, out, out2, lse, scale, causal, lengths, starts, key_mask, want_q, want_kv, want_lam):
+def _(grad, q, k, v, lam, out, kept, lse, scale, causal, lengths, starts, key_mask, want_q, want_kv, want_lam):
     _check(q, k, v, lam)
-    torch._check(grad.shape == out.shape and out2.shape == out.shape)
+    torch._check(grad.shape == out.shape and kept.shape[1:] == out.shape)
     wanted = ((q, want_q), (k, want_kv), (v, want_kv), (lam, want_lam))
     return [torch.empty(t.shape if w else (0,), dtype=t.dtype, device=t.device) for t, w in wanted]
