@@ -4,11 +4,11 @@
 //   mu = mean_c x, r = 1 / sqrt(mean_c (x - mu)^2 + eps), xh = (x - mu) r, y = xh w + b
 //   g = dy w, dx = r (g - mean_c g - xh mean_c (g xh)), dw = sum_n dy xh, db = sum_n dy
 //
-// Bound by memory: a row is read once into the registers of the LANES lanes that own it (16 lanes of a wave, a wave, or a workgroup of 256
-// or 1024, so that a lane holds at most 16 elements), its mean is taken first and then the squares of what is left, all in fp32.  The
-// backward's workgroups take rows in turn, keep their sums of dw and db in registers over all of them and write them once; a
-// second kernel adds the workgroups' sums in a fixed order, so two calls give the same bits.  Rows beyond 16384 elements are read
-// again for each pass.
+// Bound by memory: a row is read once into the registers of the LANES lanes that own it (16 lanes of a wave, a wave, or a workgroup of 128
+// to 1024, so that a lane holds at most 16 elements, 24 where that keeps a row in one wave), its mean is taken first and then the squares of
+// what is left, all in fp32.  The backward's workgroups take rows in turn, the next one's loads on their way while this one is worked on, keep
+// their sums of dw and db in registers over all of them and write them once; a second kernel adds the workgroups' sums in a fixed order, so
+// two calls give the same bits.  Rows beyond 16384 elements are read again for each pass.
 #include "mam_counter.h"
 #include "mam_types.h"
 
@@ -16,7 +16,20 @@ namespace mam {
 namespace norm {
 
 constexpr int HELD = 16;                    // elements of a lane
+constexpr int HELD_BY_WAVE = 24;            // the same where a wave has the row
 constexpr int MOST_HELD = 1024 * HELD;      // longest row that is held in registers
+
+// Threads of a workgroup: a row's lanes, or 256 for several rows.
+template <int LANES>
+constexpr int THREADS_OF = LANES > 64 ? LANES : 256;
+
+// The row of a workgroup's that a thread belongs to; the same for a wave where rows are no less than that.
+template <int LANES>
+__device__ __forceinline__ int group_of()
+{
+    if constexpr (LANES >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+    return threadIdx.x / LANES;
+}
 
 struct Args {
     const void *x, *residual, *weight, *bias;   // residual: joins only
@@ -87,19 +100,19 @@ __device__ __forceinline__ void join_piece(const Args &a, int64_t row, int c, ui
     float x[N], f[N];
     load_pack<T>(static_cast<const T *>(a.residual) + row * a.ldr + c, a.C - c, v);
     load_pack<T>(static_cast<const T *>(a.x) + row * a.ldx + c, a.C - c, x);
-    keep_factors<N>(a.drop, offset, (uint64_t)row * (uint64_t)a.C + (uint64_t)c, (a.C & 3) == 0, f);
+    keep_factors<N>(a.drop, offset, (uint64_t)row * (uint64_t)a.C + (uint64_t)c, ((uint32_t)row * (uint32_t)a.C & 3) == 0, f);
 #pragma unroll
     for (int u = 0; u < N; ++u) v[u] = (float)(T)(v[u] + keep_value(x[u], f[u]));
     store_pack<T>(static_cast<T *>(a.s) + row * a.C + c, a.C - c, v);
 }
 
 template <class T, int LANES, int PACKS, bool JOIN>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_kernel(const Args a)
+__global__ __launch_bounds__(THREADS_OF<LANES>) void norm_kernel(const Args a)
 {
-    constexpr int N = kPack<T>, THREADS = LANES > 256 ? LANES : 256;
+    constexpr int N = kPack<T>, THREADS = THREADS_OF<LANES>;
     __shared__ float scratch[LANES > 64 ? LANES / 64 : 1];
     const int lane = threadIdx.x % LANES;
-    const int64_t row = (int64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
+    const int64_t row = (int64_t)blockIdx.x * (THREADS / LANES) + group_of<LANES>();
     if (row >= a.N) return;                     // rows of more than a wave: a workgroup's, which leaves as a whole
     const uint64_t offset = JOIN ? dropout_offset(a.drop) : 0;
     float v[PACKS][N];
@@ -222,7 +235,7 @@ __device__ __forceinline__ void join_out(const BackwardArgs &a, int64_t row, int
     if (a.dx) store_pack<T>(static_cast<T *>(a.dx) + row * a.C + c, a.C - c, g);
     if (a.dropped) {
         float f[N];
-        keep_factors<N>(a.drop, offset, (uint64_t)row * (uint64_t)a.C + (uint64_t)c, (a.C & 3) == 0, f);
+        keep_factors<N>(a.drop, offset, (uint64_t)row * (uint64_t)a.C + (uint64_t)c, ((uint32_t)row * (uint32_t)a.C & 3) == 0, f);
 #pragma unroll
         for (int u = 0; u < N; ++u) f[u] = keep_value(g[u], f[u]);
         store_pack<T>(static_cast<T *>(a.dropped) + row * a.C + c, a.C - c, f);
@@ -232,12 +245,12 @@ __device__ __forceinline__ void join_out(const BackwardArgs &a, int64_t row, int
 // Workgroups take rows in turn.  A lane's columns are the same in every row, so its sums of dw and db stay in registers; the rows of
 // a workgroup that are a wave's or a part of one are joined in LDS at the end.
 template <class T, int LANES, int PACKS, bool JOIN>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_backward_kernel(const BackwardArgs a)
+__global__ __launch_bounds__(THREADS_OF<LANES>) void norm_backward_kernel(const BackwardArgs a)
 {
-    constexpr int N = kPack<T>, THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
+    constexpr int N = kPack<T>, THREADS = THREADS_OF<LANES>, ROWS = THREADS / LANES;
     __shared__ float scratch[LANES > 64 ? 2 * (LANES / 64) : 1];
     __shared__ float joined[ROWS > 1 ? ROWS * LANES * PACKS * N : 1];
-    const int lane = threadIdx.x % LANES, which = threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES, which = group_of<LANES>();
     const uint64_t offset = JOIN ? dropout_offset(a.drop) : 0;
     const float inv = 1.0f / (float)a.C;
     float w[PACKS][N], dw[PACKS][N], db[PACKS][N];
@@ -253,15 +266,33 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_backward_kerne
 #pragma unroll
         for (int u = 0; u < N; ++u) dw[i][u] = db[i][u] = 0.0f;
     }
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + which; row < a.N; row += (int64_t)gridDim.x * ROWS) {
-        float dy[PACKS][N], xh[PACKS][N];
+    Raw<T> next_dy[PACKS], next_x[PACKS];
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    const auto load_row = [&](int64_t row) {
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
             const int c = (lane + i * LANES) * N;
-            load_pack<T>(static_cast<const T *>(a.dy) + row * a.lddy + c, a.C - c, dy[i]);
-            load_pack<T>(static_cast<const T *>(a.x) + row * a.ldx + c, a.C - c, xh[i]);
+            next_dy[i] = load_raw<T>(static_cast<const T *>(a.dy) + row * a.lddy + c, a.C - c);
+            next_x[i] = load_raw<T>(static_cast<const T *>(a.x) + row * a.ldx + c, a.C - c);
         }
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        next_mean = a.mean[row];
+        next_rstd = a.rstd[row];
+    };
+    constexpr bool AHEAD = LANES < 1024;        // 16 waves have no registers for a second row
+    const int64_t first = (int64_t)blockIdx.x * ROWS + which, step = (int64_t)gridDim.x * ROWS;
+    if (AHEAD && first < a.N) load_row(first);
+    for (int64_t row = first; row < a.N; row += step) {
+        float dy[PACKS][N], xh[PACKS][N];
+        if (!AHEAD) load_row(row);
+        const float mean = next_mean, rstd = next_rstd;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i)
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                dy[i][u] = (float)next_dy[i][u];
+                xh[i][u] = (float)next_x[i][u];
+            }
+        if (AHEAD && row + step < a.N) load_row(row + step);
         float sum = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < PACKS; ++i)
@@ -416,30 +447,34 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const float *__restrict
     }
 }
 
-// Lanes of a row: 16 while they hold it in two 16-byte pieces each, else the fewest of 64, 256 and 1024 that hold it with 16 elements each.
+// Lanes of a row: 16 while they hold it in two 16-byte pieces each, a wave up to HELD_BY_WAVE elements a lane, else the fewest of 128 to 1024
+// that hold it with HELD each.
 inline int lanes_of(int64_t C, int type)
 {
     const int64_t pack = type == MAM_F32 ? 4 : 8;
-    return C <= 2 * 16 * pack ? 16 : C <= 64 * HELD ? 64 : C <= 256 * HELD ? 256 : 1024;
+    if (C <= 2 * 16 * pack) return 16;
+    if (C <= 64 * HELD_BY_WAVE) return 64;
+    int lanes = 128;
+    while (C > lanes * HELD) lanes *= 2;
+    return lanes;
 }
 
-// Workgroups of the backward: as many as run at once (two of a CU's), which have several rows each where there are many.
+// Workgroups of the backward: 16 waves for each CU, which have several rows each where there are many.
 inline int64_t backward_shares(int64_t N, int64_t C, int type)
 {
     if (C > MOST_HELD) {
         const int64_t s = ceil_div(N, 32);
         return s < 64 ? s : 64;
     }
-    const int lanes = lanes_of(C, type);
-    const int64_t rows = lanes > 256 ? 1 : 256 / lanes, groups = ceil_div(N, rows);
-    const int64_t most = 2 * (int64_t)kNumCU;
+    const int lanes = lanes_of(C, type), threads = lanes > 64 ? lanes : 256;
+    const int64_t groups = ceil_div(N, threads / lanes), most = (int64_t)kNumCU * 1024 / threads;
     return groups < most ? groups : most;
 }
 
 template <class T, int LANES, int PACKS>
 void launch_forward(const Args &a, bool join, hipStream_t st)
 {
-    constexpr int THREADS = LANES > 256 ? LANES : 256;
+    constexpr int THREADS = THREADS_OF<LANES>;
     const dim3 grid((unsigned)ceil_div(a.N, THREADS / LANES));
     if (join) hipLaunchKernelGGL((norm_kernel<T, LANES, PACKS, true>), grid, dim3(THREADS), 0, st, a);
     else hipLaunchKernelGGL((norm_kernel<T, LANES, PACKS, false>), grid, dim3(THREADS), 0, st, a);
@@ -448,7 +483,7 @@ void launch_forward(const Args &a, bool join, hipStream_t st)
 template <class T, int LANES, int PACKS>
 void launch_backward(const BackwardArgs &a, bool join, int64_t shares, hipStream_t st)
 {
-    constexpr int THREADS = LANES > 256 ? LANES : 256;
+    constexpr int THREADS = THREADS_OF<LANES>;
     if (join) hipLaunchKernelGGL((norm_backward_kernel<T, LANES, PACKS, true>), dim3((unsigned)shares), dim3(THREADS), 0, st, a);
     else hipLaunchKernelGGL((norm_backward_kernel<T, LANES, PACKS, false>), dim3((unsigned)shares), dim3(THREADS), 0, st, a);
 }
@@ -466,14 +501,25 @@ void with_shape(int C, const F &f)
     } else if (lanes == 64) {
         if (packs <= 1) f.template operator()<64, 1>();
         else if (packs == 2) f.template operator()<64, 2>();
-        else if (packs == 3) f.template operator()<64, MOST < 3 ? MOST : 3>();
-        else f.template operator()<64, MOST>();
+        else if (packs == 3) f.template operator()<64, 3>();
+        else if constexpr (N == 4) {
+            if (packs == 4) f.template operator()<64, 4>();
+            else f.template operator()<64, 6>();
+        }
+    } else if (lanes == 128) {
+        f.template operator()<128, MOST>();
     } else if (lanes == 256) {
-        if (packs <= 2) f.template operator()<256, 2>();
-        else f.template operator()<256, MOST>();
+        if constexpr (N == 4)
+            if (packs == 3) return f.template operator()<256, 3>();
+        f.template operator()<256, MOST>();
+    } else if (lanes == 512) {
+        if constexpr (N == 4)
+            if (packs == 3) return f.template operator()<512, 3>();
+        f.template operator()<512, MOST>();
     } else {
-        if (packs <= 2) f.template operator()<1024, 2>();
-        else f.template operator()<1024, MOST>();
+        if constexpr (N == 4)
+            if (packs == 3) return f.template operator()<1024, 3>();
+        f.template operator()<1024, MOST>();
     }
 }
 

@@ -45,6 +45,19 @@ __device__ __forceinline__ void store_pack(T *p, int left, const float (&v)[N])
     }
 }
 
+// A piece as it is, to be loaded before it is used: half the registers of its elements in fp32.
+template <class T>
+using Raw = typename Pack<T, kPack<T>>::type;
+template <class T>
+__device__ __forceinline__ Raw<T> load_raw(const T *p, int left)
+{
+    if (left >= kPack<T>) return *reinterpret_cast<const Raw<T> *>(p);
+    Raw<T> t;
+#pragma unroll
+    for (int u = 0; u < kPack<T>; ++u) t[u] = u < left ? p[u] : (T)0.0f;
+    return t;
+}
+
 // The same of a vector whose type is known at run time only: `same` says that it is T, else fp32.
 template <class T, int N = kPack<T>>
 __device__ __forceinline__ void load_pack_of(const void *p, bool same, int64_t at, int left, float (&v)[N])
