@@ -21,7 +21,7 @@ import mamtorch_amd as _impl
 
 _PATHS = (
     "kernel", "kernel.v1", "kernel.v1.fullyconnected", "kernel.v4", "kernel.v4.fullyconnected",
-    "kernel.v4.fullyconnected_fast",
+    "kernel.v4.fullyconnected_fast", "kernel.encoder", "nn.encoder",
     "nn", "nn.compat", "nn.v1", "nn.v1.fullyconnected", "nn.v4", "nn.v4.fullyconnected",
     "sparse", "sparse.kernel", "sparse.kernel.v1", "sparse.kernel.v1.cusparsemm",
 )

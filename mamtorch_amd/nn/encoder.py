@@ -1,0 +1,172 @@
+"""What an encoder layer has beside its MAM layers, and the layer: layer norm, dropout without a stored mask, differential attention with its
+cache, and ``MAMEncoderLayer``, in which they run together with ``FullyConnected``.
+
+The reference swaps the two Linear layers of a ViT's encoder layer for MAM layers and leaves the rest to its model library
+(examples/vitb16_imagenet1k/utils.py:50-77); here the rest is the framework's operators too (``mamtorch.kernel.encoder``).
+"""
+import math
+
+import torch
+from torch import Tensor, nn
+
+from ..kernel import encoder as K
+from .fullyconnected import FullyConnected
+
+__all__ = ["LayerNorm", "Dropout", "DiffAttention", "DiffAttentionCache", "MAMEncoderLayer"]
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the last dimension; parameters and state as ``torch.nn.LayerNorm`` has them."""
+
+    def __init__(self, features: int, eps: float = 1e-5, bias: bool = True, device=None, dtype=None):
+        super().__init__()
+        self.features, self.eps = features, eps
+        self.weight = nn.Parameter(torch.ones(features, device=device, dtype=dtype))
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(features, device=device, dtype=dtype))
+        else:
+            self.register_parameter("bias", None)
+
+    def forward(self, x: Tensor) -> Tensor:
+        return K.layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self) -> str:
+        return f"{self.features}, eps={self.eps}, bias={self.bias is not None}"
+
+
+class Dropout(nn.Module):
+    """Dropout whose mask is formed from (seed, number of the training call) where it is needed.  The number of calls is part of the module's
+    state, so that a training run that is taken up again draws on; modules of one model need seeds of their own."""
+
+    def __init__(self, p: float = 0.5, seed: int = 0):
+        super().__init__()
+        if not 0 <= p <= 1:
+            raise ValueError(f"p must be between 0 and 1, got {p}")
+        self.p, self.seed, self.calls = p, seed, 0
+
+    def next_offset(self) -> int:
+        self.calls += 1
+        return self.calls - 1
+
+    def forward(self, x: Tensor, residual: Tensor = None) -> Tensor:
+        if not self.training or self.p == 0:
+            return x if residual is None else residual + x
+        return K.dropout(x, self.p, self.seed, self.next_offset(), residual)
+
+    def get_extra_state(self):
+        return {"calls": self.calls}
+
+    def set_extra_state(self, state):
+        self.calls = int(state["calls"])
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}, seed={self.seed}"
+
+
+class DiffAttentionCache:
+    """Keys and values of up to ``most`` tokens for each request, and how many each has."""
+
+    def __init__(self, batch: int, most: int, kv_heads: int, head_size: int, value_size: int, device=None, dtype=None):
+        self.most = most
+        self.k = torch.empty(batch, most, kv_heads, 2, head_size, device=device, dtype=dtype)
+        self.v = torch.empty(batch, most, kv_heads, value_size, device=device, dtype=dtype)
+        self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
+        self.filled = 0                     # most tokens of a request, on the host
+
+    def append(self, k: Tensor, v: Tensor) -> Tensor:
+        """Puts k (batch, n, ...) and v behind what there is; returns the places of the first of them."""
+        n = k.shape[1]
+        if k.shape[0] != self.k.shape[0]:
+            raise ValueError(f"the cache is for {self.k.shape[0]} requests, got {k.shape[0]}")
+        if self.filled + n > self.most:
+            raise ValueError(f"the cache holds {self.most} tokens: {self.filled} and {n} more do not fit")
+        starts = self.lengths.clone()
+        at = starts.long()[:, None] + torch.arange(n, device=starts.device)
+        rows = torch.arange(k.shape[0], device=starts.device)[:, None]
+        self.k[rows, at] = k
+        self.v[rows, at] = v
+        self.lengths += n
+        self.filled += n
+        return starts
+
+
+class DiffAttention(nn.Module):
+    """Differential attention (T. Ye et al., "Differential Transformer", 2024): each head's map is the difference of two softmaxes, the second one weighted
+    with lambda = exp(q1 . k1) - exp(q2 . k2) + lambda_init from learned vectors, each head's output is normalised by itself and scaled with
+    1 - lambda_init.  ``heads`` heads of two maps of size hidden / (2 heads) and values of size hidden / heads, over ``kv_heads`` key heads."""
+
+    def __init__(self, hidden: int, heads: int, kv_heads: int = None, depth: int = 1, causal: bool = False, bias: bool = True, eps: float = 1e-5,
+                 device=None, dtype=None):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if hidden % (2 * heads):
+            raise ValueError(f"hidden ({hidden}) must be a multiple of twice the heads ({heads})")
+        if heads % kv_heads:
+            raise ValueError(f"kv_heads ({kv_heads}) must divide heads ({heads})")
+        kwargs = {"device": device, "dtype": dtype}
+        self.hidden, self.heads, self.kv_heads, self.causal = hidden, heads, kv_heads, causal
+        self.head_size, self.value_size = hidden // (2 * heads), hidden // heads
+        self.lambda_init = 0.8 - 0.6 * math.exp(-0.3 * (depth - 1))
+        self.query = nn.Linear(hidden, heads * 2 * self.head_size, bias=bias, **kwargs)
+        self.key = nn.Linear(hidden, kv_heads * 2 * self.head_size, bias=bias, **kwargs)
+        self.value = nn.Linear(hidden, kv_heads * self.value_size, bias=bias, **kwargs)
+        self.output = nn.Linear(hidden, hidden, bias=bias, **kwargs)
+        self.lambda_vectors = nn.Parameter(0.1 * torch.randn(4, heads, self.head_size, **kwargs))
+        self.norm = LayerNorm(self.value_size, eps, **kwargs)
+
+    def lambdas(self) -> Tensor:
+        q1, k1, q2, k2 = self.lambda_vectors.float()
+        return torch.exp((q1 * k1).sum(-1)) - torch.exp((q2 * k2).sum(-1)) + self.lambda_init
+
+    def cache(self, batch: int, most: int) -> DiffAttentionCache:
+        weight = self.key.weight
+        return DiffAttentionCache(batch, most, self.kv_heads, self.head_size, self.value_size, weight.device, weight.dtype)
+
+    def forward(self, x: Tensor, lengths: Tensor = None, key_mask: Tensor = None, cache: DiffAttentionCache = None) -> Tensor:
+        """x (batch, tokens, hidden).  With a cache, x's tokens are put behind it and see what is there (up to themselves where the module is
+        causal); lengths and key_mask (see ``kernel.encoder.diff_attention``) are for calls without one."""
+        b, n = x.shape[:2]
+        q = self.query(x).view(b, n, self.heads, 2, self.head_size)
+        k = self.key(x).view(b, n, self.kv_heads, 2, self.head_size)
+        v = self.value(x).view(b, n, self.kv_heads, self.value_size)
+        starts = None
+        if cache is not None:
+            if lengths is not None or key_mask is not None:
+                raise ValueError("a cache has lengths of its own")
+            starts = cache.append(k, v)
+            k, v, lengths = cache.k[:, :cache.filled], cache.v[:, :cache.filled], cache.lengths
+        elif self.causal:
+            starts = torch.zeros(b, device=x.device, dtype=torch.int32)
+        out = K.diff_attention(q, k, v, self.lambdas(), causal=self.causal, lengths=lengths, starts=starts if self.causal else None, key_mask=key_mask)
+        out = self.norm(out) * (1 - self.lambda_init)
+        return self.output(out.reshape(b, n, self.hidden))
+
+
+class MAMEncoderLayer(nn.Module):
+    """A pre-norm encoder layer: x + dropout(attention(norm(x))), then the same of the MAM MLP (FullyConnected -> GELU -> FullyConnected).
+    The sum between the halves, its dropout and the second norm are one operator.  ViT-B/16: hidden 768, intermediate 3072, 6 heads of two maps.
+    Further keyword arguments go to the ``FullyConnected`` layers."""
+
+    def __init__(self, hidden: int = 768, intermediate: int = 3072, heads: int = 6, kv_heads: int = None, depth: int = 1, causal: bool = False,
+                 p: float = 0.0, seed: int = 0, eps: float = 1e-5, device=None, dtype=None, **fc_kwargs):
+        super().__init__()
+        kwargs = {"device": device, "dtype": dtype}
+        self.norm1 = LayerNorm(hidden, eps, **kwargs)
+        self.attention = DiffAttention(hidden, heads, kv_heads, depth, causal, **kwargs)
+        self.dropout1 = Dropout(p, 2 * seed)
+        self.norm2 = LayerNorm(hidden, eps, **kwargs)
+        self.intermediate = FullyConnected(hidden, intermediate, **kwargs, **fc_kwargs)
+        self.act = nn.GELU()
+        self.output = FullyConnected(intermediate, hidden, **kwargs, **fc_kwargs)
+        self.dropout2 = Dropout(p, 2 * seed + 1)
+
+    def vcon_step(self) -> None:
+        self.intermediate.vcon_step()
+        self.output.vcon_step()
+
+    def forward(self, x: Tensor, lengths: Tensor = None, key_mask: Tensor = None, cache: DiffAttentionCache = None) -> Tensor:
+        a = self.attention(self.norm1(x), lengths, key_mask, cache)
+        drop, norm = self.dropout1, self.norm2
+        p = drop.p if drop.training else 0.0
+        y, s = K.add_dropout_layer_norm(a, x, norm.weight, norm.bias, p, drop.seed, drop.next_offset() if p else 0, norm.eps)
+        return self.dropout2(self.output(self.act(self.intermediate(y))), s)

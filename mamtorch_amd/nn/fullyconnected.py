@@ -13,7 +13,9 @@ counting and repr.  What differs is only how the work reaches the GPU:
   * ``update_selection_count`` is one kernel.  ``selection_count_mode="reference"`` (default)
     keeps the literal behaviour of :123-129 (per call a weight gains 1 if any row picked it as
     max and 1 if any row picked it as min, both added to ``max_selection_count``);
-    ``"hits"`` counts every pick and keeps max and min apart.
+    ``"hits"`` counts every pick and keeps max and min apart;
+  * ``wdrop_seed`` (default None: masks drawn by torch's generator, a byte a weight) takes the weight dropout's masks from
+    a counter-based generator under that seed, a new one each call, which are never stored.
 """
 import math
 
@@ -54,6 +56,7 @@ class FullyConnected(Module):
         device=None,
         dtype=None,
         selection_count_mode: str = "reference",
+        wdrop_seed: int = None,
     ) -> None:
         factory_kwargs = {"device": device, "dtype": dtype}
         super().__init__()
@@ -67,6 +70,8 @@ class FullyConnected(Module):
         self.vcon_eps = vcon_eps
         self.vcon_expand = vcon_expand
         self.wdrop_rate = wdrop_rate
+        self.wdrop_seed = wdrop_seed
+        self.wdrop_calls = 0
         self.drop_rate = drop_rate
         self.compute_exact = compute_exact
         self.train_mam_only = train_mam_only
@@ -151,6 +156,10 @@ class FullyConnected(Module):
         if self.training and self.wdrop_rate != 0:
             if not (0 < self.wdrop_rate < 1):
                 raise Exception("wdrop_rate must be between 0 and 1.")
+            if self.wdrop_seed is not None:
+                # the mask as a function of seed and call: never stored, formed again for the weight gradient
+                self.wdrop_calls += 1
+                return K.encoder.dropout(w, self.wdrop_rate, self.wdrop_seed, self.wdrop_calls - 1, scale=1.0)
             # the reference draws a float mask of the weight's size and multiplies (a second copy of W and
             # three more passes over it); here the mask is one byte per weight, drawn by torch's generator,
             # and one kernel forms weight * mask; autograd masks the weight gradient with the same call
