@@ -9,6 +9,8 @@
 // matrix cores and, in 16-bit types, the exponentials beside them.
 #include "mam_attention.h"
 
+#include <type_traits>
+
 namespace mam {
 namespace attention {
 
@@ -67,19 +69,26 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     g.rows[LAMBDA * count + id] = lam;
 }
 
-// dlambda of a head, a workgroup each.
+// dlambda of a head, a workgroup each: its waves share the requests, or some waves a request where there are fewer.
 template <class T>
 __global__ __launch_bounds__(1024) void lambda_kernel(const BackwardCall g)
 {
     __shared__ float part[16];
     const Call &a = g.a;
     const int head = blockIdx.x, hk = head / a.G, which = head % a.G;
-    const int64_t count = (int64_t)a.B * a.Hkv * a.R, terms = (int64_t)a.B * a.Lq;
-    const float *dots = g.rows + DOT2 * count;
+    const float *dots = g.rows + DOT2 * (int64_t)a.B * a.Hkv * a.R;
+    int groups = 1;
+    while (groups < 16 && groups < a.B) groups *= 2;
+    const int threads = 1024 / groups, group = threadIdx.x / threads;
     float sum = 0.0f;
-    for (int64_t t = threadIdx.x; t < terms; t += 1024) {
-        const int64_t b = t / a.Lq, i = t % a.Lq;
-        sum -= dots[(b * a.Hkv + hk) * a.R + i * a.G + which];
+    for (int b = group; b < a.B; b += groups) {
+        const float *p = dots + ((int64_t)b * a.Hkv + hk) * a.R + which;
+        for (int i = threadIdx.x % threads; i < a.Lq; i += 4 * threads) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = i + u * threads < a.Lq ? p[(int64_t)(i + u * threads) * a.G] : 0.0f;
+            sum -= (v[0] + v[1]) + (v[2] + v[3]);
+        }
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
@@ -195,69 +204,69 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
         }
     };
     int key = 0;
-    for (; key < wave_any; key += STEP)
-        tile_of(key, [&] {
-            const bool limited = key + STEP > wave_all || (!FAST && a.mask);
-            const uint32_t word = !FAST && a.mask ? mask_word(a, b, key) : 0xffffffffu;
-            Acc<TR> da[BLOCKS<TR>];
+    const auto use = [&](auto limited, uint32_t word) {
+        Acc<TR> da[BLOCKS<TR>];
+#pragma unroll
+        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+            clear<TR>(da[blk]);
+#pragma unroll
+            for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
+                mma<TR>(row_frag<T, TR>(v_tile[at], StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float ds[REGS<TR>];
 #pragma unroll
             for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-                clear<TR>(da[blk]);
+                Acc<TR> s;
+                clear<TR>(s);
 #pragma unroll
-                for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
-                    mma<TR>(row_frag<T, TR>(v_tile[at], StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
-            }
+                for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+                    mma<TR>(row_frag<T, TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                float ds[REGS<TR>];
-#pragma unroll
-                for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-                    Acc<TR> s;
-                    clear<TR>(s);
-#pragma unroll
-                    for (int kk = 0; kk < D / KS<T, TR>; ++kk)
-                        mma<TR>(row_frag<T, TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
-#pragma unroll
-                    for (int i = 0; i < TR * TR / 64; ++i) {
-                        const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
-                        float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
-                        if (limited && !(n < limit - key && (FAST || (word >> n & 1)))) p = 0.0f;
-                        ds[f] = weight[m] * p * (da[blk][i] - dot[m]);
-                    }
+                for (int i = 0; i < TR * TR / 64; ++i) {
+                    const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
+                    if (decltype(limited)::value && !(n < limit - key && (FAST || (word >> n & 1)))) p = 0.0f;
+                    ds[f] = p * (da[blk][i] - dot[m]);          // the second map's factor -lambda is a row's: it comes at the end
                 }
-                Frag<T> frag[FRAGS<T, TR>];
-                to_frags<T, TR>(ds, frag);
-#pragma unroll
-                for (int blk = 0; blk < D / TR; ++blk)
-#pragma unroll
-                    for (int j = 0; j < FRAGS<T, TR>; ++j)
-                        mma<TR>(column_frag<TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
             }
-        });
+            Frag<T> frag[FRAGS<T, TR>];
+            to_frags<T, TR>(ds, frag);
+#pragma unroll
+            for (int blk = 0; blk < D / TR; ++blk)
+#pragma unroll
+                for (int j = 0; j < FRAGS<T, TR>; ++j)
+                    mma<TR>(column_frag<TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
+        }
+    };
+    if (FAST || !a.mask)
+        for (; key + STEP <= wave_all; key += STEP) tile_of(key, [&] { use(std::false_type(), 0); });
+    for (; key < wave_any; key += STEP) tile_of(key, [&] { use(std::true_type(), !FAST && a.mask ? mask_word(a, b, key) : 0xffffffffu); });
     for (; key < end; key += STEP) tile_of(key, [] {});
     if (!there) return;
     T *out = static_cast<T *>(g.dq) + (((int64_t)b * a.Lq + query) * a.H + head) * 2 * a.d;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dq[m][blk], a.scale);
+        for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dq[m][blk], a.scale * weight[m]);
 }
 
 template <class T, int TR, int D, int DV, bool FAST>
 __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(const BackwardCall g, int key_tiles)
 {
-    constexpr int KEYS = 4 * TR, BUFFERS = TILES<T, D, DV>;
+    constexpr int ROW_KEYS = 4 * TR, BUFFERS = TILES<T, D, DV>;
     typedef Stage<T, 256, STEP, 2, D, FAST> StageQ;
     typedef Stage<T, 256, STEP, 1, DV, FAST> StageG;
     __shared__ __attribute__((aligned(16))) T q_tile[BUFFERS][STEP * StageQ::PITCH];
     __shared__ __attribute__((aligned(16))) T g_tile[BUFFERS][STEP * StageG::PITCH];
     __shared__ __attribute__((aligned(16))) float planes[BUFFERS][PLANES][STEP];
     const Call &a = g.a;
-    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, gridDim.x);
+    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, KEYS_WAVES<T, TR, D, DV> == 2 ? gridDim.x : 2 * gridDim.x);
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
     const Reach reach = reach_of(a, b);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = tile * KEYS + wave * TR, key = first + lane_row<TR>();
+    const int first = tile * ROW_KEYS + wave * TR, key = first + lane_row<TR>();
     // rows that see a key begin at (key - reach.first) * G; past every row where none does
     const auto from = [&](int k) {
         const int64_t i = (int64_t)k - reach.first;
@@ -268,7 +277,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const bool wave_seen = first < reach.keys;
     const int wave_any = wave_seen ? from(first) : a.R;
     const int wave_all = first + TR <= reach.keys && !a.mask ? from(first + TR - 1) : a.R;    // from here on every lane's key is seen
-    const int begin = tile * KEYS < reach.keys ? from(tile * KEYS) / STEP * STEP : a.R;
+    const int begin = tile * ROW_KEYS < reach.keys ? from(tile * ROW_KEYS) / STEP * STEP : a.R;
 
     const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
     const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv, a.inverse};
@@ -330,63 +339,67 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     };
     int row = begin;
     for (; row + STEP <= wave_any && row < a.R; row += STEP) tile_of(row, [] {});        // rows that see none of the wave's keys
-    for (; row < a.R; row += STEP)
-        tile_of(row, [&] {
-            const bool limited = row < wave_all;
-            Acc<TR> da[BLOCKS<TR>];
-            float p[2][REGS<TR>];
+    const auto scores = [&](int m, int blk, auto limited, float (&p)[REGS<TR>]) {      // probabilities of one map
+        Acc<TR> s;
+        clear<TR>(s);
 #pragma unroll
-            for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-                clear<TR>(da[blk]);
+        for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+            mma<TR>(row_frag<T, TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR + lane_row<TR>(), kk), k[m][kk], s);
 #pragma unroll
-                for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
-                    mma<TR>(row_frag<T, TR>(g_tile[at], StageG::PITCH, blk * TR + lane_row<TR>(), kk), v[kk], da[blk]);
+        for (int i = 0; i < TR * TR / 64; ++i) {
+            const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
+            p[f] = __builtin_amdgcn_exp2f(fmaf(s[i], c, planes[at][m ? MINUS_SUM2 : MINUS_SUM1][n]));
+            if (decltype(limited)::value && row + n < lane_from) p[f] = 0.0f;
+            if (m) p[f] *= planes[at][LAMBDA][n];       // the second map's with lambda
+        }
+    };
+    const auto use = [&](auto limited) {
+        Acc<TR> da[BLOCKS<TR>];
+        float p[2][REGS<TR>];
+#pragma unroll
+        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+            clear<TR>(da[blk]);
+#pragma unroll
+            for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
+                mma<TR>(row_frag<T, TR>(g_tile[at], StageG::PITCH, blk * TR + lane_row<TR>(), kk), v[kk], da[blk]);
+        }
+        const auto add_keys = [&](int m) {
+            Frag<T> frag[FRAGS<T, TR>];
+#pragma unroll
+            for (int f = 0; f < REGS<TR>; ++f) {
+                const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[at][m ? DOT2 : DOT1][index_of<TR>(f)];
+                p[m][f] = (m ? -p[m][f] : p[m][f]) * d;
             }
+            to_frags<T, TR>(p[m], frag);
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int blk = 0; blk < D / TR; ++blk)
 #pragma unroll
-                for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
-                    Acc<TR> s;
-                    clear<TR>(s);
+                for (int j = 0; j < FRAGS<T, TR>; ++j)
+                    mma<TR>(column_frag<TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR, j), frag[j], dk[m][blk]);
+        };
 #pragma unroll
-                    for (int kk = 0; kk < D / KS<T, TR>; ++kk)
-                        mma<TR>(row_frag<T, TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR + lane_row<TR>(), kk), k[m][kk], s);
+        for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                    for (int i = 0; i < TR * TR / 64; ++i) {
-                        const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
-                        float t = __builtin_amdgcn_exp2f(fmaf(s[i], c, planes[at][m ? MINUS_SUM2 : MINUS_SUM1][n]));
-                        if (limited && row + n < lane_from) t = 0.0f;
-                        p[m][f] = m ? t * planes[at][LAMBDA][n] : t;       // the second map's with lambda
-                    }
-                }
-            {
-                float diff[REGS<TR>];
-                Frag<T> frag[FRAGS<T, TR>];
+            for (int blk = 0; blk < BLOCKS<TR>; ++blk) scores(m, blk, limited, p[m]);
+        }
+        {
+            float diff[REGS<TR>];
+            Frag<T> frag[FRAGS<T, TR>];
 #pragma unroll
-                for (int f = 0; f < REGS<TR>; ++f) diff[f] = p[0][f] - p[1][f];
-                to_frags<T, TR>(diff, frag);
+            for (int f = 0; f < REGS<TR>; ++f) diff[f] = p[0][f] - p[1][f];
+            to_frags<T, TR>(diff, frag);
 #pragma unroll
-                for (int blk = 0; blk < DV / TR; ++blk)
+            for (int blk = 0; blk < DV / TR; ++blk)
 #pragma unroll
-                    for (int j = 0; j < FRAGS<T, TR>; ++j) mma<TR>(column_frag<TR>(g_tile[at], StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
-            }
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                float ds[REGS<TR>];
-                Frag<T> frag[FRAGS<T, TR>];
-#pragma unroll
-                for (int f = 0; f < REGS<TR>; ++f) {
-                    const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[at][m ? DOT2 : DOT1][index_of<TR>(f)];
-                    ds[f] = (m ? -p[m][f] : p[m][f]) * d;
-                }
-                to_frags<T, TR>(ds, frag);
-#pragma unroll
-                for (int blk = 0; blk < D / TR; ++blk)
-#pragma unroll
-                    for (int j = 0; j < FRAGS<T, TR>; ++j)
-                        mma<TR>(column_frag<TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR, j), frag[j], dk[m][blk]);
-            }
-        });
+                for (int j = 0; j < FRAGS<T, TR>; ++j) mma<TR>(column_frag<TR>(g_tile[at], StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
+        }
+        add_keys(0);
+        add_keys(1);
+    };
+    // Rows that a limit cuts and rows that it does not have loops of their own, and so have the rows before them: a condition in the loop has
+    // the accumulators copied in every turn (2 x 4096 causal bf16: 348 us with conditions, 252 in loops).
+    for (; row < wave_all && row < a.R; row += STEP) tile_of(row, [&] { use(std::true_type()); });
+    for (; row < a.R; row += STEP) tile_of(row, [&] { use(std::false_type()); });
     if (key >= a.Lk) return;
     const int64_t place = ((int64_t)b * a.Lk + key) * a.Hkv + hk;
     if (g.dk) {
