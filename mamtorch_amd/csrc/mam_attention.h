@@ -127,7 +127,7 @@ __device__ __forceinline__ int index_of(int f) { return (f / 4) * 4 * GROUPS<TR>
 
 // Where row `row` of a tile stands in LDS.  A pitch is 4 words more than a multiple of 32, so rows that follow each other are 4 banks apart: right for
 // the 16-byte reads of 16 rows.  The transposing read takes 4 rows of 16 words at a time: 4 consecutive ones stand 4 rows, 16 banks, apart.  fp32 columns
-// are read a row a lane group and have their rows in order.  (Rows in order in all types: profiles count 3 cycles of conflicts for one of reads.)
+// are read a row a lane group and have their rows in order.  No conflicts are counted in either type's loops.
 template <class T>
 __device__ __forceinline__ int place_of(int row)
 {
@@ -363,6 +363,34 @@ __device__ __forceinline__ void load_rows(const Source<T> &src, int row, bool th
         if (there && c < src.width) f[kk] = load_frag<T>(p + c, src.width - c);
     }
 }
+
+// What a workgroup of four waves with TR rows each knows of its rows and of the keys that they see.
+template <int TR>
+struct Place {
+    int b, hk, wave, row, query, head, limit, wave_all, wave_any, end;
+    bool there;
+
+    __device__ __forceinline__ Place(const Call &a, int row_tiles)
+    {
+        const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, row_tiles, true, gridDim.x);
+        b = bh / a.Hkv;
+        hk = bh % a.Hkv;
+        const Reach reach = reach_of(a, b);
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int first = tile * 4 * TR + wave * TR;
+        row = first + lane_row<TR>();
+        there = row < a.R;
+        query = there ? row / a.G : 0;
+        head = hk * a.G + (there ? row - query * a.G : 0);
+        limit = there ? reach.of_query(query) : 0;
+        // the keys that every row of the wave sees, and that some row of it and of the workgroup sees
+        const int wave_last = first + TR - 1 < a.R ? first + TR - 1 : a.R - 1;
+        wave_all = first < a.R ? reach.of_query(first / a.G) : 0;
+        wave_any = first < a.R ? reach.of_query(wave_last / a.G) : 0;
+        const int last = tile * 4 * TR + 4 * TR - 1 < a.R ? tile * 4 * TR + 4 * TR - 1 : a.R - 1;
+        end = reach.of_query(last / a.G);
+    }
+};
 
 // Which of keys first .. first + 31 the mask leaves, one bit each.
 __device__ __forceinline__ uint32_t mask_word(const Call &a, int b, int first)

@@ -114,111 +114,95 @@ constexpr int WAVES = DV * TR / 32 + D * TR * (int)sizeof(T) / 128 <= 160 ? 2 : 
 template <class T, int TR, int D, int DV, bool FAST>
 __global__ __launch_bounds__(256, (WAVES<T, TR, D, DV>)) void tiles_kernel(const Call a, const ForwardOut out, int row_tiles)
 {
-    constexpr int ROWS = 4 * TR, BUFFERS = TILES<T, D, DV>;
+    constexpr int BUFFERS = TILES<T, D, DV>;
     typedef Stage<T, 256, KT, 2, D, FAST> StageK;
     typedef Stage<T, 256, KT, 1, DV, FAST> StageV;
     __shared__ __attribute__((aligned(16))) T k_tile[BUFFERS][KT * StageK::PITCH];
     __shared__ __attribute__((aligned(16))) T v_tile[BUFFERS][KT * StageV::PITCH];
-    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, row_tiles, true, gridDim.x);
-    const int b = bh / a.Hkv, hk = bh % a.Hkv;
-    const Reach reach = reach_of(a, b);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = tile * ROWS + wave * TR, row = first + lane_row<TR>();
-    const bool there = row < a.R;
-    const int query = there ? row / a.G : 0, head = hk * a.G + (there ? row - query * a.G : 0);
-    const int limit = there ? reach.of_query(query) : 0;
-    // the keys that every row of the wave sees, and that some row of it and of the workgroup sees
-    const int wave_last = first + TR - 1 < a.R ? first + TR - 1 : a.R - 1;
-    const int wave_all = first < a.R ? reach.of_query(first / a.G) : 0, wave_any = first < a.R ? reach.of_query(wave_last / a.G) : 0;
-    const int last = tile * ROWS + ROWS - 1 < a.R ? tile * ROWS + ROWS - 1 : a.R - 1;
-    const int end = reach.of_query(last / a.G);
+    const Place<TR> at(a, row_tiles);
 
-    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
-    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d, 1.0f};
-    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv, 1.0f};
+    const Source<T> qs{static_cast<const T *>(a.q) + at.b * a.qb + (int64_t)at.hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
+    const Source<T> ks{static_cast<const T *>(a.k) + at.b * a.kb + at.hk * a.kh, a.kl, 0, a.km, 1, a.d, 1.0f};
+    const Source<T> vs{static_cast<const T *>(a.v) + at.b * a.vb + at.hk * a.vh, a.vl, 0, 0, 1, a.dv, 1.0f};
     Frag<T> q[2][D / KS<T, TR>];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
+    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, at.row, at.there, m, q[m]);
     const float c = a.scale * LOG2E;
 
     State<T, TR, D, DV, !FAST> state;
     state.clear();
     // a key that nobody sees is zeros in LDS, whatever its memory holds
-    const auto seen = [&](int key) { return !a.mask || a.mask[b * a.mask_b + key] != 0; };
+    const auto seen = [&](int key) { return !a.mask || a.mask[at.b * a.mask_b + key] != 0; };
     StageK k_stage;
     StageV v_stage;
-    k_stage.load(ks, 0, end, seen);
-    v_stage.load(vs, 0, end, seen);
+    k_stage.load(ks, 0, at.end, seen);
+    v_stage.load(vs, 0, at.end, seen);
     if (BUFFERS == 2) {
         k_stage.store(k_tile[0]);
         v_stage.store(v_tile[0]);
     }
     // A tile's part of the loop: `use` is what a wave that sees some of its keys does.  Waves that are past their keys go on loading for the others, in a
     // loop of its own (a condition around the products has the accumulators copied in every tile).
-    int at = 0;
+    int now = 0;
     const auto tile_of = [&](int key, const auto &use) {
-        const bool more = key + KT < end;
+        const bool more = key + KT < at.end;
         if (BUFFERS == 1) {
             __syncthreads();
             k_stage.store(k_tile[0]);
             v_stage.store(v_tile[0]);
         }
         if (more) {
-            k_stage.load(ks, key + KT, end, seen);
-            v_stage.load(vs, key + KT, end, seen);
+            k_stage.load(ks, key + KT, at.end, seen);
+            v_stage.load(vs, key + KT, at.end, seen);
         }
         __syncthreads();
         use();
         if (BUFFERS == 2) {
-            at ^= 1;
+            now ^= 1;
             if (more) {         // the other tile: every wave is past it
-                k_stage.store(k_tile[at]);
-                v_stage.store(v_tile[at]);
+                k_stage.store(k_tile[now]);
+                v_stage.store(v_tile[now]);
             }
         }
     };
     int key = 0;
     if (FAST || !a.mask)
-        for (; key + KT <= wave_all; key += KT)
-            tile_of(key, [&] { state.template keys<false>(q, k_tile[at], StageK::PITCH, v_tile[at], StageV::PITCH, c, 0, 0); });
-    for (; key < wave_any; key += KT)
+        for (; key + KT <= at.wave_all; key += KT)
+            tile_of(key, [&] { state.template keys<false>(q, k_tile[now], StageK::PITCH, v_tile[now], StageV::PITCH, c, 0, 0); });
+    for (; key < at.wave_any; key += KT)
         tile_of(key, [&] {
-            const uint32_t word = !FAST && a.mask ? mask_word(a, b, key) : 0xffffffffu;
-            state.template keys<true>(q, k_tile[at], StageK::PITCH, v_tile[at], StageV::PITCH, c, limit - key, word);
+            const uint32_t word = !FAST && a.mask ? mask_word(a, at.b, key) : 0xffffffffu;
+            state.template keys<true>(q, k_tile[now], StageK::PITCH, v_tile[now], StageV::PITCH, c, at.limit - key, word);
         });
-    for (; key < end; key += KT) tile_of(key, [] {});
-    if (!there) return;
-    const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
+    for (; key < at.end; key += KT) tile_of(key, [] {});
+    if (!at.there) return;
+    const float lam = lambda_of(a, at.head, static_cast<const T *>(nullptr));
     float inv[2], total[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         total[m] = groups_sum<TR>(state.sum[m]);
         inv[m] = total[m] > 0.0f ? 1.0f / total[m] : 0.0f;         // a row that sees nothing is zeros
     }
-    const int64_t place = (((int64_t)b * a.Lq + query) * a.H + head) * a.dv, plane = (int64_t)a.B * a.Lq * a.H * a.dv;
+    const int64_t place = (((int64_t)at.b * a.Lq + at.query) * a.H + at.head) * a.dv;
 #pragma unroll
     for (int blk = 0; blk < DV / TR; ++blk)
 #pragma unroll
         for (int f = 0; f < TR * TR / 64; f += 4) {
             const int col = blk * TR + (f / 4) * 4 * GROUPS<TR> + 4 * lane_group<TR>();
             if (col >= a.dv) continue;
-            float o[4], o1[4], o2[4];
+            float o[4], o2[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                o1[u] = state.o[0][blk][f + u] * inv[0];
                 o2[u] = state.o[1][blk][f + u] * inv[1];
-                o[u] = fmaf(-lam, o2[u], o1[u]);
+                o[u] = fmaf(-lam, o2[u], state.o[0][blk][f + u] * inv[0]);
             }
             store_pack<T, 4>(static_cast<T *>(out.out) + place + col, a.dv - col, o);
-            if (out.kept) {
-                store_pack<float, 4>(out.kept + place + col, a.dv - col, o2);
-                if (KEPT<T> == 2) store_pack<float, 4>(out.kept + plane + place + col, a.dv - col, o1);
-            }
+            if (out.kept) store_pack<float, 4>(out.kept + place + col, a.dv - col, o2);
         }
     if (out.lse && lane_group<TR>() == 0) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-            out.lse[(((int64_t)m * a.B + b) * a.H + head) * a.Lq + query] = total[m] > 0.0f ? state.top[m] + log2f(total[m]) : INFINITY;
+            out.lse[(((int64_t)m * a.B + at.b) * a.H + at.head) * a.Lq + at.query] = total[m] > 0.0f ? state.top[m] + log2f(total[m]) : INFINITY;
     }
 }
 
@@ -230,34 +214,6 @@ __global__ __launch_bounds__(256, (WAVES<T, TR, D, DV>)) void tiles_kernel(const
 // as many.  A training forward brings P2's product with the values as well, which the backward reads.
 //
 // A is scaled by g = min(the larger sum, 2^12) so that fp16 holds the probabilities of long rows as normal numbers.
-
-// What a workgroup of either pass knows of its rows and keys.
-template <int TR>
-struct Place {
-    int b, hk, wave, row, query, head, limit, wave_all, wave_any, end;
-    bool there;
-
-    __device__ __forceinline__ Place(const Call &a, int row_tiles)
-    {
-        const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, row_tiles, true, gridDim.x);
-        b = bh / a.Hkv;
-        hk = bh % a.Hkv;
-        const Reach reach = reach_of(a, b);
-        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int first = tile * 4 * TR + wave * TR;
-        row = first + lane_row<TR>();
-        there = row < a.R;
-        query = there ? row / a.G : 0;
-        head = hk * a.G + (there ? row - query * a.G : 0);
-        limit = there ? reach.of_query(query) : 0;
-        // the keys that every row of the wave sees, and that some row of it and of the workgroup sees
-        const int wave_last = first + TR - 1 < a.R ? first + TR - 1 : a.R - 1;
-        wave_all = first < a.R ? reach.of_query(first / a.G) : 0;
-        wave_any = first < a.R ? reach.of_query(wave_last / a.G) : 0;
-        const int last = tile * 4 * TR + 4 * TR - 1 < a.R ? tile * 4 * TR + 4 * TR - 1 : a.R - 1;
-        end = reach.of_query(last / a.G);
-    }
-};
 
 // Both maps' scores of 32 keys.
 template <class T, int TR, int D>

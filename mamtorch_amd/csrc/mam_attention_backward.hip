@@ -133,35 +133,24 @@ __device__ __forceinline__ void store_columns(T *p, int left, const Acc<TR> &c, 
 template <class T, int TR, int D, int DV, bool FAST>
 __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_kernel(const BackwardCall g, int row_tiles)
 {
-    constexpr int ROWS = 4 * TR, BUFFERS = TILES<T, D, DV>;
+    constexpr int BUFFERS = TILES<T, D, DV>;
     typedef Stage<T, 256, STEP, 2, D, FAST> StageK;
     typedef Stage<T, 256, STEP, 1, DV, FAST> StageV;
     __shared__ __attribute__((aligned(16))) T k_tile[BUFFERS][STEP * StageK::PITCH];
     __shared__ __attribute__((aligned(16))) T v_tile[BUFFERS][STEP * StageV::PITCH];
     const Call &a = g.a;
-    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, row_tiles, true, gridDim.x);
-    const int b = bh / a.Hkv, hk = bh % a.Hkv;
-    const Reach reach = reach_of(a, b);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = tile * ROWS + wave * TR, row = first + lane_row<TR>();
-    const bool there = row < a.R;
-    const int query = there ? row / a.G : 0, head = hk * a.G + (there ? row - query * a.G : 0);
-    const int limit = there ? reach.of_query(query) : 0;
-    const int wave_last = first + TR - 1 < a.R ? first + TR - 1 : a.R - 1;
-    const int wave_all = first < a.R ? reach.of_query(first / a.G) : 0, wave_any = first < a.R ? reach.of_query(wave_last / a.G) : 0;
-    const int last = tile * ROWS + ROWS - 1 < a.R ? tile * ROWS + ROWS - 1 : a.R - 1;
-    const int end = reach.of_query(last / a.G);
+    const Place<TR> at(a, row_tiles);
 
-    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
-    const Source<T> gs{static_cast<const T *>(g.dout) + b * g.gb + (int64_t)hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv, a.inverse};
-    const Source<T> ks{static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, a.kl, 0, a.km, 1, a.d, 1.0f};
-    const Source<T> vs{static_cast<const T *>(a.v) + b * a.vb + hk * a.vh, a.vl, 0, 0, 1, a.dv, 1.0f};
+    const Source<T> qs{static_cast<const T *>(a.q) + at.b * a.qb + (int64_t)at.hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
+    const Source<T> gs{static_cast<const T *>(g.dout) + at.b * g.gb + (int64_t)at.hk * a.G * g.gh, g.gl, g.gh, 0, a.G, a.dv, a.inverse};
+    const Source<T> ks{static_cast<const T *>(a.k) + at.b * a.kb + at.hk * a.kh, a.kl, 0, a.km, 1, a.d, 1.0f};
+    const Source<T> vs{static_cast<const T *>(a.v) + at.b * a.vb + at.hk * a.vh, a.vl, 0, 0, 1, a.dv, 1.0f};
     Frag<T> q[2][D / KS<T, TR>], grad[DV / KS<T, TR>];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
-    load_rows<T, TR, DV>(gs, row, there, 0, grad);
+    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, at.row, at.there, m, q[m]);
+    load_rows<T, TR, DV>(gs, at.row, at.there, 0, grad);
     const int64_t count = (int64_t)a.B * a.Hkv * a.R;
-    const float *plane = g.rows + (int64_t)bh * a.R + (there ? row : 0);
+    const float *plane = g.rows + ((int64_t)at.b * a.Hkv + at.hk) * a.R + (at.there ? at.row : 0);
     const float minus_sum[2] = {plane[MINUS_SUM1 * count], plane[MINUS_SUM2 * count]};
     const float dot[2] = {plane[DOT1 * count], plane[DOT2 * count]}, weight[2] = {1.0f, -plane[LAMBDA * count]};
     const float c = a.scale * LOG2E;
@@ -171,35 +160,35 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int blk = 0; blk < D / TR; ++blk) clear<TR>(dq[m][blk]);
-    const auto seen = [&](int key) { return !a.mask || a.mask[b * a.mask_b + key] != 0; };
+    const auto seen = [&](int key) { return !a.mask || a.mask[at.b * a.mask_b + key] != 0; };
     StageK k_stage;
     StageV v_stage;
-    k_stage.load(ks, 0, end, seen);
-    v_stage.load(vs, 0, end, seen);
+    k_stage.load(ks, 0, at.end, seen);
+    v_stage.load(vs, 0, at.end, seen);
     if (BUFFERS == 2) {
         k_stage.store(k_tile[0]);
         v_stage.store(v_tile[0]);
     }
     // a tile's part of the loop, and a wave that is past its keys in a loop of its own, as in the forward
-    int at = 0;
+    int now = 0;
     const auto tile_of = [&](int key, const auto &use) {
-        const bool more = key + STEP < end;
+        const bool more = key + STEP < at.end;
         if (BUFFERS == 1) {
             __syncthreads();
             k_stage.store(k_tile[0]);
             v_stage.store(v_tile[0]);
         }
         if (more) {
-            k_stage.load(ks, key + STEP, end, seen);
-            v_stage.load(vs, key + STEP, end, seen);
+            k_stage.load(ks, key + STEP, at.end, seen);
+            v_stage.load(vs, key + STEP, at.end, seen);
         }
         __syncthreads();
         use();
         if (BUFFERS == 2) {
-            at ^= 1;
+            now ^= 1;
             if (more) {
-                k_stage.store(k_tile[at]);
-                v_stage.store(v_tile[at]);
+                k_stage.store(k_tile[now]);
+                v_stage.store(v_tile[now]);
             }
         }
     };
@@ -211,7 +200,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
             clear<TR>(da[blk]);
 #pragma unroll
             for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
-                mma<TR>(row_frag<T, TR>(v_tile[at], StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
+                mma<TR>(row_frag<T, TR>(v_tile[now], StageV::PITCH, blk * TR + lane_row<TR>(), kk), grad[kk], da[blk]);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -222,12 +211,12 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
                 clear<TR>(s);
 #pragma unroll
                 for (int kk = 0; kk < D / KS<T, TR>; ++kk)
-                    mma<TR>(row_frag<T, TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
+                    mma<TR>(row_frag<T, TR>(k_tile[now] + m * D, StageK::PITCH, blk * TR + lane_row<TR>(), kk), q[m][kk], s);
 #pragma unroll
                 for (int i = 0; i < TR * TR / 64; ++i) {
                     const int f = blk * (TR * TR / 64) + i, n = index_of<TR>(f);
                     float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
-                    if (decltype(limited)::value && !(n < limit - key && (FAST || (word >> n & 1)))) p = 0.0f;
+                    if (decltype(limited)::value && !(n < at.limit - key && (FAST || (word >> n & 1)))) p = 0.0f;
                     ds[f] = p * (da[blk][i] - dot[m]);          // the second map's factor -lambda is a row's: it comes at the end
                 }
             }
@@ -237,15 +226,15 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
             for (int blk = 0; blk < D / TR; ++blk)
 #pragma unroll
                 for (int j = 0; j < FRAGS<T, TR>; ++j)
-                    mma<TR>(column_frag<TR>(k_tile[at] + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
+                    mma<TR>(column_frag<TR>(k_tile[now] + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
         }
     };
     if (FAST || !a.mask)
-        for (; key + STEP <= wave_all; key += STEP) tile_of(key, [&] { use(std::false_type(), 0); });
-    for (; key < wave_any; key += STEP) tile_of(key, [&] { use(std::true_type(), !FAST && a.mask ? mask_word(a, b, key) : 0xffffffffu); });
-    for (; key < end; key += STEP) tile_of(key, [] {});
-    if (!there) return;
-    T *out = static_cast<T *>(g.dq) + (((int64_t)b * a.Lq + query) * a.H + head) * 2 * a.d;
+        for (; key + STEP <= at.wave_all; key += STEP) tile_of(key, [&] { use(std::false_type(), 0); });
+    for (; key < at.wave_any; key += STEP) tile_of(key, [&] { use(std::true_type(), !FAST && a.mask ? mask_word(a, at.b, key) : 0xffffffffu); });
+    for (; key < at.end; key += STEP) tile_of(key, [] {});
+    if (!at.there) return;
+    T *out = static_cast<T *>(g.dq) + (((int64_t)at.b * a.Lq + at.query) * a.H + at.head) * 2 * a.d;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll

@@ -60,6 +60,11 @@ template <int N>
 __device__ __forceinline__ void keep_factors(const Dropout &d, uint64_t offset, uint64_t i, bool whole_groups, float (&f)[N])
 {
     static_assert(N % 4 == 0, "whole groups");
+    if (d.least == 0 && !d.none) {          // nothing is dropped: no words
+#pragma unroll
+        for (int u = 0; u < N; ++u) f[u] = d.scale;
+        return;
+    }
     uint32_t w[N + 4];
     const uint64_t g = i >> 2;
 #pragma unroll

@@ -94,15 +94,14 @@ __device__ __forceinline__ void row_sums(float &a, float &b, float *scratch)
 
 // A lane's piece of a join's sum, rounded to the type that it is handed on in: the norm is that of what is returned.
 template <class T>
-__device__ __forceinline__ void join_piece(const Args &a, int64_t row, int c, uint64_t offset, float (&v)[kPack<T>])
+__device__ __forceinline__ void join_piece(const Args &a, int64_t row, int c, uint64_t offset, const Raw<T> &residual, const Raw<T> &x,
+                                           float (&v)[kPack<T>])
 {
     constexpr int N = kPack<T>;
-    float x[N], f[N];
-    load_pack<T>(static_cast<const T *>(a.residual) + row * a.ldr + c, a.C - c, v);
-    load_pack<T>(static_cast<const T *>(a.x) + row * a.ldx + c, a.C - c, x);
+    float f[N];
     keep_factors<N>(a.drop, offset, (uint64_t)row * (uint64_t)a.C + (uint64_t)c, ((uint32_t)row * (uint32_t)a.C & 3) == 0, f);
 #pragma unroll
-    for (int u = 0; u < N; ++u) v[u] = (float)(T)(v[u] + keep_value(x[u], f[u]));
+    for (int u = 0; u < N; ++u) v[u] = (float)(T)((float)residual[u] + keep_value((float)x[u], f[u]));
     store_pack<T>(static_cast<T *>(a.s) + row * a.C + c, a.C - c, v);
 }
 
@@ -116,12 +115,21 @@ __global__ __launch_bounds__(THREADS_OF<LANES>) void norm_kernel(const Args a)
     if (row >= a.N) return;                     // rows of more than a wave: a workgroup's, which leaves as a whole
     const uint64_t offset = JOIN ? dropout_offset(a.drop) : 0;
     float v[PACKS][N];
+    Raw<T> residual[PACKS], x[PACKS];
+    if (JOIN) {         // all of them before the first store of s, which could be one of them for all that the compiler knows
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+            const int c = (lane + i * LANES) * N;
+            residual[i] = load_raw<T>(static_cast<const T *>(a.residual) + row * a.ldr + c, a.C - c);
+            x[i] = load_raw<T>(static_cast<const T *>(a.x) + row * a.ldx + c, a.C - c);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
         const int c = (lane + i * LANES) * N;
         if (JOIN) {
             if (c < a.C) {
-                join_piece<T>(a, row, c, offset, v[i]);
+                join_piece<T>(a, row, c, offset, residual[i], x[i], v[i]);
             } else {
 #pragma unroll
                 for (int u = 0; u < N; ++u) v[i][u] = 0.0f;
@@ -188,7 +196,9 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const Args a)
     float sum = 0.0f;
     for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
         float v[N];
-        if (JOIN) join_piece<T>(a, row, c, offset, v);
+        if (JOIN)
+            join_piece<T>(a, row, c, offset, load_raw<T>(static_cast<const T *>(a.residual) + row * a.ldr + c, a.C - c),
+                          load_raw<T>(static_cast<const T *>(a.x) + row * a.ldx + c, a.C - c), v);
         else load_pack<T>(src + c, a.C - c, v);
 #pragma unroll
         for (int u = 0; u < N; ++u) sum += c + u < a.C ? v[u] : 0.0f;
@@ -221,17 +231,20 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const Args a)
     }
 }
 
+// A piece of the sum's own gradient, zeros where it has none.
+template <class T>
+__device__ __forceinline__ Raw<T> load_ds(const BackwardArgs &a, int64_t row, int c)
+{
+    return load_raw<T>(static_cast<const T *>(a.ds) + row * a.lddsum + c, a.ds ? a.C - c : 0);
+}
+
 // What leaves a join's backward for elements c .. of a row: the gradient of the sum, and behind the dropout.
 template <class T>
-__device__ __forceinline__ void join_out(const BackwardArgs &a, int64_t row, int c, uint64_t offset, float (&g)[kPack<T>])
+__device__ __forceinline__ void join_out(const BackwardArgs &a, int64_t row, int c, uint64_t offset, const Raw<T> &ds, float (&g)[kPack<T>])
 {
     constexpr int N = kPack<T>;
-    if (a.ds) {
-        float ds[N];
-        load_pack<T>(static_cast<const T *>(a.ds) + row * a.lddsum + c, a.C - c, ds);
 #pragma unroll
-        for (int u = 0; u < N; ++u) g[u] += ds[u];
-    }
+    for (int u = 0; u < N; ++u) g[u] += (float)ds[u];
     if (a.dx) store_pack<T>(static_cast<T *>(a.dx) + row * a.C + c, a.C - c, g);
     if (a.dropped) {
         float f[N];
@@ -292,6 +305,11 @@ __global__ __launch_bounds__(THREADS_OF<LANES>) void norm_backward_kernel(const 
                 dy[i][u] = (float)next_dy[i][u];
                 xh[i][u] = (float)next_x[i][u];
             }
+        Raw<T> ds[JOIN ? PACKS : 1];
+        if (JOIN) {
+#pragma unroll
+            for (int i = 0; i < PACKS; ++i) ds[i] = load_ds<T>(a, row, (lane + i * LANES) * N);
+        }
         if (AHEAD && row + step < a.N) load_row(row + step);
         float sum = 0.0f, dot = 0.0f;
 #pragma unroll
@@ -314,7 +332,7 @@ __global__ __launch_bounds__(THREADS_OF<LANES>) void norm_backward_kernel(const 
             if (c >= a.C) continue;
 #pragma unroll
             for (int u = 0; u < N; ++u) dy[i][u] = rstd * (dy[i][u] - sum - xh[i][u] * dot);
-            if (JOIN) join_out<T>(a, row, c, offset, dy[i]);
+            if (JOIN) join_out<T>(a, row, c, offset, ds[i], dy[i]);
             else if (a.dx) store_pack<T>(static_cast<T *>(a.dx) + row * a.C + c, a.C - c, dy[i]);
         }
     }
@@ -376,7 +394,7 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const Backward
                 }
             }
             if (!pass) continue;
-            if (JOIN) join_out<T>(a, row, c, offset, g);
+            if (JOIN) join_out<T>(a, row, c, offset, load_ds<T>(a, row, c), g);
             else if (a.dx) store_pack<T>(static_cast<T *>(a.dx) + row * a.C + c, a.C - c, g);
         }
         if (!pass) {
