@@ -93,6 +93,10 @@ constexpr int KS = FE<T> * GROUPS<TR>;      // contraction length of a fragment 
 template <class T, int TR>
 constexpr int FRAGS = REGS<TR> / FE<T>;     // fragments that 32 contraction terms fill
 
+// Where 16 values of a contraction are whole fragments (fp32) a last tile of 16 keys or rows or less is half a tile's work: 197 keys are 13 of 14 halves.
+template <class T, int TR>
+constexpr bool HALVES = BLOCKS<TR> == 2 && FRAGS<T, TR> % 2 == 0;
+
 // acc += A B over KS terms
 template <int TR>
 __device__ __forceinline__ void mma(const Frag<bf16> &a, const Frag<bf16> &b, Acc<TR> &c)
@@ -168,10 +172,10 @@ __device__ __forceinline__ Frag<T> column_frag(const T *tile, int pitch, int col
 
 // 32 x TR values as the fragments of a contraction over the 32.
 template <class T, int TR>
-__device__ __forceinline__ void to_frags(const float (&p)[REGS<TR>], Frag<T> (&f)[FRAGS<T, TR>])
+__device__ __forceinline__ void to_frags(const float (&p)[REGS<TR>], Frag<T> (&f)[FRAGS<T, TR>], int count = FRAGS<T, TR>)
 {
 #pragma unroll
-    for (int j = 0; j < FRAGS<T, TR>; ++j)
+    for (int j = 0; j < count; ++j)
 #pragma unroll
         for (int u = 0; u < FE<T>; ++u) f[j][u] = (T)p[j * FE<T> + u];
 }

@@ -6,6 +6,8 @@
 // two for each (query, key), 16 cycles of a wave for 64 of them.
 #include "mam_attention.h"
 
+#include <type_traits>
+
 namespace mam {
 namespace attention {
 
@@ -39,12 +41,12 @@ struct State {
     }
 
     // Scores of one map (32 keys x TR rows) to probabilities relative to `top`, which rises first where it has to.
-    template <bool LIMITED>
+    template <bool LIMITED, int USED>
     __device__ __forceinline__ void softmax(int m, const Acc<TR> (&s)[BLOCKS<TR>], float c, int limit, uint32_t word, float (&p)[REGS<TR>])
     {
         float most = -INFINITY;
 #pragma unroll
-        for (int f = 0; f < REGS<TR>; ++f) {
+        for (int f = 0; f < USED; ++f) {
             float v = s[f / (TR * TR / 64)][f % (TR * TR / 64)];
             if constexpr (LIMITED) {
                 const int key = index_of<TR>(f);
@@ -67,24 +69,25 @@ struct State {
         const float base = top[m] == -INFINITY ? 0.0f : top[m];
         float add = 0.0f;
 #pragma unroll
-        for (int f = 0; f < REGS<TR>; ++f) {
+        for (int f = 0; f < USED; ++f) {
             p[f] = __builtin_amdgcn_exp2f(fmaf(p[f], c, -base));
             add += p[f];
         }
         sum[m] += add;
     }
 
-    // 32 keys: their scores, probabilities, and the products with their values.
-    template <bool LIMITED>
+    // 32 keys (the first 16: HALF): their scores, probabilities, and the products with their values.
+    template <bool LIMITED, bool HALF>
     __device__ __forceinline__ void keys(const Frag<T> (&q)[2][D / KS<T, TR>], const T *k_tile, int k_pitch, const T *v_tile, int v_pitch,
                                          float c, int limit, uint32_t word)
     {
+        constexpr int PART = HALF ? 2 : 1, USED = REGS<TR> / PART;
         Frag<T> frag[2][FRAGS<T, TR>];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             Acc<TR> s[BLOCKS<TR>];
 #pragma unroll
-            for (int b = 0; b < BLOCKS<TR>; ++b) {
+            for (int b = 0; b < BLOCKS<TR> / PART; ++b) {
 #pragma unroll
                 for (int i = 0; i < TR * TR / 64; ++i) s[b][i] = 0.0f;
 #pragma unroll
@@ -92,13 +95,13 @@ struct State {
                     mma<TR>(row_frag<T, TR>(k_tile + m * D, k_pitch, b * TR + lane_row<TR>(), kk), q[m][kk], s[b]);
             }
             float p[REGS<TR>];
-            softmax<LIMITED>(m, s, c, limit, word, p);
-            to_frags<T, TR>(p, frag[m]);
+            softmax<LIMITED, USED>(m, s, c, limit, word, p);
+            to_frags<T, TR>(p, frag[m], FRAGS<T, TR> / PART);
         }
 #pragma unroll
         for (int b = 0; b < DV / TR; ++b) {
 #pragma unroll
-            for (int j = 0; j < FRAGS<T, TR>; ++j) {
+            for (int j = 0; j < FRAGS<T, TR> / PART; ++j) {
                 const Frag<T> v = column_frag<TR>(v_tile, v_pitch, b * TR, j);
                 mma<TR>(v, frag[0][j], o[0][b]);
                 mma<TR>(v, frag[1][j], o[1][b]);
@@ -168,12 +171,18 @@ __global__ __launch_bounds__(256, (WAVES<T, TR, D, DV>)) void tiles_kernel(const
     int key = 0;
     if (FAST || !a.mask)
         for (; key + KT <= at.wave_all; key += KT)
-            tile_of(key, [&] { state.template keys<false>(q, k_tile[now], StageK::PITCH, v_tile[now], StageV::PITCH, c, 0, 0); });
-    for (; key < at.wave_any; key += KT)
-        tile_of(key, [&] {
-            const uint32_t word = !FAST && a.mask ? mask_word(a, at.b, key) : 0xffffffffu;
-            state.template keys<true>(q, k_tile[now], StageK::PITCH, v_tile[now], StageV::PITCH, c, at.limit - key, word);
-        });
+            tile_of(key, [&] { state.template keys<false, false>(q, k_tile[now], StageK::PITCH, v_tile[now], StageV::PITCH, c, 0, 0); });
+    const auto limited = [&](auto half) {
+        const uint32_t word = !FAST && a.mask ? mask_word(a, at.b, key) : 0xffffffffu;
+        state.template keys<true, decltype(half)::value>(q, k_tile[now], StageK::PITCH, v_tile[now], StageV::PITCH, c, at.limit - key, word);
+    };
+    constexpr int SHORT = HALVES<T, TR> ? KT / 2 : 0;
+    for (; key + SHORT < at.wave_any; key += KT) tile_of(key, [&] { limited(std::false_type()); });
+    if constexpr (SHORT > 0)
+        if (key < at.wave_any) {
+            tile_of(key, [&] { limited(std::true_type()); });
+            key += KT;
+        }
     for (; key < at.end; key += KT) tile_of(key, [] {});
     if (!at.there) return;
     const float lam = lambda_of(a, at.head, static_cast<const T *>(nullptr));

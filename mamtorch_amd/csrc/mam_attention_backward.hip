@@ -193,10 +193,11 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
         }
     };
     int key = 0;
-    const auto use = [&](auto limited, uint32_t word) {
+    const auto use = [&](auto limited, auto half, uint32_t word) {
+        constexpr int PART = decltype(half)::value ? 2 : 1;
         Acc<TR> da[BLOCKS<TR>];
 #pragma unroll
-        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+        for (int blk = 0; blk < BLOCKS<TR> / PART; ++blk) {
             clear<TR>(da[blk]);
 #pragma unroll
             for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
         for (int m = 0; m < 2; ++m) {
             float ds[REGS<TR>];
 #pragma unroll
-            for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+            for (int blk = 0; blk < BLOCKS<TR> / PART; ++blk) {
                 Acc<TR> s;
                 clear<TR>(s);
 #pragma unroll
@@ -221,17 +222,24 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
                 }
             }
             Frag<T> frag[FRAGS<T, TR>];
-            to_frags<T, TR>(ds, frag);
+            to_frags<T, TR>(ds, frag, FRAGS<T, TR> / PART);
 #pragma unroll
             for (int blk = 0; blk < D / TR; ++blk)
 #pragma unroll
-                for (int j = 0; j < FRAGS<T, TR>; ++j)
+                for (int j = 0; j < FRAGS<T, TR> / PART; ++j)
                     mma<TR>(column_frag<TR>(k_tile[now] + m * D, StageK::PITCH, blk * TR, j), frag[j], dq[m][blk]);
         }
     };
     if (FAST || !a.mask)
-        for (; key + STEP <= at.wave_all; key += STEP) tile_of(key, [&] { use(std::false_type(), 0); });
-    for (; key < at.wave_any; key += STEP) tile_of(key, [&] { use(std::true_type(), !FAST && a.mask ? mask_word(a, at.b, key) : 0xffffffffu); });
+        for (; key + STEP <= at.wave_all; key += STEP) tile_of(key, [&] { use(std::false_type(), std::false_type(), 0); });
+    const auto word_of = [&] { return !FAST && a.mask ? mask_word(a, at.b, key) : 0xffffffffu; };
+    constexpr int SHORT = HALVES<T, TR> ? STEP / 2 : 0;
+    for (; key + SHORT < at.wave_any; key += STEP) tile_of(key, [&] { use(std::true_type(), std::false_type(), word_of()); });
+    if constexpr (SHORT > 0)
+        if (key < at.wave_any) {
+            tile_of(key, [&] { use(std::true_type(), std::true_type(), word_of()); });
+            key += STEP;
+        }
     for (; key < at.end; key += STEP) tile_of(key, [] {});
     if (!at.there) return;
     T *out = static_cast<T *>(g.dq) + (((int64_t)at.b * a.Lq + at.query) * a.H + at.head) * 2 * a.d;
@@ -342,11 +350,12 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
             if (m) p[f] *= planes[at][LAMBDA][n];       // the second map's with lambda
         }
     };
-    const auto use = [&](auto limited) {
+    const auto use = [&](auto limited, auto half) {
+        constexpr int PART = decltype(half)::value ? 2 : 1;
         Acc<TR> da[BLOCKS<TR>];
         float p[2][REGS<TR>];
 #pragma unroll
-        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+        for (int blk = 0; blk < BLOCKS<TR> / PART; ++blk) {
             clear<TR>(da[blk]);
 #pragma unroll
             for (int kk = 0; kk < DV / KS<T, TR>; ++kk)
@@ -355,40 +364,43 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
         const auto add_keys = [&](int m) {
             Frag<T> frag[FRAGS<T, TR>];
 #pragma unroll
-            for (int f = 0; f < REGS<TR>; ++f) {
+            for (int f = 0; f < REGS<TR> / PART; ++f) {
                 const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[at][m ? DOT2 : DOT1][index_of<TR>(f)];
                 p[m][f] = (m ? -p[m][f] : p[m][f]) * d;
             }
-            to_frags<T, TR>(p[m], frag);
+            to_frags<T, TR>(p[m], frag, FRAGS<T, TR> / PART);
 #pragma unroll
             for (int blk = 0; blk < D / TR; ++blk)
 #pragma unroll
-                for (int j = 0; j < FRAGS<T, TR>; ++j)
+                for (int j = 0; j < FRAGS<T, TR> / PART; ++j)
                     mma<TR>(column_frag<TR>(q_tile[at] + m * D, StageQ::PITCH, blk * TR, j), frag[j], dk[m][blk]);
         };
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
-            for (int blk = 0; blk < BLOCKS<TR>; ++blk) scores(m, blk, limited, p[m]);
+            for (int blk = 0; blk < BLOCKS<TR> / PART; ++blk) scores(m, blk, limited, p[m]);
         }
         {
             float diff[REGS<TR>];
             Frag<T> frag[FRAGS<T, TR>];
 #pragma unroll
-            for (int f = 0; f < REGS<TR>; ++f) diff[f] = p[0][f] - p[1][f];
-            to_frags<T, TR>(diff, frag);
+            for (int f = 0; f < REGS<TR> / PART; ++f) diff[f] = p[0][f] - p[1][f];
+            to_frags<T, TR>(diff, frag, FRAGS<T, TR> / PART);
 #pragma unroll
             for (int blk = 0; blk < DV / TR; ++blk)
 #pragma unroll
-                for (int j = 0; j < FRAGS<T, TR>; ++j) mma<TR>(column_frag<TR>(g_tile[at], StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
+                for (int j = 0; j < FRAGS<T, TR> / PART; ++j) mma<TR>(column_frag<TR>(g_tile[at], StageG::PITCH, blk * TR, j), frag[j], dv[blk]);
         }
         add_keys(0);
         add_keys(1);
     };
     // Rows that a limit cuts and rows that it does not have loops of their own, and so have the rows before them: a condition in the loop has
     // the accumulators copied in every turn (2 x 4096 causal bf16: 348 us with conditions, 252 in loops).
-    for (; row < wave_all && row < a.R; row += STEP) tile_of(row, [&] { use(std::true_type()); });
-    for (; row < a.R; row += STEP) tile_of(row, [&] { use(std::false_type()); });
+    for (; row < wave_all && row < a.R; row += STEP) tile_of(row, [&] { use(std::true_type(), std::false_type()); });
+    constexpr int SHORT = HALVES<T, TR> ? STEP / 2 : 0;
+    for (; row + SHORT < a.R; row += STEP) tile_of(row, [&] { use(std::false_type(), std::false_type()); });
+    if constexpr (SHORT > 0)
+        if (row < a.R) tile_of(row, [&] { use(std::false_type(), std::true_type()); });
     if (key >= a.Lk) return;
     const int64_t place = ((int64_t)b * a.Lk + key) * a.Hkv + hk;
     if (g.dk) {
