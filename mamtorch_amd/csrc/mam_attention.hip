@@ -1,9 +1,12 @@
 // Differential attention, forward: out = softmax(scale Q1 K1^T) V - lambda softmax(scale Q2 K2^T) V for each head, with a
 // running maximum and sum for each of the two softmaxes and each row, so that no score leaves the registers.
 //
-// tiles: a workgroup of four waves shares tiles of 32 keys in LDS, each wave with TR rows of its own (16 or 32, mam_attention.h).
-// The next tile's loads are in flight while this one is used.  Bound by the matrix cores and, in 16-bit types, as much by the exponentials:
-// two for each (query, key), 16 cycles of a wave for 64 of them.
+// A workgroup of four waves shares tiles of 32 keys in LDS, each wave with TR rows of its own (16 or 32, mam_attention.h).  The next tile's loads are
+// in flight while this one is used.  fp32 passes over the keys once (tiles_kernel), 16-bit types twice (twice_kernel, below).
+//
+// fp32 is bound by the matrix cores: 64 images of 197 tokens, 6 heads of 64/128, 11.4 GFLOP in 159 us, 72 TFLOP/s where a large library product
+// reaches 151.  They are busy in 58 % of its cycles; a workgroup has 7 tiles only, and the rest is the loads before its first tile, which all
+// workgroups that begin together wait for at once, and its last stores.  Three waves a SIMD over one tile buffer instead of two over two: 166 -> 201 us.
 #include "mam_attention.h"
 
 #include <type_traits>
@@ -222,6 +225,11 @@ __global__ __launch_bounds__(256, (WAVES<T, TR, D, DV>)) void tiles_kernel(const
 // accumulators, nothing to scale when a maximum rises, and less work for the vector units beside the exponentials, of which there are twice
 // as many.  A training forward brings P2's product with the values as well, which the backward reads.
 //
+// Bound by the vector units and the matrix cores in turn: two exponentials a (query, key) and pass stand beside products of 16 bits.  Measured: 8 x 2048 all keys,
+// 8 heads of 64/128, bf16 356 us (206 GFLOP done, 579 TFLOP/s; a large library product reaches 1079); 2 x 4096 causal with what training keeps
+// 244 us (137 GFLOP, 564 TFLOP/s; matrix cores busy in 27 % of the cycles, vector units in about 36 %).  Deeper pipelines of the scores and queries kept in
+// LDS measured the same or slower (340 to 435 us where the first is 356).
+//
 // A is scaled by g = min(the larger sum, 2^12) so that fp16 holds the probabilities of long rows as normal numbers.
 
 // Both maps' scores of 32 keys.
@@ -256,7 +264,8 @@ __device__ __forceinline__ void hide(Acc<TR> (&s)[2][BLOCKS<TR>], int limit, uin
 template <class T, int TR, int D, int DV, bool FAST, bool KEEP>
 __global__ __launch_bounds__(256, 2) void twice_kernel(const Call a, const ForwardOut out, int row_tiles)
 {
-    constexpr int AR = TR * TR / 64, MAPS = KEEP ? 2 : 1, TURN = D <= 64 ? 2 : 1;     // two tiles of 128 elements a key leave one workgroup a CU: 138 -> 171 us
+    // TURN: two tiles between barriers measured 366 -> 354 us (8 x 2048, 64/128); of 128 elements a key they leave one workgroup a CU: 138 -> 171 us
+    constexpr int AR = TR * TR / 64, MAPS = KEEP ? 2 : 1, TURN = D <= 64 ? 2 : 1;
     typedef Stage<T, 256, KT, 2, D, FAST> StageK;
     typedef Stage<T, 256, KT, 1, DV, FAST> StageV;
     __shared__ __attribute__((aligned(16))) T k_tile[2][TURN * KT * StageK::PITCH];
@@ -495,8 +504,8 @@ extern "C" int mam_diff_attention(const mam_diff_attention_t *args, void *out, f
     const int rc = attention::fill_call(args, a);
     if (rc != MAM_OK || a.B == 0 || a.R == 0) return rc;
     if (!a.q || !a.lam || !out || (a.Lk > 0 && (!a.k || !a.v))) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
-    if (attention::use_split(a, kept != nullptr)) return attention::run_split(a, args->type, out, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
     if (!kept != !lse) return fail(MAM_ERR_INVALID_ARGUMENT, "kept and lse are wanted together");
+    if (attention::use_split(a, args->type, kept != nullptr)) return attention::run_split(a, args->type, out, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
     hipStream_t st = static_cast<hipStream_t>(stream);
     const attention::ForwardOut o{out, kept, lse};
     if (args->type == MAM_F32) return attention::with_head_sizes(a.d, a.dv, attention::Forward<float>{a, o, st});
@@ -509,5 +518,5 @@ extern "C" size_t mam_diff_attention_workspace(const mam_diff_attention_t *args)
     using namespace mam;
     attention::Call a;
     if (attention::fill_call(args, a) != MAM_OK || a.B == 0 || a.R == 0) return 0;
-    return attention::use_split(a, false) ? attention::split_workspace(a) : 0;
+    return attention::use_split(a, args->type, false) ? attention::split_workspace(a) : 0;
 }

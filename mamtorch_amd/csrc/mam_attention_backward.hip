@@ -3,10 +3,13 @@
 //   dV = A^T dO,  dA = dO V^T,  d1 = rowsum(dO O1),  d2 = rowsum(dO O2)
 //   dS1 = P1 (dA - d1),  dS2 = -lambda P2 (dA - d2),  dQm = scale dSm Km,  dKm = scale dSm^T Qm,  dlambda = -sum d2
 //
-// Three kernels: what the rows need beside the scores (sums, d1, d2, lambda), dQ by workgroups that own rows and pass over the keys, dK and dV
-// by workgroups that own keys and pass over the rows of all heads that share them.  Scores and dA are formed in both, 7 parts of
-// work instead of 5, and nothing is added to memory by more than one workgroup: no atomics, the same bits on every call.  Bound by the
-// matrix cores and, in 16-bit types, the exponentials beside them.
+// Four kernels: what the rows need beside the scores (sums, d1, d2, lambda), dQ by workgroups that own rows and pass over the keys, dK and dV
+// by workgroups that own keys and pass over the rows of all heads that share them, and dlambda.  Scores and dA are formed in both of the
+// middle ones, 7 parts of work instead of 5, and nothing is added to memory by more than one workgroup: no atomics, the same bits on every call.
+//
+// Bound by the matrix cores in fp32 and by them and the vector units in turn in 16-bit types.  Measured, fp32 64 images of 197 tokens, 6 heads of 64/128: dQ
+// 152 us (75 TFLOP/s, matrix cores busy in 60 % of the cycles), dK and dV 213 us (72 TFLOP/s, 59 %), both with the waits of short workgroups that the forward
+// has.  bf16 2 x 4096 causal, 8 heads of 64/128: dQ 160 us (644 TFLOP/s), dK and dV 253 us (544); 2 x 2048 causal of 128/256: 102 us (506), 157 us (438).
 #include "mam_attention.h"
 
 #include <type_traits>
@@ -29,7 +32,7 @@ struct BackwardCall {
     float *rows;                        // PLANES planes
 };
 
-// A row's planes: 16 lanes a row.
+// A row's planes: 16 lanes a row.  Bound by memory: 116 MB (fp32, 64 x 197 tokens of 6 x 128) in 21 us, 5.5 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
 {
@@ -69,7 +72,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     g.rows[LAMBDA * count + id] = lam;
 }
 
-// dlambda of a head, a workgroup each: its waves share the requests, or some waves a request where there are fewer.
+// dlambda of a head, a workgroup each: its waves share the requests, or some waves a request where there are fewer.  Five loads after each other and
+// the launch: 5 us.
 template <class T>
 __global__ __launch_bounds__(1024) void lambda_kernel(const BackwardCall g)
 {
@@ -259,7 +263,8 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     __shared__ __attribute__((aligned(16))) T g_tile[BUFFERS][STEP * StageG::PITCH];
     __shared__ __attribute__((aligned(16))) float planes[BUFFERS][PLANES][STEP];
     const Call &a = g.a;
-    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, KEYS_WAVES<T, TR, D, DV> == 2 ? gridDim.x : 2 * gridDim.x);
+    const int workgroups = KEYS_WAVES<T, TR, D, DV> == 2 ? gridDim.x : 2 * gridDim.x;       // as if two fit a CU
+    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, workgroups);
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
     const Reach reach = reach_of(a, b);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -394,6 +399,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
         add_keys(0);
         add_keys(1);
     };
+    // Dividing the two gradients between two passes of fewer registers costs the scores twice: 228 + 151 us where one pass takes 252.
     // Rows that a limit cuts and rows that it does not have loops of their own, and so have the rows before them: a condition in the loop has
     // the accumulators copied in every turn (2 x 4096 causal bf16: 348 us with conditions, 252 in loops).
     for (; row < wave_all && row < a.R; row += STEP) tile_of(row, [&] { use(std::true_type(), std::false_type()); });

@@ -8,6 +8,9 @@
 //
 // The ranges of a row meet in two steps, both in a fixed order: the four waves of a workgroup through LDS, and the workgroups through
 // the workspace and a second kernel where one workgroup a row would leave CUs without work.
+//
+// Measured: one token of 16 requests over caches of up to 16384 (200704 keys in all, 4 key heads of 64/128, 4 query heads each, bf16, 411 MB) 95 us, 4.3 TB/s, and 6 us
+// for the join; a large copy reaches 5.2 TB/s.  16 queries, 8 heads, over 8192 keys 13 and 11 us.
 #include "mam_attention.h"
 
 namespace mam {
@@ -26,11 +29,16 @@ inline int split_count(const Call &a)
     return n < 1 ? 1 : (int)n;
 }
 
-// Rows of one tile always; more where their workgroups of the tiles' kernels would leave half of the CUs without work.
-bool use_split(const Call &a, bool keep)
+// Rows of one tile always; more where the call's tiles of 16 rows are two a CU at most, one in 16-bit types of heads past 64: there the tiles' kernels,
+// which pass over all keys in every workgroup, leave CUs and their waves idle, and here every tile reads the keys for itself.  Both measured, tiles' -> here:
+// bf16 64/128 over 4096 keys 512 tiles 185..197 -> 84..122 us, 1024 tiles 191 -> 160 to 225 -> 369; 128/256 256 tiles 243 -> 156, 384 tiles 121 -> 154 (2048
+// keys), 512 tiles 243 -> 245; fp32 64/128 over 1024 keys 512 tiles 120 -> 97, 1024 tiles 131 -> 205; 128/256 512 tiles 945 -> 714 (causal).  Few keys
+// leave a wave too few of them: fp32, 312 tiles over 197 keys 30 -> 39 us.  16 queries of 2048 (request, head) pairs over 512 keys, bf16: 152 -> 111 us.
+bool use_split(const Call &a, int type, bool keep)
 {
     if (keep || a.Lk < 1) return false;
-    return a.R <= ROWS || (a.R <= 8 * ROWS && (int64_t)a.B * a.Hkv * ceil_div(a.R, 64) < kNumCU / 2 && a.Lk >= 512);
+    const int64_t tiles = (int64_t)a.B * a.Hkv * ceil_div(a.R, ROWS);
+    return a.R <= ROWS || (a.Lk >= 512 && tiles <= (type == MAM_F32 || (a.d <= 64 && a.dv <= 128) ? 2 : 1) * kNumCU);
 }
 
 // A partial row: both maps' products relative to their maxima, then maximum and sum of each.
@@ -337,19 +345,27 @@ __global__ __launch_bounds__(256) void join_kernel(const Call a, void *out, cons
         factor[m] = total > 0.0f ? mine / total : 0.0f;
     }
     const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
+    const int left = a.dv - 4 * lane;
     float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; ++s) {
-        const float f0 = __shfl(factor[0], s), f1 = -lam * __shfl(factor[1], s);
-        if (4 * lane < a.dv) {
-            float p1[4], p2[4];
-            load_pack<float, 4>(p + s * step + 4 * lane, a.dv - 4 * lane, p1);
-            load_pack<float, 4>(p + s * step + a.dv + 4 * lane, a.dv - 4 * lane, p2);
+    constexpr int AHEAD = 8;            // parts on their way at once
+    for (int s0 = 0; s0 < splits; s0 += AHEAD) {        // every lane stays to the end: each has a split's factors
+        float p1[AHEAD][4], p2[AHEAD][4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) r[u] = fmaf(f1, p2[u], fmaf(f0, p1[u], r[u]));
+        for (int u = 0; u < AHEAD; ++u) {
+            const float *t = p + (s0 + u < splits ? s0 + u : splits - 1) * step + 4 * lane;
+            load_pack<float, 4>(t, left, p1[u]);
+            load_pack<float, 4>(t + a.dv, left, p2[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int s = s0 + u;
+            const float f0 = s < splits ? __shfl(factor[0], s) : 0.0f, f1 = s < splits ? -lam * __shfl(factor[1], s) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = fmaf(f1, p2[u][e], fmaf(f0, p1[u][e], r[e]));
         }
     }
-    if (4 * lane < a.dv)
-        store_pack<T, 4>(static_cast<T *>(out) + (((int64_t)b * a.Lq + query) * a.H + head) * a.dv + 4 * lane, a.dv - 4 * lane, r);
+    if (left > 0)
+        store_pack<T, 4>(static_cast<T *>(out) + (((int64_t)b * a.Lq + query) * a.H + head) * a.dv + 4 * lane, left, r);
 }
 
 template <class T>

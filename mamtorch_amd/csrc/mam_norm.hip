@@ -9,6 +9,10 @@
 // what is left, all in fp32.  The backward's workgroups take rows in turn, the next one's loads on their way while this one is worked on, keep
 // their sums of dw and db in registers over all of them and write them once; a second kernel adds the workgroups' sums in a fixed order, so
 // two calls give the same bits.  Rows beyond 16384 elements are read again for each pass.
+//
+// Measured (forward, backward; a large copy reaches 5.2 TB/s): norm of 12608 x 768 fp32 17.2 and 22.2 us, 4.5 and 5.2 TB/s; of 16384 x 4096 fp16 62 and 89 us,
+// 4.3 and 4.5 TB/s; join of 12608 x 768 fp32 37.4 and 47 us, 4.1 TB/s both.  Ragged rows in 16 bits are further off: 8191 x 1030 fp16 joined take 38 and
+// 47 us, 1.8 TB/s: a wave's third piece is nearly empty, the generator forms a group more a piece, and one batch of waves holds all rows. 197 x 768: 4.5 us, the launch.
 #include "mam_counter.h"
 #include "mam_types.h"
 

@@ -308,7 +308,7 @@ Tensors diff_attention_cuda(const Tensor &q, const Tensor &k, const Tensor &v, c
     const int64_t planes = a.type == MAM_F32 ? 1 : 2;
     Tensor kept = with_sums ? at::empty({planes, a.B, a.Lq, a.H, a.Dv}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
     Tensor lse = with_sums ? at::empty({2, a.B, a.H, a.Lq}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
-    const Tensor ws = workspace_for(mam_diff_attention_workspace(&a), q);
+    const Tensor ws = workspace_for(with_sums ? 0 : mam_diff_attention_workspace(&a), q);
     check_rc(mam_diff_attention(&a, out.data_ptr(), with_sums ? kept.data_ptr<float>() : nullptr, with_sums ? lse.data_ptr<float>() : nullptr,
                                 out_ptr(ws), ws.defined() ? ws.numel() : 0, current_stream(q)),
              "mam_diff_attention");

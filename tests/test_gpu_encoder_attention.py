@@ -156,6 +156,19 @@ def test_few_queries_over_long_keys(b, lq, lk, h, hk, d, dv, dtype):
     _check(q, k, v, lam, None, backward=False, key_mask=mask)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b, lq, lk, h, hk, d, dv", [(1, 200, 600, 4, 2, 64, 128), (2, 513, 520, 2, 2, 32, 64), (2, 100, 1100, 2, 1, 128, 256),
+                                                     (1, 37, 2049, 3, 1, 50, 33)])
+def test_many_queries_of_few_requests(b, lq, lk, h, hk, d, dv, dtype):
+    q, k, v, lam, _ = _operands(b, lq, lk, h, hk, d, dv, dtype, seed=lk + 1)
+    lengths = torch.tensor([max(0, lk - 300 * i) for i in range(b)], dtype=torch.int32)
+    _check(q, k, v, lam, None, backward=False)
+    _check(q, k, v, lam, None, backward=False, causal=True)
+    _check(q, k, v, lam, None, backward=False, lengths=lengths, causal=True, starts=lengths - lq)
+    mask = torch.rand(b, lk, generator=torch.Generator().manual_seed(lk)) < 0.5
+    _check(q, k, v, lam, None, backward=False, key_mask=mask, causal=True)
+
+
 def test_lam_in_32_bits_beside_16_bit_operands():
     q, k, v, lam, dout = _operands(2, 30, 40, 4, 2, 32, 64, torch.bfloat16, seed=9)
     _check(q, k, v, lam.float(), dout)
