@@ -3,7 +3,7 @@
 //   dV = A^T dO,  dA = dO V^T,  d1 = rowsum(dO O1),  d2 = rowsum(dO O2)
 //   dS1 = P1 (dA - d1),  dS2 = -lambda P2 (dA - d2),  dQm = scale dSm Km,  dKm = scale dSm^T Qm,  dlambda = -sum d2
 //
-// Four kernels: what the rows need beside the scores (sums, d1, d2, lambda), dQ by workgroups that own rows and pass over the keys, dK and dV
+// Four kernels: what the rows need beside the scores (sums, d1, d2, lambda), dQ and the rows' d2 for dlambda by workgroups that own rows and pass over the keys, dK and dV
 // by workgroups that own keys and pass over the rows of all heads that share them, and dlambda.  Scores and dA are formed in both of the
 // middle ones, 7 parts of work instead of 5, and nothing is added to memory by more than one workgroup: no atomics, the same bits on every call.
 //
@@ -19,8 +19,9 @@ namespace attention {
 
 constexpr int STEP = KT;        // keys (dQ) or rows (dK, dV) of a tile
 
-// What a row brings beside its query: five planes of B * Hkv * R floats.
-enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, PLANES };
+// Planes of B * Hkv * R floats: what a row brings beside its query, and d2 again, from the probabilities before they are rounded to the operands' type.
+// Rounded ones put an error of their type's last place into every row's d2; dlambda, their sum, was over 1.5 times as far off as one that is rounded once.
+enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, BROUGHT, EXACT2 = BROUGHT, PLANES };
 
 struct BackwardCall {
     Call a;
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(1024) void lambda_kernel(const BackwardCall g)
     __shared__ float part[16];
     const Call &a = g.a;
     const int head = blockIdx.x, hk = head / a.G, which = head % a.G;
-    const float *dots = g.rows + DOT2 * (int64_t)a.B * a.Hkv * a.R;
+    const float *dots = g.rows + EXACT2 * (int64_t)a.B * a.Hkv * a.R;
     int groups = 1;
     while (groups < 16 && groups < a.B) groups *= 2;
     const int threads = 1024 / groups, group = threadIdx.x / threads;
@@ -158,6 +159,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
     const float minus_sum[2] = {plane[MINUS_SUM1 * count], plane[MINUS_SUM2 * count]};
     const float dot[2] = {plane[DOT1 * count], plane[DOT2 * count]}, weight[2] = {1.0f, -plane[LAMBDA * count]};
     const float c = a.scale * LOG2E;
+    float exact = 0.0f;         // this lane's share of sum_j P2 (dA - d2) with the d2 that was brought: the rest of the exact one
 
     Acc<TR> dq[2][D / TR];
 #pragma unroll
@@ -223,6 +225,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
                     float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, minus_sum[m]));
                     if (decltype(limited)::value && !(n < at.limit - key && (FAST || (word >> n & 1)))) p = 0.0f;
                     ds[f] = p * (da[blk][i] - dot[m]);          // the second map's factor -lambda is a row's: it comes at the end
+                    if (m) exact += ds[f];
                 }
             }
             Frag<T> frag[FRAGS<T, TR>];
@@ -245,7 +248,10 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
             key += STEP;
         }
     for (; key < at.end; key += STEP) tile_of(key, [] {});
+    exact = groups_sum<TR>(exact);
     if (!at.there) return;
+    if (lane_group<TR>() == 0) g.rows[EXACT2 * count + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row] = dot[1] + exact;
+    if (!g.dq) return;
     T *out = static_cast<T *>(g.dq) + (((int64_t)at.b * a.Lq + at.query) * a.H + at.head) * 2 * a.d;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -261,7 +267,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     typedef Stage<T, 256, STEP, 1, DV, FAST> StageG;
     __shared__ __attribute__((aligned(16))) T q_tile[BUFFERS][STEP * StageQ::PITCH];
     __shared__ __attribute__((aligned(16))) T g_tile[BUFFERS][STEP * StageG::PITCH];
-    __shared__ __attribute__((aligned(16))) float planes[BUFFERS][PLANES][STEP];
+    __shared__ __attribute__((aligned(16))) float planes[BUFFERS][BROUGHT][STEP];
     const Call &a = g.a;
     const int workgroups = KEYS_WAVES<T, TR, D, DV> == 2 ? gridDim.x : 2 * gridDim.x;       // as if two fit a CU
     const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, workgroups);
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     // a row past the last has a sum of +inf: its probabilities are 0
     const auto load_planes = [&](int row0) {
         const int p = threadIdx.x / STEP, row = row0 + threadIdx.x % STEP;
-        if (p < PLANES) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
+        if (p < BROUGHT) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
     };
     if (begin < a.R) {
         q_stage.load(qs, begin, a.R, in);
@@ -317,7 +323,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const auto store = [&](int to) {
         q_stage.store(q_tile[to]);
         g_stage.store(g_tile[to]);
-        if (threadIdx.x < PLANES * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = plane;
+        if (threadIdx.x < BROUGHT * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = plane;
     };
     if (BUFFERS == 2 && begin < a.R) store(0);
     int at = 0;
@@ -439,7 +445,7 @@ struct Backward {
             hipLaunchKernelGGL((rows_kernel<T>), dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, st, g);
             rc = check_launch("attention::rows_kernel");
         }
-        if (rc == MAM_OK && g.dq && rows > 0) {
+        if (rc == MAM_OK && (g.dq || g.dlam) && rows > 0) {
             const dim3 grid((unsigned)(row_tiles * a.B * a.Hkv));
             if (a.fast) hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, true>), grid, dim3(256), 0, st, g, (int)row_tiles);
             else hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, false>), grid, dim3(256), 0, st, g, (int)row_tiles);

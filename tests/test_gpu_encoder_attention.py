@@ -174,6 +174,19 @@ def test_lam_in_32_bits_beside_16_bit_operands():
     _check(q, k, v, lam.float(), dout)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_lam_does_not_go_through_rounded_probabilities(dtype):
+    # Products of 16-bit operands are exact and sums fp32, so an fp32 dlam is off by what a probability is: its score's sum of 16 products
+    # and the exponential, (16 + 4) 2^-24 of sum |q k| / 4 (at most 12 here) times log2(e) and as much for the sums, below 2^-15; a probability
+    # in bf16 is off by 2^-9.
+    q, k, v, lam, dout = _operands(1, 2, 8, 8, 8, 16, 32, dtype, seed=31)
+    leaf = lam.float().to(DEV).requires_grad_(True)
+    dlam, = torch.autograd.grad(enc.diff_attention(q.to(DEV), k.to(DEV), v.to(DEV), leaf), leaf, dout.to(DEV))
+    p2 = torch.softmax(torch.einsum("bihd,bjhd->bhij", q[..., 1, :].double(), k[..., 1, :].double()) / 4, -1)
+    terms = p2 * torch.einsum("bihc,bjhc->bhij", dout.double(), v.double())
+    ref.assert_within(dlam, -terms.sum((0, 2, 3)), 2.0 ** -15 * terms.abs().sum((0, 2, 3)), "dlam")
+
+
 def test_gradients_agree_with_differences():
     q, k, v, lam, dout = _operands(1, 9, 12, 2, 1, 8, 8, torch.float32, seed=10)
     gpu = [t.to(DEV).requires_grad_(True) for t in (q, k, v, lam)]
