@@ -113,11 +113,9 @@ __device__ __forceinline__ void mma(const Frag<f16> &a, const Frag<f16> &b, Acc<
 template <int TR>
 __device__ __forceinline__ void mma(const Frag<float> &a, const Frag<float> &b, Acc<TR> &c)
 {
+    static_assert(TR == 16, "fp32 tiles are of 16 rows (TILE_ROWS)");
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        if constexpr (TR == 32) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[u], b[u], c, 0, 0, 0);
-        else c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u], b[u], c, 0, 0, 0);
-    }
+    for (int u = 0; u < 4; ++u) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u], b[u], c, 0, 0, 0);
 }
 
 template <int TR>

@@ -19,9 +19,10 @@ namespace attention {
 
 constexpr int STEP = KT;        // keys (dQ) or rows (dK, dV) of a tile
 
-// Planes of B * Hkv * R floats: what a row brings beside its query, and d2 again, from the probabilities before they are rounded to the operands' type.
-// Rounded ones put an error of their type's last place into every row's d2; dlambda, their sum, was over 1.5 times as far off as one that is rounded once.
-enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, BROUGHT, EXACT2 = BROUGHT, PLANES };
+// What a row brings beside its query: five planes of B * Hkv * R floats.  The queries' kernel, which is the last to read d2, puts it back as formed from the
+// probabilities before they are rounded to the operands' type, for dlambda: rounded ones put an error of their type's last place into every row's d2, and
+// their sum was over 1.5 times as far off as one that is rounded once.
+enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, PLANES };
 
 struct BackwardCall {
     Call a;
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(1024) void lambda_kernel(const BackwardCall g)
     __shared__ float part[16];
     const Call &a = g.a;
     const int head = blockIdx.x, hk = head / a.G, which = head % a.G;
-    const float *dots = g.rows + EXACT2 * (int64_t)a.B * a.Hkv * a.R;
+    const float *dots = g.rows + DOT2 * (int64_t)a.B * a.Hkv * a.R;
     int groups = 1;
     while (groups < 16 && groups < a.B) groups *= 2;
     const int threads = 1024 / groups, group = threadIdx.x / threads;
@@ -155,9 +156,9 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
     for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, at.row, at.there, m, q[m]);
     load_rows<T, TR, DV>(gs, at.row, at.there, 0, grad);
     const int64_t count = (int64_t)a.B * a.Hkv * a.R;
-    const float *plane = g.rows + ((int64_t)at.b * a.Hkv + at.hk) * a.R + (at.there ? at.row : 0);
-    const float minus_sum[2] = {plane[MINUS_SUM1 * count], plane[MINUS_SUM2 * count]};
-    const float dot[2] = {plane[DOT1 * count], plane[DOT2 * count]}, weight[2] = {1.0f, -plane[LAMBDA * count]};
+    const float *plane = g.rows + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row;
+    const auto brought = [&](int p) { return at.there ? plane[p * count] : 0.0f; };      // a wave reads the planes of its own rows only
+    const float minus_sum[2] = {brought(MINUS_SUM1), brought(MINUS_SUM2)}, dot[2] = {brought(DOT1), brought(DOT2)}, weight[2] = {1.0f, -brought(LAMBDA)};
     const float c = a.scale * LOG2E;
     float exact = 0.0f;         // this lane's share of sum_j P2 (dA - d2) with the d2 that was brought: the rest of the exact one
 
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
     for (; key < at.end; key += STEP) tile_of(key, [] {});
     exact = groups_sum<TR>(exact);
     if (!at.there) return;
-    if (lane_group<TR>() == 0) g.rows[EXACT2 * count + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row] = dot[1] + exact;
+    if (lane_group<TR>() == 0) g.rows[DOT2 * count + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row] = dot[1] + exact;
     if (!g.dq) return;
     T *out = static_cast<T *>(g.dq) + (((int64_t)at.b * a.Lq + at.query) * a.H + at.head) * 2 * a.d;
 #pragma unroll
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     typedef Stage<T, 256, STEP, 1, DV, FAST> StageG;
     __shared__ __attribute__((aligned(16))) T q_tile[BUFFERS][STEP * StageQ::PITCH];
     __shared__ __attribute__((aligned(16))) T g_tile[BUFFERS][STEP * StageG::PITCH];
-    __shared__ __attribute__((aligned(16))) float planes[BUFFERS][BROUGHT][STEP];
+    __shared__ __attribute__((aligned(16))) float planes[BUFFERS][PLANES][STEP];
     const Call &a = g.a;
     const int workgroups = KEYS_WAVES<T, TR, D, DV> == 2 ? gridDim.x : 2 * gridDim.x;       // as if two fit a CU
     const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, workgroups);
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     // a row past the last has a sum of +inf: its probabilities are 0
     const auto load_planes = [&](int row0) {
         const int p = threadIdx.x / STEP, row = row0 + threadIdx.x % STEP;
-        if (p < BROUGHT) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
+        if (p < PLANES) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
     };
     if (begin < a.R) {
         q_stage.load(qs, begin, a.R, in);
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const auto store = [&](int to) {
         q_stage.store(q_tile[to]);
         g_stage.store(g_tile[to]);
-        if (threadIdx.x < BROUGHT * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = plane;
+        if (threadIdx.x < PLANES * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = plane;
     };
     if (BUFFERS == 2 && begin < a.R) store(0);
     int at = 0;
@@ -445,17 +446,18 @@ struct Backward {
             hipLaunchKernelGGL((rows_kernel<T>), dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, st, g);
             rc = check_launch("attention::rows_kernel");
         }
-        if (rc == MAM_OK && (g.dq || g.dlam) && rows > 0) {
-            const dim3 grid((unsigned)(row_tiles * a.B * a.Hkv));
-            if (a.fast) hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, true>), grid, dim3(256), 0, st, g, (int)row_tiles);
-            else hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, false>), grid, dim3(256), 0, st, g, (int)row_tiles);
-            rc = check_launch("attention::queries_kernel");
-        }
+        // before the queries' kernel, which changes d2
         if (rc == MAM_OK && (g.dk || g.dv) && key_tiles * a.B * a.Hkv > 0) {
             const dim3 grid((unsigned)(key_tiles * a.B * a.Hkv));
             if (a.fast && g.fast) hipLaunchKernelGGL((keys_kernel<T, TR, D, DV, true>), grid, dim3(256), 0, st, g, (int)key_tiles);
             else hipLaunchKernelGGL((keys_kernel<T, TR, D, DV, false>), grid, dim3(256), 0, st, g, (int)key_tiles);
             rc = check_launch("attention::keys_kernel");
+        }
+        if (rc == MAM_OK && (g.dq || g.dlam) && rows > 0) {
+            const dim3 grid((unsigned)(row_tiles * a.B * a.Hkv));
+            if (a.fast) hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, true>), grid, dim3(256), 0, st, g, (int)row_tiles);
+            else hipLaunchKernelGGL((queries_kernel<T, TR, D, DV, false>), grid, dim3(256), 0, st, g, (int)row_tiles);
+            rc = check_launch("attention::queries_kernel");
         }
         if (rc == MAM_OK && g.dlam && a.H > 0) {
             hipLaunchKernelGGL((lambda_kernel<T>), dim3((unsigned)a.H), dim3(1024), 0, st, g);

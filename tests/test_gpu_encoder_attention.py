@@ -1,4 +1,6 @@
 """GPU tests of differential attention and its gradients against the definition in 64 bits."""
+import ctypes
+
 import pytest
 import torch
 
@@ -279,6 +281,26 @@ def test_refusals():
     for call in bad:
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_c_entry_wants_what_the_backward_reads_together():
+    from mamtorch_amd import capi
+    # 600 keys are split over workgroups, 6 are not
+    q, k, v, lam, _ = (t.to(DEV) for t in _operands(1, 2, 600, 1, 1, 8, 16, torch.float32, seed=17))
+    for keys in (600, 6):
+        a = capi.DiffAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), q.stride()[:4], k.stride()[:4], v.stride()[:3],
+                               B=1, Lq=2, Lk=keys, H=1, Hkv=1, D=8, Dv=16, scale=1.0, type=0, lam_type=0)
+        need = capi.lib().mam_diff_attention_workspace(ctypes.byref(a))
+        assert (need > 0) == (keys == 600)
+        ws = torch.empty(max(1, need), dtype=torch.uint8, device=DEV)
+        out, kept, lse = torch.zeros(1, 2, 1, 16, device=DEV), torch.zeros(1, 2, 1, 16, device=DEV), torch.zeros(2, 1, 1, 2, device=DEV)
+        stream = torch.cuda.current_stream().cuda_stream
+        for which in ((kept.data_ptr(), None), (None, lse.data_ptr())):
+            assert capi.lib().mam_diff_attention(ctypes.byref(a), out.data_ptr(), *which, ws.data_ptr(), need, stream) == -1    # invalid argument
+        if need:
+            assert capi.lib().mam_diff_attention(ctypes.byref(a), out.data_ptr(), None, None, None, 0, stream) == -3            # no workspace
+        torch.cuda.synchronize()
+        assert not out.any() and not kept.any() and not lse.any()
 
 
 def test_opcheck():
