@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/mam_hip.h"
+#include "mam_rows.h"
 
 namespace {
 
@@ -65,16 +66,8 @@ Rows rows_of(const Tensor &x, const char *name)
     TORCH_CHECK(x.dim() >= 1, name, " must have at least one dimension");
     const int64_t c = x.size(-1), n = c ? x.numel() / c : 0;
     if (x.is_contiguous() || x.numel() == 0) return {x, n, c, c};
-    const bool unit = c == 1 || x.stride(-1) == 1;
-    int64_t ld = 0, next = 0;      // stride of a row, and what the next outer dimension's must be
-    bool even = unit;
-    for (int64_t i = x.dim() - 2; even && i >= 0; --i) {
-        if (x.size(i) == 1) continue;
-        if (!ld) ld = x.stride(i);
-        else even = x.stride(i) == next;
-        next = x.stride(i) * x.size(i);
-    }
-    if (even && (!ld || ld >= c)) return {x, n, c, ld ? ld : c};
+    const int64_t ld = mam::row_stride(x.sizes().data(), x.strides().data(), x.dim());
+    if (ld >= 0) return {x, n, c, ld};
     return {x.contiguous(), n, c, c};
 }
 
