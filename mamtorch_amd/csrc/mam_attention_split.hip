@@ -258,25 +258,22 @@ __global__ __launch_bounds__(256, D > 64 || (sizeof(T) == 4 && DV > 64) ? 1 : 2)
         }
     }
     __syncthreads();
-    float most[2], total[2];
+    // A range of which a row sees nothing has a sum of 0, and its products do not count whatever the values there hold.  Scores that are all NaN leave
+    // the maximum at -inf too, but not the sum: they go on as NaN.
+    float most[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        most[m] = fmaxf(fmaxf(tops[m][0][lane], tops[m][1][lane]), fmaxf(tops[m][2][lane], tops[m][3][lane]));
-        total[m] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) total[m] += most[m] == -INFINITY ? 0.0f : sums[m][w][lane] * __builtin_amdgcn_exp2f(tops[m][w][lane] - most[m]);
-    }
+    for (int m = 0; m < 2; ++m) most[m] = fmaxf(fmaxf(tops[m][0][lane], tops[m][1][lane]), fmaxf(tops[m][2][lane], tops[m][3][lane]));
     for (int w = 0; w < 4; ++w) {
         if (w == wave) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                const float factor = top[m] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[m] - most[m]);
+                const float factor = __builtin_amdgcn_exp2f(top[m] - most[m]);
 #pragma unroll
                 for (int j = 0; j < E; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float &cell = joined[m][lane][E * (4 * group + i) + j];
-                        const float part = top[m] == -INFINITY ? 0.0f : o[m][j][i] * factor;
+                        const float part = sum[m] == 0.0f ? 0.0f : o[m][j][i] * factor;
                         cell = w ? cell + part : part;
                     }
             }
@@ -292,7 +289,7 @@ __global__ __launch_bounds__(256, D > 64 || (sizeof(T) == 4 && DV > 64) ? 1 : 2)
         m_top[m] = fmaxf(fmaxf(tops[m][0][mine], tops[m][1][mine]), fmaxf(tops[m][2][mine], tops[m][3][mine]));
         m_sum[m] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m_sum[m] += m_top[m] == -INFINITY ? 0.0f : sums[m][w][mine] * __builtin_amdgcn_exp2f(tops[m][w][mine] - m_top[m]);
+        for (int w = 0; w < 4; ++w) m_sum[m] += sums[m][w][mine] == 0.0f ? 0.0f : sums[m][w][mine] * __builtin_amdgcn_exp2f(tops[m][w][mine] - m_top[m]);
     }
     if (splits == 1) {
         const int i = out_row / a.G, h = hk * a.G + out_row - i * a.G;
