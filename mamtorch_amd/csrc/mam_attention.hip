@@ -230,7 +230,8 @@ __global__ __launch_bounds__(256, (WAVES<T, TR, D, DV>)) void tiles_kernel(const
 // 244 us (137 GFLOP, 564 TFLOP/s; matrix cores busy in 27 % of the cycles, vector units in about 36 %).  Deeper pipelines of the scores and queries kept in
 // LDS measured the same or slower (340 to 435 us where the first is 356).
 //
-// A is scaled by g = min(the larger sum, 2^12) so that fp16 holds the probabilities of long rows as normal numbers.
+// Both products are scaled so that fp16 holds the probabilities of long rows as normal numbers: P2 by g2 = min(the larger sum, 2^12), A by
+// g = min(g2, 2^12 / |lambda|), which keeps both of its terms below 2^13 whatever lambda is.
 
 // Both maps' scores of 32 keys.
 template <class T, int TR, int D>
@@ -331,17 +332,18 @@ __global__ __launch_bounds__(256, 2) void twice_kernel(const Call a, const Forwa
             });
         for (; t < tiles; t += TURN) turn(t, [](const T *) {});
     }
-    // base[m]: what the second pass subtracts, so that exp2(score - base) is g P; +inf where a row sees nothing
+    // base[m]: what the second pass subtracts, so that exp2(score - base) is g P1 and g2 P2; +inf where a row sees nothing
     float lse[2], base[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         sum[m] = groups_sum<TR>(sum[m]);
         lse[m] = sum[m] > 0.0f ? top[m] + log2f(sum[m]) : INFINITY;
     }
-    const float g = fminf(fmaxf(fmaxf(sum[0], sum[1]), 1.0f), 4096.0f), back = 1.0f / g, shift = log2f(g);
-#pragma unroll
-    for (int m = 0; m < 2; ++m) base[m] = lse[m] - shift;
     const float lam = lambda_of(a, at.head, static_cast<const T *>(nullptr));
+    const float g2 = fminf(fmaxf(fmaxf(sum[0], sum[1]), 1.0f), 4096.0f), g = fminf(g2, 4096.0f / fmaxf(fabsf(lam), 1.0f));
+    const float back = 1.0f / g, weight = lam * (g / g2);
+    base[0] = lse[0] - log2f(g);
+    base[1] = lse[1] - log2f(g2);
 
     // second pass
     Acc<TR> o[MAPS][DV / TR];
@@ -378,7 +380,7 @@ __global__ __launch_bounds__(256, 2) void twice_kernel(const Call a, const Forwa
             for (int f = 0; f < REGS<TR>; ++f) {
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][f / AR][f % AR], c, -base[0]));
                 const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][f / AR][f % AR], c, -base[1]));
-                p[0][f] = fmaf(-lam, p2, p1);
+                p[0][f] = fmaf(-weight, p2, p1);
                 if (KEEP) p[MAPS - 1][f] = p2;
             }
 #pragma unroll
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void twice_kernel(const Call a, const Forwa
             for (int u = 0; u < 4; ++u) {
                 r[u] = o[0][blk][f + u] * back;
                 if (KEEP) {
-                    o2[u] = o[MAPS - 1][blk][f + u] * back;
+                    o2[u] = o[MAPS - 1][blk][f + u] * (1.0f / g2);
                     o1[u] = fmaf(lam, o2[u], r[u]);
                 }
             }
