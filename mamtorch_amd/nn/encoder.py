@@ -10,7 +10,7 @@ import torch
 from torch import Tensor, nn
 
 from ..kernel import encoder as K
-from .fullyconnected import FullyConnected
+from .fullyconnected import FullyConnected, check_counted
 
 __all__ = ["LayerNorm", "Dropout", "DiffAttention", "DiffAttentionCache", "MAMEncoderLayer"]
 
@@ -36,22 +36,31 @@ class LayerNorm(nn.Module):
 
 class Dropout(nn.Module):
     """Dropout whose mask is formed from (seed, number of the training call) where it is needed.  The number of calls is part of the module's
-    state, so that a training run that is taken up again draws on; modules of one model need seeds of their own."""
+    state, so that a training run that is taken up again draws on; modules of one model need seeds of their own.
 
-    def __init__(self, p: float = 0.5, seed: int = 0):
+    step: one int64 element on the GPU, by which the mask is numbered instead of by calls.  The training loop advances it between steps, after the
+    backward pass; every call of a step draws the same mask, so what is computed again in the backward pass (activation checkpointing) and the replays
+    of a captured step are right.  Numbered by calls, a training call in a backward pass, under capture or in a DataParallel replica is an error: it would
+    draw another mask than the one whose gradient is wanted, or the same one in every step."""
+
+    def __init__(self, p: float = 0.5, seed: int = 0, step: Tensor = None):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError(f"p must be between 0 and 1, got {p}")
-        self.p, self.seed, self.calls = p, seed, 0
+        self.p, self.seed, self.step, self.calls = p, seed, step, 0
 
     def next_offset(self) -> int:
+        """Offset of this training call's mask, to which ``step`` is added where there is one."""
+        if self.step is not None:
+            return 0
+        check_counted(self, "step")
         self.calls += 1
         return self.calls - 1
 
     def forward(self, x: Tensor, residual: Tensor = None) -> Tensor:
         if not self.training or self.p == 0:
             return x if residual is None else residual + x
-        return K.dropout(x, self.p, self.seed, self.next_offset(), residual)
+        return K.dropout(x, self.p, self.seed, self.next_offset(), residual, step=self.step)
 
     def get_extra_state(self):
         return {"calls": self.calls}
@@ -145,20 +154,22 @@ class DiffAttention(nn.Module):
 class MAMEncoderLayer(nn.Module):
     """A pre-norm encoder layer: x + dropout(attention(norm(x))), then the same of the MAM MLP (FullyConnected -> GELU -> FullyConnected).
     The sum between the halves, its dropout and the second norm are one operator.  ViT-B/16: hidden 768, intermediate 3072, 6 heads of two maps.
-    Further keyword arguments go to the ``FullyConnected`` layers."""
+    step: what numbers the masks instead of calls (see ``Dropout``), those of the ``FullyConnected`` layers' weights too.  Further keyword arguments go to
+    the ``FullyConnected`` layers."""
 
     def __init__(self, hidden: int = 768, intermediate: int = 3072, heads: int = 6, kv_heads: int = None, depth: int = 1, causal: bool = False,
-                 p: float = 0.0, seed: int = 0, eps: float = 1e-5, device=None, dtype=None, **fc_kwargs):
+                 p: float = 0.0, seed: int = 0, eps: float = 1e-5, device=None, dtype=None, step: Tensor = None, **fc_kwargs):
         super().__init__()
         kwargs = {"device": device, "dtype": dtype}
+        fc_kwargs.setdefault("wdrop_step", step)
         self.norm1 = LayerNorm(hidden, eps, **kwargs)
         self.attention = DiffAttention(hidden, heads, kv_heads, depth, causal, **kwargs)
-        self.dropout1 = Dropout(p, 2 * seed)
+        self.dropout1 = Dropout(p, 2 * seed, step)
         self.norm2 = LayerNorm(hidden, eps, **kwargs)
         self.intermediate = FullyConnected(hidden, intermediate, **kwargs, **fc_kwargs)
         self.act = nn.GELU()
         self.output = FullyConnected(intermediate, hidden, **kwargs, **fc_kwargs)
-        self.dropout2 = Dropout(p, 2 * seed + 1)
+        self.dropout2 = Dropout(p, 2 * seed + 1, step)
 
     def vcon_step(self) -> None:
         self.intermediate.vcon_step()
@@ -168,5 +179,6 @@ class MAMEncoderLayer(nn.Module):
         a = self.attention(self.norm1(x), lengths, key_mask, cache)
         drop, norm = self.dropout1, self.norm2
         p = drop.p if drop.training else 0.0
-        y, s = K.add_dropout_layer_norm(a, x, norm.weight, norm.bias, p, drop.seed, drop.next_offset() if p else 0, norm.eps)
+        y, s = K.add_dropout_layer_norm(a, x, norm.weight, norm.bias, p, drop.seed, drop.next_offset() if p else 0, norm.eps,
+                                        step=drop.step if p else None)
         return self.dropout2(self.output(self.act(self.intermediate(y))), s)

@@ -15,7 +15,8 @@ counting and repr.  What differs is only how the work reaches the GPU:
     max and 1 if any row picked it as min, both added to ``max_selection_count``);
     ``"hits"`` counts every pick and keeps max and min apart;
   * ``wdrop_seed`` (default None: masks drawn by torch's generator, a byte a weight) takes the weight dropout's masks from
-    a counter-based generator under that seed, a new one each call, which are never stored.
+    a counter-based generator under that seed, a new one each training call, which are never stored; ``wdrop_step`` (one int64
+    element on the GPU) numbers them instead of calls, as ``nn.Dropout``'s ``step`` does.
 """
 import math
 
@@ -27,6 +28,23 @@ from torch.nn import Module, Parameter
 from .. import kernel as K
 
 __all__ = ["FullyConnected"]
+
+
+def check_counted(module: Module, step: str) -> None:
+    """Refuses a mask that a module numbers by its training calls where calls do not number it: a forward that is computed again in a backward pass
+    would draw another mask than the one whose gradient is wanted, the replays of a captured one and DataParallel's replicas the same in every step."""
+    if torch.compiler.is_compiling():
+        return
+    where = None
+    if torch._C._current_graph_task_id() != -1:
+        where = "in a backward pass"
+    elif getattr(module, "_is_replica", False):
+        where = "in a replica"
+    elif torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        where = "under graph capture"
+    if where:
+        raise RuntimeError(f"{type(module).__name__} numbers its masks by training calls, which a forward {where} does not follow; give it "
+                           f"`{step}`, an int64 element on the GPU that the training loop advances between steps")
 
 
 class FullyConnected(Module):
@@ -57,6 +75,7 @@ class FullyConnected(Module):
         dtype=None,
         selection_count_mode: str = "reference",
         wdrop_seed: int = None,
+        wdrop_step: Tensor = None,
     ) -> None:
         factory_kwargs = {"device": device, "dtype": dtype}
         super().__init__()
@@ -71,6 +90,7 @@ class FullyConnected(Module):
         self.vcon_expand = vcon_expand
         self.wdrop_rate = wdrop_rate
         self.wdrop_seed = wdrop_seed
+        self.wdrop_step = wdrop_step
         self.wdrop_calls = 0
         self.drop_rate = drop_rate
         self.compute_exact = compute_exact
@@ -157,7 +177,10 @@ class FullyConnected(Module):
             if not (0 < self.wdrop_rate < 1):
                 raise Exception("wdrop_rate must be between 0 and 1.")
             if self.wdrop_seed is not None:
-                # the mask as a function of seed and call: never stored, formed again for the weight gradient
+                # the mask as a function of seed and call (or step): never stored, formed again for the weight gradient
+                if self.wdrop_step is not None:
+                    return K.encoder.dropout(w, self.wdrop_rate, self.wdrop_seed, scale=1.0, step=self.wdrop_step)
+                check_counted(self, "wdrop_step")
                 self.wdrop_calls += 1
                 return K.encoder.dropout(w, self.wdrop_rate, self.wdrop_seed, self.wdrop_calls - 1, scale=1.0)
             # the reference draws a float mask of the weight's size and multiplies (a second copy of W and
