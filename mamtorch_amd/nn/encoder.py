@@ -36,21 +36,31 @@ class LayerNorm(nn.Module):
 
 class Dropout(nn.Module):
     """Dropout whose mask is formed from (seed, number of the training call) where it is needed.  The number of calls is part of the module's
-    state, so that a training run that is taken up again draws on; modules of one model need seeds of their own.
+    state, so that a training run that is taken up again draws on.
+
+    seed: modules of one model need seeds of their own, or they drop the same elements.  By default each takes one from torch's generator, when it is
+    made (with p = 0, when it is first needed); that one is part of the state too, and a module whose seed was not given takes it up with the state.
 
     step: one int64 element on the GPU, by which the mask is numbered instead of by calls.  The training loop advances it between steps, after the
     backward pass; every call of a step draws the same mask, so what is computed again in the backward pass (activation checkpointing) and the replays
     of a captured step are right.  Numbered by calls, a training call in a backward pass, under capture or in a DataParallel replica is an error: it would
     draw another mask than the one whose gradient is wanted, or the same one in every step."""
 
-    def __init__(self, p: float = 0.5, seed: int = 0, step: Tensor = None):
+    def __init__(self, p: float = 0.5, seed: int = None, step: Tensor = None):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError(f"p must be between 0 and 1, got {p}")
-        self.p, self.seed, self.step, self.calls = p, seed, step, 0
+        self.p, self.seed, self.seed_given, self.step, self.calls = p, seed, seed is not None, step, 0
+        if p > 0:
+            self._need_seed()
+
+    def _need_seed(self) -> None:
+        if self.seed is None:
+            self.seed = int(torch.randint(2 ** 63 - 1, (), device="cpu"))
 
     def next_offset(self) -> int:
-        """Offset of this training call's mask, to which ``step`` is added where there is one."""
+        """Offset of this training call's mask (to which ``step`` is added where there is one), under ``seed``."""
+        self._need_seed()
         if self.step is not None:
             return 0
         check_counted(self, "step")
@@ -60,13 +70,16 @@ class Dropout(nn.Module):
     def forward(self, x: Tensor, residual: Tensor = None) -> Tensor:
         if not self.training or self.p == 0:
             return x if residual is None else residual + x
-        return K.dropout(x, self.p, self.seed, self.next_offset(), residual, step=self.step)
+        offset = self.next_offset()
+        return K.dropout(x, self.p, self.seed, offset, residual, step=self.step)
 
     def get_extra_state(self):
-        return {"calls": self.calls}
+        return {"calls": self.calls, "seed": self.seed}
 
     def set_extra_state(self, state):
         self.calls = int(state["calls"])
+        if not self.seed_given and state.get("seed") is not None:
+            self.seed = int(state["seed"])
 
     def extra_repr(self) -> str:
         return f"p={self.p}, seed={self.seed}"
@@ -154,22 +167,24 @@ class DiffAttention(nn.Module):
 class MAMEncoderLayer(nn.Module):
     """A pre-norm encoder layer: x + dropout(attention(norm(x))), then the same of the MAM MLP (FullyConnected -> GELU -> FullyConnected).
     The sum between the halves, its dropout and the second norm are one operator.  ViT-B/16: hidden 768, intermediate 3072, 6 heads of two maps.
-    step: what numbers the masks instead of calls (see ``Dropout``), those of the ``FullyConnected`` layers' weights too.  Further keyword arguments go to
+    seed: of the two dropouts, each under a key formed from it and from depth; layers of one depth need seeds of their own, by default drawn as ``Dropout``
+    does.  step: what numbers the masks instead of calls (see ``Dropout``), those of the ``FullyConnected`` layers' weights too.  Further keyword arguments go to
     the ``FullyConnected`` layers."""
 
     def __init__(self, hidden: int = 768, intermediate: int = 3072, heads: int = 6, kv_heads: int = None, depth: int = 1, causal: bool = False,
-                 p: float = 0.0, seed: int = 0, eps: float = 1e-5, device=None, dtype=None, step: Tensor = None, **fc_kwargs):
+                 p: float = 0.0, seed: int = None, eps: float = 1e-5, device=None, dtype=None, step: Tensor = None, **fc_kwargs):
         super().__init__()
         kwargs = {"device": device, "dtype": dtype}
         fc_kwargs.setdefault("wdrop_step", step)
+        seeds = (None, None) if seed is None else (2 * seed + (depth - 1 << 32), 2 * seed + 1 + (depth - 1 << 32))
         self.norm1 = LayerNorm(hidden, eps, **kwargs)
         self.attention = DiffAttention(hidden, heads, kv_heads, depth, causal, **kwargs)
-        self.dropout1 = Dropout(p, 2 * seed, step)
+        self.dropout1 = Dropout(p, seeds[0], step)
         self.norm2 = LayerNorm(hidden, eps, **kwargs)
         self.intermediate = FullyConnected(hidden, intermediate, **kwargs, **fc_kwargs)
         self.act = nn.GELU()
         self.output = FullyConnected(intermediate, hidden, **kwargs, **fc_kwargs)
-        self.dropout2 = Dropout(p, 2 * seed + 1, step)
+        self.dropout2 = Dropout(p, seeds[1], step)
 
     def vcon_step(self) -> None:
         self.intermediate.vcon_step()
@@ -179,6 +194,6 @@ class MAMEncoderLayer(nn.Module):
         a = self.attention(self.norm1(x), lengths, key_mask, cache)
         drop, norm = self.dropout1, self.norm2
         p = drop.p if drop.training else 0.0
-        y, s = K.add_dropout_layer_norm(a, x, norm.weight, norm.bias, p, drop.seed, drop.next_offset() if p else 0, norm.eps,
-                                        step=drop.step if p else None)
+        offset = drop.next_offset() if p else 0
+        y, s = K.add_dropout_layer_norm(a, x, norm.weight, norm.bias, p, drop.seed if p else 0, offset, norm.eps, step=drop.step if p else None)
         return self.dropout2(self.output(self.act(self.intermediate(y))), s)

@@ -39,3 +39,55 @@ def test_calls_number_the_masks_where_nothing_else_does():
     assert [module.next_offset() for _ in range(3)] == [0, 1, 2] and module.get_extra_state()["calls"] == 3
     module.step = torch.zeros(1, dtype=torch.int64)
     assert [module.next_offset() for _ in range(3)] == [0, 0, 0] and module.get_extra_state()["calls"] == 3
+
+
+def _keys(layer):
+    return [layer.dropout1.seed, layer.dropout2.seed]
+
+
+def _layer(**kwargs):
+    return mt.nn.MAMEncoderLayer(hidden=24, intermediate=40, heads=2, **kwargs)
+
+
+def test_modules_without_a_seed_take_one_of_their_own():
+    torch.manual_seed(0)
+    layers = [_layer(p=0.1) for _ in range(3)]
+    drops = [mt.nn.Dropout(), mt.nn.Dropout()]
+    keys = [k for layer in layers for k in _keys(layer)] + [d.seed for d in drops]
+    assert len(set(keys)) == 8
+    torch.manual_seed(0)
+    assert _keys(_layer(p=0.1)) == keys[:2]
+
+
+def test_a_module_that_drops_nothing_draws_nothing():
+    torch.manual_seed(0)
+    before = torch.random.get_rng_state()
+    module = mt.nn.Dropout(0.0)
+    assert torch.equal(torch.random.get_rng_state(), before) and module.seed is None
+    module.p = 0.5
+    module.next_offset()
+    other = mt.nn.Dropout(0.0)
+    other.next_offset()
+    assert module.seed is not None and module.seed != other.seed
+
+
+def test_layers_of_one_seed_differ_by_depth():
+    keys = [k for depth in range(1, 13) for k in _keys(_layer(p=0.1, seed=7, depth=depth))]
+    assert len(set(keys)) == 24 and keys[:2] == [14, 15]
+
+
+def test_a_drawn_seed_is_taken_up_with_the_state_and_a_given_one_kept():
+    layer = _layer(p=0.1)
+    layer.dropout1.next_offset()
+    other, given = _layer(p=0.1), _layer(p=0.1, seed=7)
+    for to in (other, given):
+        to.load_state_dict(layer.state_dict())
+        assert to.dropout1.calls == 1 and to.dropout2.calls == 0
+    assert _keys(other) == _keys(layer) and _keys(given) == [14, 15]
+    other.load_state_dict(given.state_dict())
+    assert _keys(other) == [14, 15]
+    state = layer.state_dict()
+    state["dropout1._extra_state"] = {"calls": 4}           # as it was before seeds were part of it
+    keys = _keys(other)
+    other.load_state_dict(state)
+    assert other.dropout1.calls == 4 and other.dropout1.seed == keys[0]
