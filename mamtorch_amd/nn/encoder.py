@@ -168,7 +168,7 @@ class MAMEncoderLayer(nn.Module):
     """A pre-norm encoder layer: x + dropout(attention(norm(x))), then the same of the MAM MLP (FullyConnected -> GELU -> FullyConnected).
     The sum between the halves, its dropout and the second norm are one operator.  ViT-B/16: hidden 768, intermediate 3072, 6 heads of two maps.
     seed: of the two dropouts, each under a key formed from it and from depth; layers of one depth need seeds of their own, by default drawn as ``Dropout``
-    does.  step: what numbers the masks instead of calls (see ``Dropout``), those of the ``FullyConnected`` layers' weights too.  Further keyword arguments go to
+    does.  ``wdrop_seed`` is likewise the two weights'.  step: what numbers the masks instead of calls (see ``Dropout``), those of the ``FullyConnected`` layers' weights too.  Further keyword arguments go to
     the ``FullyConnected`` layers."""
 
     def __init__(self, hidden: int = 768, intermediate: int = 3072, heads: int = 6, kv_heads: int = None, depth: int = 1, causal: bool = False,
@@ -177,13 +177,15 @@ class MAMEncoderLayer(nn.Module):
         kwargs = {"device": device, "dtype": dtype}
         fc_kwargs.setdefault("wdrop_step", step)
         seeds = (None, None) if seed is None else (2 * seed + (depth - 1 << 32), 2 * seed + 1 + (depth - 1 << 32))
+        wdrop_seed = fc_kwargs.pop("wdrop_seed", None)      # high bits: no key of a weight is a dropout's or the other weight's
+        wdrop_seeds = (None, None) if wdrop_seed is None else tuple(wdrop_seed + (depth - 1 << 32) + (n << 61) for n in (1, 2))
         self.norm1 = LayerNorm(hidden, eps, **kwargs)
         self.attention = DiffAttention(hidden, heads, kv_heads, depth, causal, **kwargs)
         self.dropout1 = Dropout(p, seeds[0], step)
         self.norm2 = LayerNorm(hidden, eps, **kwargs)
-        self.intermediate = FullyConnected(hidden, intermediate, **kwargs, **fc_kwargs)
+        self.intermediate = FullyConnected(hidden, intermediate, wdrop_seed=wdrop_seeds[0], **kwargs, **fc_kwargs)
         self.act = nn.GELU()
-        self.output = FullyConnected(intermediate, hidden, **kwargs, **fc_kwargs)
+        self.output = FullyConnected(intermediate, hidden, wdrop_seed=wdrop_seeds[1], **kwargs, **fc_kwargs)
         self.dropout2 = Dropout(p, seeds[1], step)
 
     def vcon_step(self) -> None:

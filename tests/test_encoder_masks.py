@@ -91,3 +91,10 @@ def test_a_drawn_seed_is_taken_up_with_the_state_and_a_given_one_kept():
     keys = _keys(other)
     other.load_state_dict(state)
     assert other.dropout1.calls == 4 and other.dropout1.seed == keys[0]
+
+
+def test_weights_of_a_layer_have_masks_of_their_own():
+    layers = [_layer(p=0.1, seed=7, depth=depth, wdrop_rate=0.5, wdrop_seed=14) for depth in (1, 2)]
+    keys = [k & 2 ** 64 - 1 for layer in layers for k in (*_keys(layer), layer.intermediate.wdrop_seed, layer.output.wdrop_seed)]
+    assert len(set(keys)) == 8
+    assert _layer(wdrop_rate=0.5).output.wdrop_seed is None
