@@ -53,6 +53,10 @@ class FullyConnected(Module):
     __constants__ = ["in_features", "out_features"]
     in_features: int
     out_features: int
+    # for modules that were saved whole before they had these
+    wdrop_seed = None
+    wdrop_step = None
+    wdrop_calls = 0
     weight: Tensor
 
     def __init__(

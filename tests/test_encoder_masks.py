@@ -1,4 +1,6 @@
 """CPU tests of what numbers the masks of the modules that form them from counters."""
+import io
+
 import pytest
 import torch
 
@@ -98,3 +100,15 @@ def test_weights_of_a_layer_have_masks_of_their_own():
     keys = [k & 2 ** 64 - 1 for layer in layers for k in (*_keys(layer), layer.intermediate.wdrop_seed, layer.output.wdrop_seed)]
     assert len(set(keys)) == 8
     assert _layer(wdrop_rate=0.5).output.wdrop_seed is None
+
+
+def test_a_module_that_was_saved_whole_before_it_had_a_seed_still_trains(monkeypatch):
+    module = mt.nn.FullyConnected(6, 4, wdrop_rate=0.5)
+    for name in ("wdrop_seed", "wdrop_step", "wdrop_calls"):
+        del module.__dict__[name]
+    file = io.BytesIO()
+    torch.save(module, file)
+    file.seek(0)
+    module = torch.load(file, weights_only=False).train()
+    monkeypatch.setattr(mt.kernel.v4, "apply_keep", lambda w, keep: w * keep)
+    assert module._dropped_weight().shape == (4, 6) and sorted(module.state_dict()) == ["bias", "weight"]
