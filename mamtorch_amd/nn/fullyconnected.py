@@ -174,6 +174,19 @@ class FullyConnected(Module):
         K.v4.selection_count(self.argmax, self.argmin, self.max_selection_count,
                              self.min_selection_count, mode)
 
+    # The number of calls that the weight's masks have been drawn for is part of the state where they are numbered by it, so that a training run that
+    # is taken up again draws on; a state without it leaves it as it is.
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self.wdrop_seed is not None:
+            destination[prefix + "wdrop_calls"] = torch.tensor(self.wdrop_calls)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        calls = state_dict.pop(prefix + "wdrop_calls", None)
+        if calls is not None:
+            self.wdrop_calls = int(calls)
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
     def _dropped_weight(self) -> Tensor:
         """Weight with the training-time weight dropout applied, still (out, in)."""
         w = self.weight

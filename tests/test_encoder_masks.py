@@ -112,3 +112,19 @@ def test_a_module_that_was_saved_whole_before_it_had_a_seed_still_trains(monkeyp
     module = torch.load(file, weights_only=False).train()
     monkeypatch.setattr(mt.kernel.v4, "apply_keep", lambda w, keep: w * keep)
     assert module._dropped_weight().shape == (4, 6) and sorted(module.state_dict()) == ["bias", "weight"]
+
+
+def test_calls_of_a_weights_dropout_are_part_of_the_state():
+    make = lambda **kwargs: torch.nn.Sequential(mt.nn.FullyConnected(6, 4, **kwargs), torch.nn.ReLU())      # noqa: E731
+    counted, other, plain = make(wdrop_rate=0.5, wdrop_seed=3), make(wdrop_rate=0.5, wdrop_seed=3), make()
+    counted[0].wdrop_calls = 5
+    state = counted.state_dict()
+    assert sorted(state) == ["0.bias", "0.wdrop_calls", "0.weight"] and sorted(plain.state_dict()) == ["0.bias", "0.weight"]
+    other.load_state_dict(state)
+    assert other[0].wdrop_calls == 5 and torch.equal(other[0].weight, counted[0].weight)
+    other.load_state_dict(plain.state_dict())               # a state without it
+    assert other[0].wdrop_calls == 5 and torch.equal(other[0].weight, plain[0].weight)
+    plain.load_state_dict(state)                            # a layer without a seed
+    assert "0.wdrop_calls" in state
+    with pytest.raises(RuntimeError, match="Unexpected"):
+        other.load_state_dict({**state, "0.wdrop_call": torch.tensor(1)})
