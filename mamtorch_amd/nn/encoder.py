@@ -46,6 +46,9 @@ class Dropout(nn.Module):
     of a captured step are right.  Numbered by calls, a training call in a backward pass, under capture or in a DataParallel replica is an error: it would
     draw another mask than the one whose gradient is wanted, or the same one in every step."""
 
+    # for modules that were saved whole before they had these
+    step, seed_given = None, True
+
     def __init__(self, p: float = 0.5, seed: int = None, step: Tensor = None):
         super().__init__()
         if not 0 <= p <= 1:

@@ -128,3 +128,16 @@ def test_calls_of_a_weights_dropout_are_part_of_the_state():
     assert "0.wdrop_calls" in state
     with pytest.raises(RuntimeError, match="Unexpected"):
         other.load_state_dict({**state, "0.wdrop_call": torch.tensor(1)})
+
+
+def test_a_dropout_that_was_saved_whole_before_it_had_a_step_still_draws():
+    module = mt.nn.Dropout(0.5, 3)
+    for name in ("step", "seed_given"):
+        del module.__dict__[name]
+    file = io.BytesIO()
+    torch.save(module, file)
+    file.seek(0)
+    module = torch.load(file, weights_only=False).train()
+    assert module.next_offset() == 0 and module.step is None
+    module.load_state_dict(mt.nn.Dropout(0.5, 8).state_dict())
+    assert module.seed == 3 and module.calls == 0
