@@ -19,10 +19,22 @@ namespace attention {
 
 constexpr int STEP = KT;        // keys (dQ) or rows (dK, dV) of a tile
 
-// What a row brings beside its query: five planes of B * Hkv * R floats.  The queries' kernel, which is the last to read d2, puts it back as formed from the
+// What a row brings beside its query: five planes of B * Hkv * R floats, in fp16 a sixth, its gradient's size (below).  The queries' kernel, which is the last to read d2, puts it back as formed from the
 // probabilities before they are rounded to the operands' type, for dlambda: rounded ones put an error of their type's last place into every row's d2, and
 // their sum was over 1.5 times as far off as one that is rounded once.
-enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, PLANES };
+enum { MINUS_SUM1, MINUS_SUM2, DOT1, DOT2, LAMBDA, PLANES, SIZE = PLANES };
+
+// fp16 holds gradients of scores, dSm, as normal numbers from 2^-14 to 2^16 only: those of 4096 keys and a dO of 1e-4 are 2e-7, those of a dO behind a loss
+// scaler can leave it at the top where dQ and dK do not.  So they are formed times 2^shift, a row's own for dQ and the workgroup's for dK, from the size of dO:
+// its rows' sums of absolute values.  Ordinary gradients, of 2^3 to 2^9, are left as they are; smaller ones are brought up to 2^3, larger ones down to 2^9.
+// P (dA - d) is at most a quarter of dA's range, half of size max |V|: it stays below 2^16 while values are below 2^13 (2^8 from 2^8 on).
+template <class T>
+constexpr bool SHIFTED = std::is_same<T, f16>::value;
+__device__ __forceinline__ int shift_of(float size)
+{
+    const int e = __builtin_amdgcn_frexp_expf(size);        // size = m 2^e, m from 1/2 to 1
+    return size > 0.0f ? (e < 4 ? 4 - e : e > 9 ? 9 - e : 0) : 0;
+}
 
 struct BackwardCall {
     Call a;
@@ -31,7 +43,7 @@ struct BackwardCall {
     const float *kept, *lse;            // KEPT<T> planes like out
     bool fast;                          // dout may be read by Stage<..., FAST> like the operands
     void *dq, *dk, *dv, *dlam;
-    float *rows;                        // PLANES planes
+    float *rows;                        // PLANES planes, one more in fp16
 };
 
 // A row's planes: 16 lanes a row.  Bound by memory: 116 MB (fp32, 64 x 197 tokens of 6 x 128) in 21 us, 5.5 TB/s.
@@ -46,7 +58,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     const T *grad = static_cast<const T *>(g.dout) + b * g.gb + query * g.gl + head * g.gh;
     const int64_t at = (((int64_t)b * a.Lq + query) * a.H + head) * a.dv;
     const int64_t plane = (int64_t)a.B * a.Lq * a.H * a.dv;
-    float dot = 0.0f, dot2 = 0.0f;
+    float dot = 0.0f, dot2 = 0.0f, size = 0.0f;
     for (int c = lane * kPack<T>; c < a.dv; c += 16 * kPack<T>) {
         float v[kPack<T>], o[kPack<T>], o2[kPack<T>];
         load_pack<T>(grad + c, a.dv - c, v);
@@ -57,12 +69,14 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
         for (int u = 0; u < kPack<T>; ++u) {
             dot = fmaf(v[u], o[u], dot);
             dot2 = fmaf(v[u], o2[u], dot2);
+            size += fabsf(v[u]);
         }
     }
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {
         dot += __shfl_xor(dot, m);
         dot2 += __shfl_xor(dot2, m);
+        if (SHIFTED<T>) size += __shfl_xor(size, m);
     }
     if (lane) return;
     const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
@@ -72,6 +86,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     g.rows[DOT1 * count + id] = KEPT<T> == 2 ? dot : fmaf(lam, dot2, dot);      // O1 = out + lambda O2
     g.rows[DOT2 * count + id] = dot2;
     g.rows[LAMBDA * count + id] = lam;
+    if (SHIFTED<T>) g.rows[SIZE * count + id] = size;
 }
 
 // dlambda of a head, a workgroup each: its waves share the requests, or some waves a request where there are fewer.  Five loads after each other and
@@ -158,7 +173,8 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
     const int64_t count = (int64_t)a.B * a.Hkv * a.R;
     const float *plane = g.rows + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row;
     const auto brought = [&](int p) { return at.there ? plane[p * count] : 0.0f; };      // a wave reads the planes of its own rows only
-    const float minus_sum[2] = {brought(MINUS_SUM1), brought(MINUS_SUM2)}, dot[2] = {brought(DOT1), brought(DOT2)}, weight[2] = {1.0f, -brought(LAMBDA)};
+    const float shift = SHIFTED<T> ? (float)shift_of(brought(SIZE)) : 0.0f, back = SHIFTED<T> ? __builtin_amdgcn_exp2f(-shift) : 1.0f;
+    const float minus_sum[2] = {brought(MINUS_SUM1) + shift, brought(MINUS_SUM2) + shift}, dot[2] = {brought(DOT1), brought(DOT2)}, weight[2] = {1.0f, -brought(LAMBDA)};
     const float c = a.scale * LOG2E;
     float exact = 0.0f;         // this lane's share of sum_j P2 (dA - d2) with the d2 that was brought: the rest of the exact one
 
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
             key += STEP;
         }
     for (; key < at.end; key += STEP) tile_of(key, [] {});
-    exact = groups_sum<TR>(exact);
+    exact = groups_sum<TR>(exact) * back;
     if (!at.there) return;
     if (lane_group<TR>() == 0) g.rows[DOT2 * count + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row] = dot[1] + exact;
     if (!g.dq) return;
@@ -257,7 +273,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dq[m][blk], a.scale * weight[m]);
+        for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dq[m][blk], a.scale * weight[m] * back);
 }
 
 template <class T, int TR, int D, int DV, bool FAST>
@@ -269,6 +285,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     __shared__ __attribute__((aligned(16))) T q_tile[BUFFERS][STEP * StageQ::PITCH];
     __shared__ __attribute__((aligned(16))) T g_tile[BUFFERS][STEP * StageG::PITCH];
     __shared__ __attribute__((aligned(16))) float planes[BUFFERS][PLANES][STEP];
+    __shared__ float sizes[4];
     const Call &a = g.a;
     const int workgroups = KEYS_WAVES<T, TR, D, DV> == 2 ? gridDim.x : 2 * gridDim.x;       // as if two fit a CU
     const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, tile = tile_of_turn(blockIdx.x / heads, key_tiles, false, workgroups);
@@ -299,6 +316,17 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const int64_t count = (int64_t)a.B * a.Hkv * a.R;
     const float *rows = g.rows + (int64_t)bh * a.R;
     const float c = a.scale * LOG2E;
+    float up = 1.0f;            // 2^shift of the largest row that the workgroup's keys are seen by, the second map's lambda counted
+    if (SHIFTED<T>) {
+        float size = 0.0f;
+        for (int r = begin + threadIdx.x; r < a.R; r += 256) size = fmaxf(size, rows[SIZE * count + r] * fmaxf(fabsf(rows[LAMBDA * count + r]), 1.0f));
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) size = fmaxf(size, __shfl_xor(size, m));
+        if ((threadIdx.x & 63) == 0) sizes[wave] = size;
+        __syncthreads();
+        size = fmaxf(fmaxf(sizes[0], sizes[1]), fmaxf(sizes[2], sizes[3]));
+        up = __builtin_amdgcn_exp2f((float)__builtin_amdgcn_readfirstlane(shift_of(size)));
+    }
 
     Acc<TR> dk[2][D / TR], dv[DV / TR];
 #pragma unroll
@@ -315,6 +343,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const auto load_planes = [&](int row0) {
         const int p = threadIdx.x / STEP, row = row0 + threadIdx.x % STEP;
         if (p < PLANES) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
+        if (SHIFTED<T> && (p == DOT1 || p == DOT2)) plane *= up;
     };
     if (begin < a.R) {
         q_stage.load(qs, begin, a.R, in);
@@ -377,7 +406,8 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
             Frag<T> frag[FRAGS<T, TR>];
 #pragma unroll
             for (int f = 0; f < REGS<TR> / PART; ++f) {
-                const float d = da[f / (TR * TR / 64)][f % (TR * TR / 64)] - planes[at][m ? DOT2 : DOT1][index_of<TR>(f)];
+                const float all = da[f / (TR * TR / 64)][f % (TR * TR / 64)], own = planes[at][m ? DOT2 : DOT1][index_of<TR>(f)];
+                const float d = SHIFTED<T> ? fmaf(all, up, -own) : all - own;
                 p[m][f] = (m ? -p[m][f] : p[m][f]) * d;
             }
             to_frags<T, TR>(p[m], frag, FRAGS<T, TR> / PART);
@@ -421,7 +451,7 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dk[m][blk], a.scale);
+            for (int blk = 0; blk < D / TR; ++blk) store_columns<T, TR>(out + m * a.d + blk * TR, a.d - blk * TR, dk[m][blk], a.scale * (1.0f / up));
     }
     if (g.dv) {
         T *out = static_cast<T *>(g.dv) + place * a.dv;
@@ -473,7 +503,7 @@ struct Backward {
 extern "C" size_t mam_diff_attention_backward_workspace(const mam_diff_attention_t *args)
 {
     if (!args || args->B <= 0 || args->Lq <= 0 || args->H <= 0) return 0;
-    return (size_t)mam::attention::PLANES * (size_t)args->B * (size_t)args->Lq * (size_t)args->H * sizeof(float);
+    return (size_t)(mam::attention::PLANES + (args->type == MAM_F16 ? 1 : 0)) * (size_t)args->B * (size_t)args->Lq * (size_t)args->H * sizeof(float);
 }
 
 extern "C" int mam_diff_attention_backward(const mam_diff_attention_t *args, const void *dout, const int64_t *dout_stride, const void *out,
