@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const BackwardCall g)
     g.rows[DOT1 * count + id] = KEPT<T> == 2 ? dot : fmaf(lam, dot2, dot);      // O1 = out + lambda O2
     g.rows[DOT2 * count + id] = dot2;
     g.rows[LAMBDA * count + id] = lam;
-    if (SHIFTED<T>) g.rows[SIZE * count + id] = size;
+    if (SHIFTED<T>) g.rows[SIZE * count + id] = size * fmaxf(fabsf(lam), 1.0f);       // the second map's gradients come with lambda
 }
 
 // dlambda of a head, a workgroup each: its waves share the requests, or some waves a request where there are fewer.  Five loads after each other and
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256, (QUERIES_WAVES<T, TR, D, DV>)) void queries_ke
     const int64_t count = (int64_t)a.B * a.Hkv * a.R;
     const float *plane = g.rows + ((int64_t)at.b * a.Hkv + at.hk) * a.R + at.row;
     const auto brought = [&](int p) { return at.there ? plane[p * count] : 0.0f; };      // a wave reads the planes of its own rows only
-    const float shift = SHIFTED<T> ? (float)shift_of(brought(SIZE)) : 0.0f, back = SHIFTED<T> ? __builtin_amdgcn_exp2f(-shift) : 1.0f;
+    const float shift = SHIFTED<T> ? (float)shift_of(brought(SIZE) / fmaxf(fabsf(brought(LAMBDA)), 1.0f)) : 0.0f, back = SHIFTED<T> ? __builtin_amdgcn_exp2f(-shift) : 1.0f;
     const float minus_sum[2] = {brought(MINUS_SUM1) + shift, brought(MINUS_SUM2) + shift}, dot[2] = {brought(DOT1), brought(DOT2)}, weight[2] = {1.0f, -brought(LAMBDA)};
     const float c = a.scale * LOG2E;
     float exact = 0.0f;         // this lane's share of sum_j P2 (dA - d2) with the d2 that was brought: the rest of the exact one
@@ -316,17 +316,6 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const int64_t count = (int64_t)a.B * a.Hkv * a.R;
     const float *rows = g.rows + (int64_t)bh * a.R;
     const float c = a.scale * LOG2E;
-    float up = 1.0f;            // 2^shift of the largest row that the workgroup's keys are seen by, the second map's lambda counted
-    if (SHIFTED<T>) {
-        float size = 0.0f;
-        for (int r = begin + threadIdx.x; r < a.R; r += 256) size = fmaxf(size, rows[SIZE * count + r] * fmaxf(fabsf(rows[LAMBDA * count + r]), 1.0f));
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) size = fmaxf(size, __shfl_xor(size, m));
-        if ((threadIdx.x & 63) == 0) sizes[wave] = size;
-        __syncthreads();
-        size = fmaxf(fmaxf(sizes[0], sizes[1]), fmaxf(sizes[2], sizes[3]));
-        up = __builtin_amdgcn_exp2f((float)__builtin_amdgcn_readfirstlane(shift_of(size)));
-    }
 
     Acc<TR> dk[2][D / TR], dv[DV / TR];
 #pragma unroll
@@ -343,17 +332,35 @@ __global__ __launch_bounds__(256, (KEYS_WAVES<T, TR, D, DV>)) void keys_kernel(c
     const auto load_planes = [&](int row0) {
         const int p = threadIdx.x / STEP, row = row0 + threadIdx.x % STEP;
         if (p < PLANES) plane = row < a.R ? rows[p * count + row] : p <= MINUS_SUM2 ? -INFINITY : 0.0f;
-        if (SHIFTED<T> && (p == DOT1 || p == DOT2)) plane *= up;
     };
     if (begin < a.R) {
         q_stage.load(qs, begin, a.R, in);
         g_stage.load(gs, begin, a.R, in);
         load_planes(begin);
     }
+    float up = 1.0f;            // 2^shift of the largest row that the workgroup's keys are seen by
+    if (SHIFTED<T>) {           // behind the first tile's loads
+        float size = 0.0f;
+        for (int r = begin + threadIdx.x; r < a.R; r += 8 * 256) {       // eight loads on their way; past the end the last row again
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = rows[SIZE * count + (r + 256 * u < a.R ? r + 256 * u : a.R - 1)];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) size = fmaxf(size, v[u]);
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) size = fmaxf(size, __shfl_xor(size, m));
+        if ((threadIdx.x & 63) == 0) sizes[wave] = size;
+        __syncthreads();
+        size = fmaxf(fmaxf(sizes[0], sizes[1]), fmaxf(sizes[2], sizes[3]));
+        up = __builtin_amdgcn_exp2f((float)__builtin_amdgcn_readfirstlane(shift_of(size)));
+    }
+    const float plane_up = threadIdx.x / STEP == DOT1 || threadIdx.x / STEP == DOT2 ? up : 1.0f;
     const auto store = [&](int to) {
         q_stage.store(q_tile[to]);
         g_stage.store(g_tile[to]);
-        if (threadIdx.x < PLANES * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = plane;
+        // scaled here and not where it is asked for, which would wait for it
+        if (threadIdx.x < PLANES * STEP) planes[to][threadIdx.x / STEP][threadIdx.x % STEP] = SHIFTED<T> ? plane * plane_up : plane;
     };
     if (BUFFERS == 2 && begin < a.R) store(0);
     int at = 0;
