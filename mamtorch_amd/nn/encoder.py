@@ -144,8 +144,10 @@ class DiffAttention(nn.Module):
         return torch.exp((q1 * k1).sum(-1)) - torch.exp((q2 * k2).sum(-1)) + self.lambda_init
 
     def cache(self, batch: int, most: int) -> DiffAttentionCache:
+        """A cache for this module's keys and values, in the type that they have where it is made (under autocast, autocast's)."""
         weight = self.key.weight
-        return DiffAttentionCache(batch, most, self.kv_heads, self.head_size, self.value_size, weight.device, weight.dtype)
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else weight.dtype
+        return DiffAttentionCache(batch, most, self.kv_heads, self.head_size, self.value_size, weight.device, dtype)
 
     def forward(self, x: Tensor, lengths: Tensor = None, key_mask: Tensor = None, cache: DiffAttentionCache = None) -> Tensor:
         """x (batch, tokens, hidden).  With a cache, x's tokens are put behind it and see what is there (up to themselves where the module is
@@ -170,6 +172,8 @@ class DiffAttention(nn.Module):
 class MAMEncoderLayer(nn.Module):
     """A pre-norm encoder layer: x + dropout(attention(norm(x))), then the same of the MAM MLP (FullyConnected -> GELU -> FullyConnected).
     The sum between the halves, its dropout and the second norm are one operator.  ViT-B/16: hidden 768, intermediate 3072, 6 heads of two maps.
+    Parameters and x are float32, as the MAM layers are; under autocast the attention runs in 16 bits between them.
+
     seed: of the two dropouts, each under a key formed from it and from depth; layers of one depth need seeds of their own, by default drawn as ``Dropout``
     does.  ``wdrop_seed`` is likewise the two weights'.  step: what numbers the masks instead of calls (see ``Dropout``), those of the ``FullyConnected`` layers' weights too.  Further keyword arguments go to
     the ``FullyConnected`` layers."""
@@ -196,7 +200,7 @@ class MAMEncoderLayer(nn.Module):
         self.output.vcon_step()
 
     def forward(self, x: Tensor, lengths: Tensor = None, key_mask: Tensor = None, cache: DiffAttentionCache = None) -> Tensor:
-        a = self.attention(self.norm1(x), lengths, key_mask, cache)
+        a = self.attention(self.norm1(x), lengths, key_mask, cache).to(x.dtype)      # 16 bits under autocast
         drop, norm = self.dropout1, self.norm2
         p = drop.p if drop.training else 0.0
         offset = drop.next_offset() if p else 0
