@@ -474,7 +474,7 @@ int fill_call(const mam_diff_attention_t *a, Call &c)
     if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 0 || a->Hkv < 0) return fail(MAM_ERR_INVALID_ARGUMENT, "negative size");
     if (a->H > 0 && (a->Hkv < 1 || a->H % a->Hkv)) return fail(MAM_ERR_INVALID_ARGUMENT, "the key heads must divide the query heads");
     if (!head_sizes_fit(a->D, a->Dv)) return fail(MAM_ERR_UNSUPPORTED, "head sizes are 1 to 128 (queries, keys) and 1 to 256 (values)");
-    if (!(a->scale > 0.0) || !(a->scale <= 1e30)) return fail(MAM_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+    if (!((float)a->scale > 0.0f) || !(a->scale <= 1e30)) return fail(MAM_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
     const int64_t most = INT32_MAX / 4;
     if (a->B > most || a->Lq > most || a->Lk > most || a->H > most || a->Lq * (a->H > 0 ? a->H : 1) > most)
         return fail(MAM_ERR_UNSUPPORTED, "a dimension exceeds 2^29");

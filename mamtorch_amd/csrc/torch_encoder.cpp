@@ -258,7 +258,7 @@ AttentionCall attention_call(const Tensor &q, const Tensor &k, const Tensor &v, 
     a.lam_type = type_of(lam, "lam");
     TORCH_CHECK(a.lam_type == a.type || a.lam_type == MAM_F32, "lam must be float32 or of q's type");
     TORCH_CHECK(lam.dim() == 1 && lam.size(0) == a.H && lam.is_contiguous(), "lam must be a contiguous vector of ", a.H, " heads");
-    TORCH_CHECK(scale > 0 && scale <= 1e30, "scale must be positive and finite, got ", scale);
+    TORCH_CHECK(static_cast<float>(scale) > 0 && scale <= 1e30, "scale must be positive and finite in float32, got ", scale);
     for (const MaybeTensor *t : {&lengths, &starts}) {
         const char *name = t == &lengths ? "lengths" : "starts";
         if (!has(*t)) continue;
