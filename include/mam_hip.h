@@ -540,7 +540,7 @@ typedef struct mam_diff_attention_t {
 } mam_diff_attention_t;
 
 /* out (B, Lq, H, Dv) contiguous; for the backward, or NULL: kept, fp32 planes of out's shape (one for fp32 operands, P2 V; two for 16-bit
- * operands, P2 V and P1 V), and lse (2, B, H, Lq) fp32, log2 of each row's sum of exponentials, +inf where it sees no key.  The workspace (of the
+ * operands, P2 V and P1 V), and lse (2, B, H, Lq) fp32, log2 of each row's sum of exponentials, +inf where it sees no key.  A query that holds NaN gives NaN.  The workspace (of the
  * sizes and type; 0 for most calls, not used where kept is given) holds partial results where the keys of a call with few tiles of rows are
  * split over workgroups. */
 size_t mam_diff_attention_workspace(const mam_diff_attention_t *args);

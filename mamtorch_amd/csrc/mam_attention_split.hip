@@ -217,7 +217,9 @@ __global__ __launch_bounds__(256, D > 64 || (sizeof(T) == 4 && DV > 64) ? 1 : 2)
                 sum[m] += p[f];
             }
             to_frags<T, TR>(p, frag[m]);
-            if (PARTS == 2 && m == 0) {         // what 16 bits leave of the first map's probabilities, as a product of its own
+            // What 16 bits leave of the first map's probabilities, as a product of its own.  The second map, which lambda weighs down, goes without: 0.0019 against
+            // 64 bits in bf16 where fp32 probabilities give 0.0017.
+            if (PARTS == 2 && m == 0) {
 #pragma unroll
                 for (int f = 0; f < REGS<TR>; ++f) p[f] -= element(frag[0][f / FE<T>], f % FE<T>);
                 to_frags<T, TR>(p, rest);

@@ -21,7 +21,9 @@ def diff_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, scale: float = 
     causal: query i sees keys j <= i + starts[batch]; starts: int32 (batch), the place of the first query among the keys, by default
     keys - queries.
     A query that sees no key gives zeros.  Where a causal call's keys or values hold NaN or infinities, the queries before them may be reached
-    too.  Softmaxes and sums are float32; probabilities enter the product with v in its type."""
+    too.  Softmaxes and sums are float32.  In 16-bit types what enters a second product is rounded to the type: the
+    probabilities beside v and, in the backward pass, beside the incoming gradient, and the gradients of the scores.  Training keeps two float32
+    tensors of the result's shape (float32 operands: one) until the backward pass."""
     return K.diff_attention.default(q, k, v, lam, float(q.shape[-1] ** -0.5 if scale is None else scale), bool(causal), lengths, starts,
                                     key_mask, False)[0]
 

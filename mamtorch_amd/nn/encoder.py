@@ -89,7 +89,8 @@ class Dropout(nn.Module):
 
 
 class DiffAttentionCache:
-    """Keys and values of up to ``most`` tokens for each request, and how many each has."""
+    """Keys and values of up to ``most`` tokens for each request, and how many each has: as many for every request, since an append puts the same number
+    behind each."""
 
     def __init__(self, batch: int, most: int, kv_heads: int, head_size: int, value_size: int, device=None, dtype=None):
         self.most = most
@@ -116,9 +117,12 @@ class DiffAttentionCache:
 
 
 class DiffAttention(nn.Module):
-    """Differential attention (T. Ye et al., "Differential Transformer", 2024): each head's map is the difference of two softmaxes, the second one weighted
+    """Differential attention after T. Ye et al., "Differential Transformer", 2024: each head's map is the difference of two softmaxes, the second one weighted
     with lambda = exp(q1 . k1) - exp(q2 . k2) + lambda_init from learned vectors, each head's output is normalised by itself and scaled with
-    1 - lambda_init.  ``heads`` heads of two maps of size hidden / (2 heads) and values of size hidden / heads, over ``kv_heads`` key heads."""
+    1 - lambda_init.  ``heads`` heads of two maps of size hidden / (2 heads) and values of size hidden / heads, over ``kv_heads`` key heads.
+
+    Not as there: lambda is a head's own, not the layer's, and a head's output goes through a layer norm with mean and bias, not a root-mean-square norm, so weights do
+    not carry over."""
 
     def __init__(self, hidden: int, heads: int, kv_heads: int = None, depth: int = 1, causal: bool = False, bias: bool = True, eps: float = 1e-5,
                  device=None, dtype=None):
