@@ -43,8 +43,9 @@ class Dropout(nn.Module):
 
     step: one int64 element on the GPU, by which the mask is numbered instead of by calls.  The training loop advances it between steps, after the
     backward pass; every call of a step draws the same mask, so what is computed again in the backward pass (activation checkpointing) and the replays
-    of a captured step are right.  Numbered by calls, a training call in a backward pass, under capture or in a DataParallel replica is an error: it would
-    draw another mask than the one whose gradient is wanted, or the same one in every step."""
+    of a captured step are right.  The word is the loop's to save, and a copy of the module has a copy of it.  Numbered by calls, a training call in a backward pass, under capture or in a DataParallel replica is an error: it would
+    draw another mask than the one whose gradient is wanted, or the same one in every step; and compiled code leaves its graph at every mask, which ``fullgraph``
+    refuses."""
 
     # for modules that were saved whole before they had these
     step, seed_given = None, True

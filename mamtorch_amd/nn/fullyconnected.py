@@ -33,9 +33,7 @@ __all__ = ["FullyConnected"]
 def check_counted(module: Module, step: str) -> None:
     """Refuses a mask that a module numbers by its training calls where calls do not number it: a forward that is computed again in a backward pass
     would draw another mask than the one whose gradient is wanted, the replays of a captured one and DataParallel's replicas the same in every step."""
-    if torch.compiler.is_compiling():
-        return
-    where = None
+    where = None        # compiled code leaves its graph for these questions, which every call asks again
     if torch._C._current_graph_task_id() != -1:
         where = "in a backward pass"
     elif getattr(module, "_is_replica", False):

@@ -126,3 +126,33 @@ def test_masks_numbered_by_calls_refuse_capture(name):
             module(x)
     torch.cuda.synchronize()
     module(x)
+
+
+@pytest.mark.parametrize("name", ["dropout", "fullyconnected", "layer"])
+def test_compiled_modules_draw_the_same_masks(name):
+    x = _inputs()
+    counted = _modules(None)[name].to(DEV).train()
+    other = copy.deepcopy(counted)
+    torch._dynamo.reset()
+    compiled = torch.compile(counted, backend="eager")
+    for _ in range(3):
+        _close([compiled(x).detach()], [other(x).detach()])
+    # computed again in a backward pass, with the check in the compiled code
+    y = checkpoint(lambda t: compiled(t).square(), x.requires_grad_(True), use_reentrant=False)
+    with pytest.raises(RuntimeError, match="in a backward pass"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["dropout", "fullyconnected", "layer"])
+def test_modules_with_a_step_compile_as_a_whole(name):
+    step, x = _step(3), _inputs()
+    module = _modules(step)[name].to(DEV).train()
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda t: module(t).square(), backend="eager", fullgraph=True)
+    for _ in range(2):
+        want = _run(module, _plain, x)
+        x1 = x.detach().requires_grad_(True)
+        for call in (compiled, lambda t: checkpoint(compiled, t, use_reentrant=False)):
+            y = call(x1)
+            _close([y.detach(), *torch.autograd.grad(y.sum(), [x1, *module.parameters()])], want)
+        step += 1
