@@ -369,7 +369,7 @@ def _plain_extend(state, counts):
     take = want + shared.long()
     until = take.cumsum(0)
     free = refs == 0
-    served = until <= free.sum()
+    served = (until <= free.sum()) | (take == 0)
     order = (~free).int().sort(stable=True).indices                 # free pages in order, then the others
     slot = torch.arange(slots, device=DEV)
     first = (until - take)[:, None]
