@@ -554,6 +554,91 @@ int mam_diff_attention_backward(const mam_diff_attention_t *args, const void *do
                                 const float *kept, const float *lse, void *dq, void *dk, void *dv, void *dlam, void *workspace,
                                 size_t workspace_bytes, void *stream);
 
+/*
+ * Norms of queries and keys for each head with the position rotation in the same pass: for each row of D elements of q (B, L, H, M, D) and k (B, L, Hkv, M, D)
+ *     y = R(place) (x / sqrt(mean(x^2) + eps) * weight)
+ * where R turns pair i of `pairs` by place * frequencies[i] radians: elements i and i + pairs, or (interleaved) 2 i and 2 i + 1; the elements behind the pairs are not turned.
+ * D <= 128; strides in elements, the last dimension has stride 1.
+ *   q_weight, k_weight (D) of `weight_type` (`type` or MAM_F32), or NULL;  norm 0: rotation alone
+ *   frequencies (pairs) fp64;  positions (B, L) int32 with strides, or NULL: the token's number.  The angle is formed in fp64.
+ */
+typedef struct mam_norm_rotate_t {
+    const void *q, *k, *q_weight, *k_weight;
+    int64_t q_stride[4], k_stride[4];                /* batch, token, head, map */
+    const double *frequencies;
+    const int32_t *positions;
+    int64_t position_stride[2];
+    int64_t B, L, H, Hkv, M, D, pairs;
+    double eps;
+    int norm, interleaved, type, weight_type;
+} mam_norm_rotate_t;
+
+/* q_out, k_out contiguous, of q's and k's shapes. */
+int mam_norm_rotate(const mam_norm_rotate_t *args, void *q_out, void *k_out, void *stream);
+/* From the outputs' gradients (strides of batch, token, head, map in HOST memory, last dimension 1): dq, dk contiguous, dq_weight, dk_weight (D) of weight_type; each may
+ * be NULL, and an output's gradient that none of them needs.  The workspace is for the weights' gradients.  Deterministic. */
+size_t mam_norm_rotate_backward_workspace(const mam_norm_rotate_t *args);
+int mam_norm_rotate_backward(const mam_norm_rotate_t *args, const void *q_grad, const int64_t *q_grad_stride, const void *k_grad,
+                             const int64_t *k_grad_stride, void *dq, void *dk, void *dq_weight, void *dk_weight, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/*
+ * A cache in pages of S tokens (a multiple of 16): keys k (P, Hkv, S, 2, D) and values v (P, Hkv, S, Dv), contiguous, from a multiple of 16 bytes on.
+ *   table (B, slots) int32: the page of a request's tokens slot * S .. slot * S + S - 1, -1: none;  lengths (B) int32: its tokens
+ *   counts (B) int32 or NULL: how many of a call's new tokens a request has, all where NULL
+ * What stands in them is device memory and is not trusted: no entry leads out of the pages, tokens without a page are not written and not seen.
+ */
+typedef struct mam_pages_t {
+    void *k, *v;
+    const int32_t *table, *lengths, *counts;
+    int64_t P, S, Hkv, D, Dv, B, slots;
+    int type;
+} mam_pages_t;
+
+/* mam_norm_rotate of q and k (M = 2) with new tokens behind those of the cache: q_out as there; keys, and the values v (B, L, Hkv, Dv; strides of batch, token, head in HOST
+ * memory), go to the pages of tokens lengths[b] + i.  positions NULL: lengths[b] + i.  Lengths are not changed. */
+int mam_norm_rotate_append(const mam_norm_rotate_t *args, const void *v, const int64_t *v_stride, const mam_pages_t *pages, void *q_out, void *stream);
+
+/*
+ * The bookkeeping of pages, on the device: refs (P) int32, how many requests hold a page, 0 where it is free.  At most 4096 requests.  Pages behind a request's
+ * tokens are its own.
+ *   extend: room for counts[b] tokens behind each request's, from the free pages of lowest number, in the requests' order.  A begun last page that other requests hold as well is
+ *           given up for a new one, but by the last request that holds it: copies (B, 2) gets (page, new page), which mam_pages_copy takes, or -1, -1.  granted (B): counts[b], or 0 where the
+ *           free pages or the slots do not reach; such a request is left as it was, and those behind it that need pages are too.
+ *   fork:   request b goes on from request sources[b] as it was before the call; one that goes on from none (a number that is no request) is left empty.
+ *   trim:   requests have ends[b] tokens (no more than their pages hold); pages behind are given back.
+ */
+size_t mam_pages_extend_workspace(int64_t B, int64_t slots, int64_t P);
+int mam_pages_extend(int32_t *table, const int32_t *lengths, int32_t *refs, const int32_t *counts, int32_t *granted, int32_t *copies, int64_t B,
+                     int64_t slots, int64_t P, int64_t S, void *workspace, size_t workspace_bytes, void *stream);
+int mam_pages_fork(int32_t *table, int32_t *lengths, int32_t *refs, const int32_t *sources, int64_t B, int64_t slots, int64_t P, int64_t S, void *stream);
+int mam_pages_trim(int32_t *table, int32_t *lengths, int32_t *refs, const int32_t *ends, int64_t B, int64_t slots, int64_t P, int64_t S, void *stream);
+/* Page copies[i][0] to copies[i][1], i below n; none where either is no page. */
+int mam_pages_copy(const mam_pages_t *pages, const int32_t *copies, int64_t n, void *stream);
+/* Token lengths[b] + path[b, i] becomes token lengths[b] + i, for i below counts[b] (n where NULL).  path (B, n) int32 ascends; from an entry on that does not, a
+ * request's tokens stay. */
+int mam_pages_compact(const mam_pages_t *pages, const int32_t *path, int64_t n, void *stream);
+/* Trees of n <= 64 drafted tokens: parents (B, n) int32, a token before it or -1 (so is anything else taken).  masks (B, n): bit j where token j is i itself or above it;
+ * positions (B, n): lengths[b] (0 where NULL) and how many are above it. */
+int mam_draft_tree(const int32_t *parents, const int32_t *lengths, int64_t *masks, int32_t *positions, int64_t B, int64_t n, void *stream);
+
+/*
+ * Differential attention (mam_diff_attention) of N new tokens q (B, N, H, 2, D) over the pages: every one sees the lengths[b] tokens of the cache, and of the new ones, which
+ * stand behind them in the pages, those up to itself or, N <= 64, those that its mask (masks (B, N), a bit a token) names.  out (B, N, H, Dv) contiguous; zeros for tokens from counts[b] on, and
+ * for those that see nothing.
+ */
+typedef struct mam_diff_attention_pages_t {
+    const void *q, *lam;
+    int64_t q_stride[4];
+    const int64_t *masks;
+    int64_t N, H;
+    double scale;
+    int lam_type;
+    mam_pages_t pages;
+} mam_diff_attention_pages_t;
+size_t mam_diff_attention_pages_workspace(const mam_diff_attention_pages_t *args);
+int mam_diff_attention_pages(const mam_diff_attention_pages_t *args, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

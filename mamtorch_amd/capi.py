@@ -50,6 +50,9 @@ EXPORTS = (
     "mam_dropout", "mam_layer_norm", "mam_layer_norm_backward_workspace", "mam_layer_norm_backward",
     "mam_add_dropout_layer_norm", "mam_add_dropout_layer_norm_backward",
     "mam_diff_attention_workspace", "mam_diff_attention", "mam_diff_attention_backward_workspace", "mam_diff_attention_backward",
+    "mam_norm_rotate", "mam_norm_rotate_backward_workspace", "mam_norm_rotate_backward", "mam_norm_rotate_append",
+    "mam_pages_extend_workspace", "mam_pages_extend", "mam_pages_fork", "mam_pages_trim", "mam_pages_copy", "mam_pages_compact", "mam_draft_tree",
+    "mam_diff_attention_pages_workspace", "mam_diff_attention_pages",
 )
 
 _i64 = ctypes.c_int64
@@ -71,6 +74,26 @@ class DiffAttention(ctypes.Structure):
                 ("lengths", _ptr), ("starts", _ptr), ("key_mask", _ptr), ("mask_stride", _i64)] + [
                 (n, _i64) for n in ("B", "Lq", "Lk", "H", "Hkv", "D", "Dv")] + [
                 ("scale", ctypes.c_double), ("causal", _int), ("type", _int), ("lam_type", _int)]
+
+
+class NormRotate(ctypes.Structure):
+    """mam_norm_rotate_t"""
+    _fields_ = [(n, _ptr) for n in ("q", "k", "q_weight", "k_weight")] + [
+        ("q_stride", _i64 * 4), ("k_stride", _i64 * 4), ("frequencies", _ptr), ("positions", _ptr), ("position_stride", _i64 * 2)] + [
+        (n, _i64) for n in ("B", "L", "H", "Hkv", "M", "D", "pairs")] + [
+        ("eps", ctypes.c_double), ("norm", _int), ("interleaved", _int), ("type", _int), ("weight_type", _int)]
+
+
+class Pages(ctypes.Structure):
+    """mam_pages_t"""
+    _fields_ = [(n, _ptr) for n in ("k", "v", "table", "lengths", "counts")] + [
+        (n, _i64) for n in ("P", "S", "Hkv", "D", "Dv", "B", "slots")] + [("type", _int)]
+
+
+class DiffAttentionPages(ctypes.Structure):
+    """mam_diff_attention_pages_t"""
+    _fields_ = [("q", _ptr), ("lam", _ptr), ("q_stride", _i64 * 4), ("masks", _ptr), ("N", _i64), ("H", _i64), ("scale", ctypes.c_double),
+                ("lam_type", _int), ("pages", Pages)]
 
 
 def lib():
@@ -151,6 +174,22 @@ def lib():
         l.mam_diff_attention_backward_workspace.argtypes = [_a]
         l.mam_diff_attention_backward_workspace.restype = _size
         l.mam_diff_attention_backward.argtypes = [_a, _ptr, ctypes.POINTER(_i64)] + [_ptr] * 8 + [_size, _ptr]
+        _r, _g, _ints = ctypes.POINTER(NormRotate), ctypes.POINTER(Pages), ctypes.POINTER(_i64)
+        l.mam_norm_rotate.argtypes = [_r, _ptr, _ptr, _ptr]
+        l.mam_norm_rotate_backward_workspace.argtypes = [_r]
+        l.mam_norm_rotate_backward_workspace.restype = _size
+        l.mam_norm_rotate_backward.argtypes = [_r, _ptr, _ints, _ptr, _ints] + [_ptr] * 5 + [_size, _ptr]
+        l.mam_norm_rotate_append.argtypes = [_r, _ptr, _ints, _g, _ptr, _ptr]
+        l.mam_pages_extend_workspace.argtypes = [_i64] * 3
+        l.mam_pages_extend_workspace.restype = _size
+        l.mam_pages_extend.argtypes = [_ptr] * 6 + [_i64] * 4 + [_ptr, _size, _ptr]
+        l.mam_pages_fork.argtypes = l.mam_pages_trim.argtypes = [_ptr] * 4 + [_i64] * 4 + [_ptr]
+        l.mam_pages_copy.argtypes = l.mam_pages_compact.argtypes = [_g, _ptr, _i64, _ptr]
+        l.mam_draft_tree.argtypes = [_ptr] * 4 + [_i64] * 2 + [_ptr]
+        _p = ctypes.POINTER(DiffAttentionPages)
+        l.mam_diff_attention_pages_workspace.argtypes = [_p]
+        l.mam_diff_attention_pages_workspace.restype = _size
+        l.mam_diff_attention_pages.argtypes = [_p, _ptr, _ptr, _size, _ptr]
         _f = ctypes.c_float
         l.mam_prune_row_offsets.argtypes = [_ptr, _i64, _int, _ptr, _ptr, _i64, _f, _ptr, _i64, _i64, _ptr]
         l.mam_prune_fill_csr.argtypes = [_ptr, _i64, _int, _ptr, _ptr, _i64, _f, _ptr, _ptr, _ptr, _i64, _i64, _ptr]
