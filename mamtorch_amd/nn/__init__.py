@@ -6,8 +6,8 @@ from .fullyconnected import FullyConnected
 from .convert import MAMMlp, add_mam_to_model, get_layers
 from .legacy import FullyConnectedV1, MAMDense
 from .conv import MAMConv1d, MAMConv2d
-from .encoder import LayerNorm, Dropout, DiffAttention, DiffAttentionCache, MAMEncoderLayer
+from .encoder import LayerNorm, Dropout, DiffAttention, DiffAttentionCache, DiffAttentionPages, PageTable, MAMEncoderLayer
 from . import compat, v1, v4
 
 __all__ = ["FullyConnected", "MAMMlp", "add_mam_to_model", "get_layers", "FullyConnectedV1", "MAMDense", "MAMConv1d", "MAMConv2d", "LayerNorm", "Dropout", "DiffAttention",
-           "DiffAttentionCache", "MAMEncoderLayer", "compat", "v1", "v4"]
+           "DiffAttentionCache", "DiffAttentionPages", "PageTable", "MAMEncoderLayer", "compat", "v1", "v4"]
