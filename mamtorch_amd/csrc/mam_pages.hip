@@ -85,75 +85,100 @@ __device__ __forceinline__ int before(int v, int *waves, int &total)
 // Room for counts[b] tokens behind each request's, by one workgroup.  What a request takes: pages for slots that have none, and one for a begun last page that others
 // hold too, unless they all come before it and take one themselves.  The requests' needs are added up, the free pages are ranked, and rank r goes to the request
 // whose needs reach past r.  A request whose needs go beyond what is free gets nothing, and so do those behind it that need any.
+//
+// Bound by latency: a request a thread (four where there are more than 1024), its few loads side by side, those of the first 16384 pages' counts before all.  Measured:
+// 256 requests of up to 1021 tokens, all of them beams of four that write to pages in common, 1507 pages, 10 us (four requests a thread from the start on: 24 us).
 constexpr int EXTEND = 1024, PER = MOST_REQUESTS / EXTEND, SCAN = 16;
+
+// Which of pages at .. at + 15 are free, a bit each.
+__device__ __forceinline__ uint32_t free_of(const Book &k, int at)
+{
+    uint32_t free = 0;
+    if (at + SCAN <= k.P) {
+        typedef int32_t words __attribute__((ext_vector_type(4), aligned(4)));
+        words w[SCAN / 4];
+#pragma unroll
+        for (int i = 0; i < SCAN / 4; ++i) w[i] = *reinterpret_cast<const words *>(k.refs + at + 4 * i);
+#pragma unroll
+        for (int i = 0; i < SCAN; ++i) free |= (uint32_t)(w[i / 4][i % 4] == 0) << i;
+    } else {
+        for (int i = 0; i < SCAN && at + i < k.P; ++i) free |= (uint32_t)(k.refs[at + i] == 0) << i;
+    }
+    return free;
+}
+
 __global__ __launch_bounds__(EXTEND) void extend_kernel(const Book k, const int32_t *__restrict__ counts, int32_t *__restrict__ granted,
                                                         int32_t *__restrict__ copies, int32_t *__restrict__ found)
 {
-    __shared__ int until[MOST_REQUESTS];        // needs of the requests up to this one
-    __shared__ int last[MOST_REQUESTS];         // begun last page that others hold too, or -1
+    __shared__ int until[MOST_REQUESTS];                                        // needs of the requests up to this one
+    __shared__ __attribute__((aligned(16))) int last[MOST_REQUESTS];           // begun last page that others hold too, or -1
     __shared__ int waves[EXTEND / 64];
     const int t = threadIdx.x;
-    int held[PER], want[PER], n_of[PER], c_of[PER];
+    uint32_t free = free_of(k, t * SCAN);
+    int held[PER], want[PER], n_of[PER], c_of[PER], copy[PER], first[PER];
+    bool shared = false;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-        const int b = t * PER + u;
-        held[u] = want[u] = n_of[u] = c_of[u] = 0;
-        if (b >= k.B) continue;
-        const int n = length_at(k, k.lengths[b]), c = counts[b];
-        const int32_t *row = k.table + (int64_t)b * k.slots;
-        const int64_t end = (int64_t)n + (c > 0 ? c : 0);
-        const bool fits = c > 0 && end <= (int64_t)k.slots * k.S;
-        const int slots = fits ? (int)((end + k.S - 1) / k.S) : 0, begun = n / k.S;
-        int page = -1;
-        if (fits && n % k.S) {
-            page = row[begun];
-            if (!is_page(k, page) || k.refs[page] < 2) page = -1;
-        }
-        last[b] = page;
-        int h = (n + k.S - 1) / k.S;
-        while (h < slots && row[h] >= 0) ++h;
-        held[u] = h;
-        want[u] = h < slots ? slots - h : 0;
-        n_of[u] = n;
-        c_of[u] = fits ? c : 0;
-    }
-    __syncthreads();
-    int copy[PER], mine = 0;
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-        const int b = t * PER + u;
+        const int b = u * EXTEND + t;
+        held[u] = want[u] = n_of[u] = c_of[u] = first[u] = 0;
         copy[u] = -1;
-        if (b < k.B && last[b] >= 0) {
-            int earlier = 0;
-            for (int i = 0; i < b; ++i) earlier += last[i] == last[b];
-            if (k.refs[last[b]] - earlier > 1) copy[u] = last[b];
+        if (b < k.B) {
+            const int n = length_at(k, k.lengths[b]), c = counts[b];
+            const int32_t *row = k.table + (int64_t)b * k.slots;
+            const int64_t end = (int64_t)n + (c > 0 ? c : 0);
+            const bool fits = c > 0 && end <= (int64_t)k.slots * k.S;
+            const int slots = fits ? (int)((end + k.S - 1) / k.S) : 0;
+            int h = (n + k.S - 1) / k.S, page = -1;
+            int behind = h < slots ? row[h] : -1;
+            if (fits && n % k.S) {
+                page = row[n / k.S];
+                if (!is_page(k, page) || k.refs[page] < 2) page = -1;
+            }
+            while (behind >= 0) {
+                ++h;
+                behind = h < slots ? row[h] : -1;
+            }
+            held[u] = h;
+            want[u] = h < slots ? slots - h : 0;
+            n_of[u] = n;
+            c_of[u] = fits ? c : 0;
+            last[b] = page;
+            shared = shared || page >= 0;
+        } else if (b < MOST_REQUESTS) {
+            last[b] = -1;
         }
-        mine += want[u] + (copy[u] >= 0);
     }
-    int total;
-    int sum = before<EXTEND>(mine, waves, total);
-    const int first = sum;
+    // of the requests that write to a page, the earlier ones give it up first
+    if (__syncthreads_or(shared)) {
+        typedef int quad __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int b = u * EXTEND + t, page = b < k.B ? last[b] : -1;
+            if (page < 0) continue;
+            int earlier = 0, i = 0;
+            for (; i + 4 <= b; i += 4) {
+                const quad w = *reinterpret_cast<const quad *>(last + i);
+                earlier += (w[0] == page) + (w[1] == page) + (w[2] == page) + (w[3] == page);
+            }
+            for (; i < b; ++i) earlier += last[i] == page;
+            if (k.refs[page] - earlier > 1) copy[u] = page;
+        }
+    }
+    int total = 0;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-        sum += want[u] + (copy[u] >= 0);
-        if (t * PER + u < k.B) until[t * PER + u] = sum;
+        if (u * EXTEND >= k.B) break;
+        const int take = want[u] + (copy[u] >= 0);
+        int all;
+        first[u] = total + before<EXTEND>(take, waves, all);
+        if (u * EXTEND + t < k.B) until[u * EXTEND + t] = first[u] + take;
+        total += all;
     }
     // the free pages of lowest number, as many as are needed, by rank
     int have = 0;
     for (int base = 0; base < k.P && have < total; base += EXTEND * SCAN) {
-        uint32_t free = 0;
         const int at = base + t * SCAN;
-        if (at + SCAN <= k.P) {
-            typedef int32_t words __attribute__((ext_vector_type(4), aligned(4)));
-#pragma unroll
-            for (int i = 0; i < SCAN; i += 4) {
-                const words w = *reinterpret_cast<const words *>(k.refs + at + i);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) free |= (uint32_t)(w[u] == 0) << (i + u);
-            }
-        } else {
-            for (int i = 0; i < SCAN && at + i < k.P; ++i) free |= (uint32_t)(k.refs[at + i] == 0) << i;
-        }
+        if (base > 0) free = free_of(k, at);
         int all;
         int rank = have + before<EXTEND>(__popc(free), waves, all);
         for (; free && rank < total; free &= free - 1) found[rank++] = at + __ffs(free) - 1;
@@ -162,26 +187,22 @@ __global__ __launch_bounds__(EXTEND) void extend_kernel(const Book k, const int3
     __threadfence_block();
     __syncthreads();
     // requests whose needs are met are the first ones, and of those behind them the ones without needs
-    int from = first;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-        const int b = t * PER + u, take = want[u] + (copy[u] >= 0);
-        if (b < k.B) {
-            const bool served = c_of[u] > 0 && (take == 0 || from + take <= have);
-            granted[b] = served ? c_of[u] : 0;
-            const bool moved = served && copy[u] >= 0;
-            const int to = moved ? found[from] : -1;
-            copies[2 * b] = moved ? copy[u] : -1;
-            copies[2 * b + 1] = to;
-            if (moved) {
-                atomicSub(&k.refs[copy[u]], 1);
-                k.refs[to] = 1;
-                k.table[(int64_t)b * k.slots + n_of[u] / k.S] = to;
-            }
-            // what the ranks below need of it: whether its first page is a copy's, and the slot of the next one
-            last[b] = served && want[u] > 0 ? 2 * held[u] + (copy[u] >= 0) : -1;
+        const int b = u * EXTEND + t, take = want[u] + (copy[u] >= 0);
+        if (b >= k.B) continue;
+        const bool served = c_of[u] > 0 && (take == 0 || first[u] + take <= have), moved = served && copy[u] >= 0;
+        const int to = moved ? found[first[u]] : -1;
+        granted[b] = served ? c_of[u] : 0;
+        copies[2 * b] = moved ? copy[u] : -1;
+        copies[2 * b + 1] = to;
+        if (moved) {
+            atomicSub(&k.refs[copy[u]], 1);
+            k.refs[to] = 1;
+            k.table[(int64_t)b * k.slots + n_of[u] / k.S] = to;
         }
-        from += take;
+        // what the ranks below need of it: whether its first page is a copy's, and the slot of the next one
+        last[b] = served && want[u] > 0 ? 2 * held[u] + (copy[u] >= 0) : -1;
     }
     __syncthreads();
     const int ranks = total < have ? total : have;
@@ -228,19 +249,29 @@ __global__ __launch_bounds__(TRIM) void trim_kernel(const Book k, const int32_t 
 }
 
 // Request b goes on from request sources[b]: its table becomes that one's, up to the page of its last token; a source that is no request leaves it empty.  A workgroup has
-// some columns of the table for itself, all requests of them in LDS, so that the table is changed in place.  The lengths, which every workgroup reads, change in a launch of
-// their own behind it.
-constexpr int FORK = 256, FORK_CELLS = 8192;
-__global__ __launch_bounds__(FORK) void fork_kernel(const Book k, const int32_t *__restrict__ sources, int columns)
+// some columns of the table for itself, all requests of them in LDS, so that the table is changed in place.  Every workgroup reads the lengths: where one has the whole
+// table it changes them at its end, else a launch of their own does.  Measured: 256 requests of 16 pages 6.5 us (17 and 4 us by 256 threads and a launch for the lengths).
+constexpr int FORK = 1024, FORK_CELLS = 8192;
+__device__ __forceinline__ void fork_lengths(const Book &k, const int32_t *sources, int32_t *old)
+{
+    for (int b = threadIdx.x; b < k.B; b += FORK) old[b] = length_at(k, k.lengths[b]);
+    __syncthreads();
+    for (int b = threadIdx.x; b < k.B; b += FORK) {
+        const int source = sources[b];
+        k.lengths[b] = source >= 0 && source < k.B ? old[source] : 0;
+    }
+}
+
+__global__ __launch_bounds__(FORK) void fork_kernel(const Book k, const int32_t *__restrict__ sources, int columns, int whole)
 {
     __shared__ int32_t old[FORK_CELLS];
-    const int first = blockIdx.x * columns, width = k.slots - first < columns ? k.slots - first : columns;
-    for (int e = threadIdx.x; e < k.B * width; e += FORK) {
+    const int first = blockIdx.x * columns, width = k.slots - first < columns ? k.slots - first : columns, cells = k.B * width;
+    for (int e = threadIdx.x; e < cells; e += FORK) {
         const int b = e / width, c = e - b * width;
         old[e] = k.table[(int64_t)b * k.slots + first + c];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < k.B * width; e += FORK) {
+    for (int e = threadIdx.x; e < cells; e += FORK) {
         const int b = e / width, c = e - b * width, source = sources[b];
         int page = -1;
         if (source >= 0 && source < k.B && first + c < (length_at(k, k.lengths[source]) + k.S - 1) / k.S) page = old[source * width + c];
@@ -250,17 +281,16 @@ __global__ __launch_bounds__(FORK) void fork_kernel(const Book k, const int32_t 
         if (is_page(k, page)) atomicAdd(&k.refs[page], 1);
         if (is_page(k, was)) atomicSub(&k.refs[was], 1);
     }
+    if (whole) {
+        __syncthreads();
+        fork_lengths(k, sources, old);
+    }
 }
 
-__global__ __launch_bounds__(1024) void fork_lengths_kernel(const Book k, const int32_t *__restrict__ sources)
+__global__ __launch_bounds__(FORK) void fork_lengths_kernel(const Book k, const int32_t *__restrict__ sources)
 {
     __shared__ int32_t old[MOST_REQUESTS];
-    for (int b = threadIdx.x; b < k.B; b += 1024) old[b] = length_at(k, k.lengths[b]);
-    __syncthreads();
-    for (int b = threadIdx.x; b < k.B; b += 1024) {
-        const int source = sources[b];
-        k.lengths[b] = source >= 0 && source < k.B ? old[source] : 0;
-    }
+    fork_lengths(k, sources, old);
 }
 
 typedef uint32_t Words __attribute__((ext_vector_type(4)));
@@ -403,14 +433,16 @@ extern "C" int mam_pages_fork(int32_t *table, int32_t *lengths, int32_t *refs, c
     if (rc != MAM_OK || k.B == 0) return rc;
     if (!sources) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (k.slots > 0) {
-        int columns = pages::FORK_CELLS / k.B;          // 2 at least: FORK_CELLS is twice the most requests
-        if (columns > 32) columns = 32;
-        hipLaunchKernelGGL(pages::fork_kernel, dim3((unsigned)ceil_div(k.slots, columns)), dim3(pages::FORK), 0, st, k, sources, columns);
+    const int64_t cells = (int64_t)k.B * k.slots;
+    const bool whole = cells > 0 && cells <= pages::FORK_CELLS;
+    if (cells > 0) {
+        int columns = whole ? k.slots : (int)ceil_div(k.slots, kNumCU);         // as many workgroups as CUs, of 2 columns at most where there are 4096 requests
+        if (columns > pages::FORK_CELLS / k.B) columns = pages::FORK_CELLS / k.B;
+        hipLaunchKernelGGL(pages::fork_kernel, dim3((unsigned)ceil_div(k.slots, columns)), dim3(pages::FORK), 0, st, k, sources, columns, (int)whole);
         rc = check_launch("pages::fork_kernel");
-        if (rc != MAM_OK) return rc;
+        if (rc != MAM_OK || whole) return rc;
     }
-    hipLaunchKernelGGL(pages::fork_lengths_kernel, dim3(1), dim3(1024), 0, st, k, sources);
+    hipLaunchKernelGGL(pages::fork_lengths_kernel, dim3(1), dim3(pages::FORK), 0, st, k, sources);
     return check_launch("pages::fork_lengths_kernel");
 }
 

@@ -384,6 +384,27 @@ Tensor norm_rotate_append_autograd(const Tensor &q, const Tensor &k, const Tenso
     return op.call(q, k, v, k_pages, v_pages, table, lengths, counts, q_weight, k_weight, frequencies, positions, eps, norm, interleaved);
 }
 
+typedef void CopySignature(const Tensor &, const Tensor &, const Tensor &);
+
+void pages_copy_autograd(const Tensor &k_pages, const Tensor &v_pages, const Tensor &copies)
+{
+    static const auto op = find<CopySignature>("mamtorch_kernel_encoder::pages_copy");
+    check_serving(recording(k_pages, v_pages), "pages_copy");
+    at::AutoDispatchBelowADInplaceOrView below;
+    op.call(k_pages, v_pages, copies);
+}
+
+typedef void CompactSignature(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const MaybeTensor &);
+
+void pages_compact_autograd(const Tensor &k_pages, const Tensor &v_pages, const Tensor &table, const Tensor &lengths, const Tensor &path,
+                            const MaybeTensor &counts)
+{
+    static const auto op = find<CompactSignature>("mamtorch_kernel_encoder::pages_compact");
+    check_serving(recording(k_pages, v_pages), "pages_compact");
+    at::AutoDispatchBelowADInplaceOrView below;
+    op.call(k_pages, v_pages, table, lengths, path, counts);
+}
+
 typedef Tensor PagesSignature(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, double, const MaybeTensor &,
                               const MaybeTensor &);
 
@@ -436,4 +457,8 @@ TORCH_LIBRARY_IMPL(mamtorch_kernel_encoder, Autograd, m)
     m.impl("norm_rotate", &norm_rotate_autograd);
     m.impl("norm_rotate_append", &norm_rotate_append_autograd);
     m.impl("diff_attention_pages", &diff_attention_pages_autograd);
+    m.impl("pages_copy", &pages_copy_autograd);
+    m.impl("pages_compact", &pages_compact_autograd);
+    // whole numbers alone: nothing for autograd to look at
+    for (const char *name : {"pages_extend", "pages_fork", "pages_trim", "draft_tree"}) m.impl(name, torch::CppFunction::makeFallthrough());
 }
