@@ -13,7 +13,10 @@ namespace mam {
 namespace attention {
 
 constexpr int ROWS = 16;                // rows of a wave
-constexpr float SLACK = 8.0f;           // see mam_attention.hip
+#ifndef FEWROWS
+#define FEWROWS 16
+#endif
+constexpr int FEW = FEWROWS;
 
 // A request's table, walked in steps of 16 tokens.
 struct Walk {
@@ -331,19 +334,262 @@ __global__ __launch_bounds__(256, D > 64 || (sizeof(T) == 4 && DV > 64) ? 1 : 2)
     }
 }
 
-// Workgroups that share a row's keys: two a CU over the whole call, but 64 keys a wave at least of what a request has room for.
-inline int pages_split_count(const Call &a)
+// ---- more rows: tiles of keys in LDS ----
+// Where a key head has more rows than a wave takes, every wave for itself reads K and V again from the L2: 128 rows a key head (trees of 32 tokens, four heads each) 99 us.  Here eight waves
+// share them: four row groups of TR rows, and two halves of the workgroup's keys, each with a tile of 32 keys in LDS for its four waves.  The halves meet in LDS, the workgroups
+// that share a row's keys in the workspace.
+//
+// ROWS16 rounded once: what 16 bits leave of the first map's probabilities is not kept here, as in mam_attention.hip's kernels for many rows; a product more for 0.0019 against 0.0024.
+
+// 32 rows of MAPS segments of W elements between the pages and LDS by 256 threads (Stage, with 16 rows in a page each).
+template <class T, int MAPS, int W, bool FAST>
+struct PageStage {
+    typedef Stage<T, 256, KT, MAPS, W, FAST> Dense;
+    static constexpr int PITCH = Dense::PITCH, N = Dense::N, SEGMENT = Dense::SEGMENT, PER = Dense::PER;
+    static_assert(64 / PER <= 16, "the rows of a wave's pieces stand in one page");
+    Frag<T> piece[N];
+
+    static __device__ __forceinline__ int thread() { return threadIdx.x & 255; }
+    static __device__ __forceinline__ uint32_t first_of(int i) { return (i * 256 + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3) * 64u); }
+    static __device__ __forceinline__ int map_of(int i) { return MAPS == 1 ? 0 : (int)(first_of(i) / SEGMENT); }
+    static __device__ __forceinline__ int block_of(int i) { return (int)(first_of(i) % SEGMENT / PER / 16); }
+    static __device__ __forceinline__ int row_of(int i) { return (int)((i * 256 + thread()) % SEGMENT / PER); }
+    static __device__ __forceinline__ int column_of(int i) { return (int)((i * 256 + thread()) % SEGMENT % PER * FE<T>); }
+
+    // row0, row1: where the two halves of 16 begin, -1: nowhere; left: how many of the 32 there are.  Others are zeros.
+    __device__ __forceinline__ void load(const T *pool, int64_t row0, int64_t row1, int width, int left)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t begin = block_of(i) ? row1 : row0;
+            const T *base = pool + (begin < 0 ? 0 : begin) * (MAPS * width) + map_of(i) * width;
+            const bool ok = begin >= 0 && row_of(i) < left && column_of(i) < width;
+            const uint32_t off = (uint32_t)(row_of(i) & 15) * (uint32_t)(MAPS * width) + (uint32_t)column_of(i);
+            if constexpr (FAST) {
+                piece[i] = buffer_frag<T>(base, ok ? off * (uint32_t)sizeof(T) : NOWHERE);
+            } else {
+#pragma unroll
+                for (int u = 0; u < FE<T>; ++u) piece[i][u] = (T)0.0f;
+                if (ok) piece[i] = load_frag<T>(base + off, width - column_of(i));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *tile) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<Frag<T> *>(tile + place_of<T>(row_of(i)) * PITCH + map_of(i) * W + column_of(i)) = piece[i];
+    }
+};
+
+constexpr int LDS_BYTES = 160 * 1024;
+template <class T, int D, int DV>
+constexpr int TILE_BYTES = KT * (2 * D + DV + 2 * FE<T>) * (int)sizeof(T);
+// Tiles of a half of the workgroup: one is written while the other is read, where both fit.
+template <class T, int D, int DV>
+constexpr int PAGE_TILES = 4 * TILE_BYTES<T, D, DV> <= LDS_BYTES - 1024 ? 2 : 1;
+
+template <class T, int TR, int D, int DV, bool FAST>
+__global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks, void *out, float *partial,
+                                                            int splits, int row_tiles)
 {
-    const int64_t rows = (int64_t)a.B * a.Hkv * ceil_div(a.R, ROWS), most = ceil_div(a.Lk, 4 * 64);
-    int64_t n = ceil_div(2 * (int64_t)kNumCU, rows);
-    if (n > 64) n = 64;
-    if (n > most) n = most;
-    return n < 1 ? 1 : (int)n;
+    constexpr int BUFFERS = PAGE_TILES<T, D, DV>, AR = TR * TR / 64, ACC = DV / TR * AR;
+    typedef PageStage<T, 2, D, FAST> StageK;
+    typedef PageStage<T, 1, DV, FAST> StageV;
+    constexpr int TILES_AT = 2 * BUFFERS * TILE_BYTES<T, D, DV>, JOIN_AT = 4 * 64 * ACC * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[TILES_AT > JOIN_AT ? TILES_AT : JOIN_AT];
+    __shared__ float tops[2][4][TR], sums[2][4][TR];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2, heads = a.B * a.Hkv;
+    const int bh = blockIdx.x % heads, rest_id = blockIdx.x / heads, tile = row_tiles - 1 - rest_id % row_tiles, split = rest_id / row_tiles;
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int length = length_of(p, b), count = count_of(p, b, a.Lq), room = p.slots * p.S;
+    const int first = tile * 4 * TR + (wave & 3) * TR, row = first + lane_row<TR>();
+    const int query = row < a.R ? row / a.G : 0;
+    const bool there = row < a.R && query < count;
+    const uint64_t mask = masks && there ? (uint64_t)masks[(int64_t)b * a.Lq + query] : 0;
+    const int limit = there ? length + (masks ? count : query + 1) : 0;
+    // keys that rows up to `last` see at most: none where the first of them is no query
+    const auto reach = [&](int from, int last) {
+        const int q = (last < a.R ? last : a.R - 1) / a.G;
+        const int n = length + (masks || q + 1 > count ? count : q + 1);
+        return from >= a.R || from / a.G >= count ? 0 : n < room ? n : room;
+    };
+    const int wave_any = reach(first, first + TR - 1), any = reach(tile * 4 * TR, tile * 4 * TR + 4 * TR - 1);
+    // and those that every row of the wave sees (rows that are none see what they like)
+    const int wave_all = masks || wave_any == 0 ? length : length + first / a.G + 1;
+    // the workgroup's tiles, and this half's
+    const int tiles = (any + KT - 1) / KT, per = (tiles + splits - 1) / splits, from = split * per < tiles ? split * per : tiles;
+    const int mine = from + per < tiles ? per : tiles - from, part = (mine + 1) / 2;
+    const int begin = from + half * part, number = half ? mine - part : part;
+
+    const Source<T> qs{static_cast<const T *>(a.q) + b * a.qb + (int64_t)hk * a.G * a.qh, a.ql, a.qh, a.qm, a.G, a.d, a.inverse};
+    Frag<T> q[2][D / KS<T, TR>];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
+    const float c = a.scale * LOG2E;
+    State<T, TR, D, DV, true> state;
+    state.clear();
+
+    T *k_tile = reinterpret_cast<T *>(lds + half * BUFFERS * TILE_BYTES<T, D, DV>), *v_tile = k_tile + KT * StageK::PITCH;
+    constexpr int NEXT = TILE_BYTES<T, D, DV> / (int)sizeof(T);
+    StageK k_stage;
+    StageV v_stage;
+    Walk walk(p, b, hk, begin * KT);
+    uint32_t pages = 0, next_pages = 0;         // which halves of the tile have a page
+    const auto load = [&](int t) {
+        const int64_t row0 = walk.next(), row1 = walk.next();
+        next_pages = (row0 < 0 ? 0u : 0xffffu) | (row1 < 0 ? 0u : 0xffff0000u);
+        k_stage.load(static_cast<const T *>(p.k), row0, row1, a.d, any - t * KT);
+        v_stage.load(static_cast<const T *>(p.v), row0, row1, a.dv, any - t * KT);
+    };
+    if (number > 0) {
+        load(begin);
+        if (BUFFERS == 2) {
+            k_stage.store(k_tile);
+            v_stage.store(v_tile);
+        }
+    }
+    // A tile's part of the loop, with `use` what a wave does that sees some of its keys.  The first half has as many tiles as the second, or one more; waves that are past their
+    // keys go on loading for the others, in a loop of its own (a condition around the products has the accumulators copied in every tile).
+    int now = 0, i = 0;
+    const auto tile_of = [&](const auto &use) {
+        const bool more = i + 1 < number;
+        if (BUFFERS == 1) {
+            __syncthreads();
+            if (i < number) {
+                k_stage.store(k_tile);
+                v_stage.store(v_tile);
+            }
+        }
+        pages = next_pages;
+        if (more) load(begin + i + 1);
+        __syncthreads();
+        use((begin + i) * KT, k_tile + now * NEXT, v_tile + now * NEXT);
+        if (BUFFERS == 2) {
+            now ^= 1;
+            if (more) {         // the other tile: every wave is past it
+                k_stage.store(k_tile + now * NEXT);
+                v_stage.store(v_tile + now * NEXT);
+            }
+        }
+        ++i;
+    };
+    const int open = (wave_all < wave_any ? wave_all : wave_any) / KT - begin, seen = (wave_any + KT - 1) / KT - begin;
+    while (i < number && i < open && next_pages == 0xffffffffu)
+        tile_of([&](int, const T *k, const T *v) { state.template keys<false, false>(q, k, StageK::PITCH, v, StageV::PITCH, c, 0, 0); });
+    while (i < number && i < seen)
+        tile_of([&](int key, const T *k, const T *v) {
+            const uint32_t word = (masks ? seen_word(key, length, mask) : 0xffffffffu) & pages;
+            state.template keys<true, false>(q, k, StageK::PITCH, v, StageV::PITCH, c, limit - key, word);
+        });
+    while (i < part) tile_of([](int, const T *, const T *) {});
+
+    // the halves: the second one's sums, then its products map by map; a row that is no query's has seen nothing
+    float factor[2], total[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        total[m] = there ? groups_sum<TR>(state.sum[m]) : 0.0f;
+        if (!there) state.top[m] = -INFINITY;
+    }
+    __syncthreads();
+    if (half && lane_group<TR>() == 0) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            tops[m][wave & 3][lane_row<TR>()] = state.top[m];
+            sums[m][wave & 3][lane_row<TR>()] = total[m];
+        }
+    }
+    float *cells = reinterpret_cast<float *>(lds) + (wave & 3) * 64 * ACC + (threadIdx.x & 63);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        if (m) __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int blk = 0; blk < DV / TR; ++blk)
+#pragma unroll
+                for (int f = 0; f < AR; ++f) cells[(blk * AR + f) * 64] = state.o[m][blk][f];
+        }
+        __syncthreads();
+        if (!half) {
+            // a range of which a row sees nothing has a sum of 0, and its products do not count whatever the values there hold
+            const float top = tops[m][wave & 3][lane_row<TR>()], sum = sums[m][wave & 3][lane_row<TR>()], most = fmaxf(top, state.top[m]);
+            const float old = total[m] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(state.top[m] - most), more = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top - most);
+#pragma unroll
+            for (int blk = 0; blk < DV / TR; ++blk)
+#pragma unroll
+                for (int f = 0; f < AR; ++f) {
+                    const float x = total[m] == 0.0f ? 0.0f : state.o[m][blk][f] * old, y = sum == 0.0f ? 0.0f : cells[(blk * AR + f) * 64] * more;
+                    state.o[m][blk][f] = x + y;
+                }
+            total[m] = (total[m] == 0.0f ? 0.0f : total[m] * old) + (sum == 0.0f ? 0.0f : sum * more);
+            state.top[m] = most;
+        }
+    }
+    if (half || row >= a.R) return;
+    if (splits == 1) {
+        const int head = hk * a.G + row - query * a.G;
+        const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
+#pragma unroll
+        for (int m = 0; m < 2; ++m) factor[m] = total[m] > 0.0f ? 1.0f / total[m] : 0.0f;
+        T *to = static_cast<T *>(out) + (((int64_t)b * a.Lq + query) * a.H + head) * a.dv;
+#pragma unroll
+        for (int blk = 0; blk < DV / TR; ++blk)
+#pragma unroll
+            for (int f = 0; f < AR; f += 4) {
+                const int col = blk * TR + (f / 4) * 4 * GROUPS<TR> + 4 * lane_group<TR>();
+                if (col >= a.dv) continue;
+                float r[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) r[u] = fmaf(-lam, state.o[1][blk][f + u] * factor[1], state.o[0][blk][f + u] * factor[0]);
+                store_pack<T, 4>(to + col, a.dv - col, r);
+            }
+    } else {
+        float *to = partial + (((int64_t)split * a.B * a.Hkv + bh) * a.R + row) * (2 * (int64_t)a.dv + 4);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int blk = 0; blk < DV / TR; ++blk)
+#pragma unroll
+                for (int f = 0; f < AR; f += 4) {
+                    const int col = blk * TR + (f / 4) * 4 * GROUPS<TR> + 4 * lane_group<TR>();
+                    if (col >= a.dv) continue;
+                    float r[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) r[u] = state.o[m][blk][f + u];
+                    store_pack<float, 4>(to + m * a.dv + col, a.dv - col, r);
+                }
+            if (lane_group<TR>() == 0) {
+                to[2 * a.dv + 2 * m] = state.top[m];
+                to[2 * a.dv + 2 * m + 1] = total[m];
+            }
+        }
+    }
 }
 
-inline size_t pages_workspace(const Call &a)
+// How a call runs: rows of a wave in tiles (0: streamed, 16 rows), workgroups that share a row's keys.
+struct Plan { int tr, splits; };
+
+// Rows of a wave's tile in LDS; streamed rows where a key head has few.
+inline int tile_rows(const Call &a, int type)
 {
-    const int n = pages_split_count(a);
+    if (a.R <= FEW) return 0;
+    return type == MAM_F32 || a.d > 64 || a.dv > 128 || a.R <= 64 ? 16 : 32;
+}
+
+// Workgroups that share a row's keys: two a CU over the whole call, but 64 keys a wave at least of what a request has room for; of the tiles' eight waves one a CU.
+inline Plan plan_of(const Call &a, int type)
+{
+    Plan p{tile_rows(a, type), 1};
+    const int64_t rows = (int64_t)a.B * a.Hkv * ceil_div(a.R, p.tr ? 4 * p.tr : ROWS), most = ceil_div(a.Lk, 4 * 64);
+    int64_t n = p.tr ? kNumCU / (rows > 0 ? rows : 1) : ceil_div(2 * (int64_t)kNumCU, rows);
+    if (n > 64) n = 64;
+    if (n > most) n = most;
+    p.splits = n < 1 ? 1 : (int)n;
+    return p;
+}
+
+inline size_t pages_workspace(const Call &a, int type)
+{
+    const int n = plan_of(a, type).splits;
     return n > 1 ? (size_t)n * a.B * a.Hkv * a.R * partial_size(a) * sizeof(float) : 0;
 }
 
@@ -354,16 +600,33 @@ struct PagesRun {
     const int64_t *masks;
     void *out;
     float *partial;
+    Plan plan;
     hipStream_t st;
+    template <int D, int DV, int TR, bool FAST>
+    void tiles(dim3 grid, int row_tiles) const
+    {
+        hipLaunchKernelGGL((page_tiles_kernel<T, TR, D, DV, FAST>), grid, dim3(512), 0, st, a, p, masks, out, partial, plan.splits, row_tiles);
+    }
     template <int D, int DV>
     int operator()() const
     {
-        const int splits = pages_split_count(a);
-        const int64_t row_tiles = ceil_div(a.R, ROWS), blocks = row_tiles * a.B * a.Hkv * splits;
+        const int64_t row_tiles = ceil_div(a.R, plan.tr ? 4 * plan.tr : ROWS), blocks = row_tiles * a.B * a.Hkv * plan.splits;
         if (blocks > INT32_MAX) return fail(MAM_ERR_UNSUPPORTED, "too many tiles");
         const dim3 grid((unsigned)blocks);
-        if (a.fast) hipLaunchKernelGGL((pages_kernel<T, D, DV, true>), grid, dim3(256), 0, st, a, p, masks, out, partial, splits, (int)row_tiles);
-        else hipLaunchKernelGGL((pages_kernel<T, D, DV, false>), grid, dim3(256), 0, st, a, p, masks, out, partial, splits, (int)row_tiles);
+        if (plan.tr == 32) {
+            if constexpr (sizeof(T) == 2 && D <= 64) {
+                if (a.fast) tiles<D, DV, 32, true>(grid, (int)row_tiles);
+                else tiles<D, DV, 32, false>(grid, (int)row_tiles);
+            }
+            return check_launch("attention::page_tiles_kernel");
+        }
+        if (plan.tr) {
+            if (a.fast) tiles<D, DV, 16, true>(grid, (int)row_tiles);
+            else tiles<D, DV, 16, false>(grid, (int)row_tiles);
+            return check_launch("attention::page_tiles_kernel");
+        }
+        if (a.fast) hipLaunchKernelGGL((pages_kernel<T, D, DV, true>), grid, dim3(256), 0, st, a, p, masks, out, partial, plan.splits, (int)row_tiles);
+        else hipLaunchKernelGGL((pages_kernel<T, D, DV, false>), grid, dim3(256), 0, st, a, p, masks, out, partial, plan.splits, (int)row_tiles);
         return check_launch("attention::pages_kernel");
     }
 };
@@ -399,7 +662,7 @@ extern "C" size_t mam_diff_attention_pages_workspace(const mam_diff_attention_pa
     attention::Call a;
     Pages p;
     if (attention::fill_pages_call(args, a, p) != MAM_OK || a.B == 0 || a.R == 0) return 0;
-    return attention::pages_workspace(a);
+    return attention::pages_workspace(a, args->pages.type);
 }
 
 extern "C" int mam_diff_attention_pages(const mam_diff_attention_pages_t *args, void *out, void *workspace, size_t workspace_bytes, void *stream)
@@ -410,14 +673,15 @@ extern "C" int mam_diff_attention_pages(const mam_diff_attention_pages_t *args, 
     int rc = attention::fill_pages_call(args, a, p);
     if (rc != MAM_OK || a.B == 0 || a.R == 0) return rc;
     if (!a.q || !a.lam || !out || (p.P > 0 && (!p.k || !p.v))) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
-    const size_t need = attention::pages_workspace(a);
+    const size_t need = attention::pages_workspace(a, args->pages.type);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(MAM_ERR_WORKSPACE, "the attention needs %zu workspace bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);
     hipStream_t st = static_cast<hipStream_t>(stream);
     float *partial = need > 0 ? static_cast<float *>(workspace) : nullptr;
-    if (args->pages.type == MAM_F32) rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<float>{a, p, args->masks, out, partial, st});
-    else if (args->pages.type == MAM_BF16) rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<bf16>{a, p, args->masks, out, partial, st});
-    else rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<f16>{a, p, args->masks, out, partial, st});
+    const attention::Plan plan = attention::plan_of(a, args->pages.type);
+    if (args->pages.type == MAM_F32) rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<float>{a, p, args->masks, out, partial, plan, st});
+    else if (args->pages.type == MAM_BF16) rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<bf16>{a, p, args->masks, out, partial, plan, st});
+    else rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<f16>{a, p, args->masks, out, partial, plan, st});
     if (rc != MAM_OK || need == 0) return rc;
-    return attention::join_parts(a, args->pages.type, out, partial, attention::pages_split_count(a), st);
+    return attention::join_parts(a, args->pages.type, out, partial, plan.splits, st);
 }

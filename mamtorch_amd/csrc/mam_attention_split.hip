@@ -17,7 +17,6 @@ namespace mam {
 namespace attention {
 
 constexpr int ROWS = 16;                // rows of a wave
-constexpr float SLACK = 8.0f;           // see mam_attention.hip
 
 // Workgroups that share a row's keys: two a CU over the whole call, but 64 keys a wave at least.
 inline int split_count(const Call &a)
