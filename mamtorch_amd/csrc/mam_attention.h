@@ -533,10 +533,6 @@ int fill_call(const mam_diff_attention_t *a, Call &c);
 bool use_split(const Call &a, int type, bool keep);
 size_t split_workspace(const Call &a);
 int run_split(const Call &a, int type, void *out, void *workspace, size_t workspace_bytes, hipStream_t st);
-// The parts of every row, `splits` (at most 64) planes of split_workspace()'s rows, as the result.
-int join_parts(const Call &a, int type, void *out, const float *partial, int splits, hipStream_t st);
-// A partial row: both maps' products relative to their maxima, then maximum and sum of each.
-inline int64_t partial_size(const Call &a) { return 2 * (int64_t)a.dv + 4; }
 
 }  // namespace attention
 }  // namespace mam

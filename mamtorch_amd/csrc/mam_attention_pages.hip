@@ -11,12 +11,13 @@
 
 namespace mam {
 namespace attention {
+namespace {         // names of mam_attention_split.hip's own parts, for the paged ones
 
 constexpr int ROWS = 16;                // rows of a wave
-#ifndef FEWROWS
-#define FEWROWS 16
-#endif
-constexpr int FEW = FEWROWS;
+
+// A partial row: both maps' products relative to their maxima, then maximum and sum of each.
+inline int64_t partial_size(const Call &a) { return 2 * (int64_t)a.dv + 4; }
+constexpr int FEW = 16;                 // rows of a key head that are streamed
 
 // A value that all lanes share, where the compiler does not see it: loops over it are branches of the wave, not of lanes.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -57,6 +58,45 @@ struct Walk {
     }
 };
 
+// The same as pointers to a key head's rows: a page's are found once, and 16 tokens on they are a step on.
+struct PageWalk {
+    Walk walk;
+    const unsigned char *k_pages, *v_pages, *k, *v;
+    int64_t k_row, v_row;               // bytes
+    int left;                           // tokens of the page from the pointers on
+    bool there;
+
+    __device__ __forceinline__ PageWalk(const Pages &p, int b, int head, int key, int size)
+        : walk(p, b, head, key), k_pages(static_cast<const unsigned char *>(p.k)), v_pages(static_cast<const unsigned char *>(p.v)), k_row(2 * p.d * size), v_row(p.dv * size)
+    {
+        find();
+    }
+    __device__ __forceinline__ void find()
+    {
+        left = walk.S - walk.off;
+        const int64_t row = walk.next();
+        there = row >= 0;
+        k = k_pages + (there ? row : 0) * k_row;
+        v = v_pages + (there ? row : 0) * v_row;
+    }
+    __device__ __forceinline__ bool next(const unsigned char *&k_rows, const unsigned char *&v_rows)
+    {
+        const bool was = there;
+        k_rows = k;
+        v_rows = v;
+        left -= 16;
+        if (left == 0) {
+            walk.slot += walk.off > 0;          // the walk has looked at the page's first tokens alone
+            walk.off = 0;
+            find();
+        } else {
+            k += 16 * k_row;
+            v += 16 * v_row;
+        }
+        return was;
+    }
+};
+
 // Bits of the keys key .. key + 31 that a row sees: all of the cache's `length`, then those that `mask` names.
 __device__ __forceinline__ uint32_t seen_word(int key, int length, uint64_t mask)
 {
@@ -65,6 +105,58 @@ __device__ __forceinline__ uint32_t seen_word(int key, int length, uint64_t mask
     if (behind >= 0) return (uint32_t)(mask >> behind);
     if (behind <= -32) return 0xffffffffu;
     return ((1u << -behind) - 1) | (uint32_t)(mask << -behind);
+}
+
+// A workgroup's share of a call: a request, and which part of its keys.  The slots go to the requests by their lengths: one each, the others in proportion, as far as a part keeps
+// LEAST_TILES tiles.  Every wave works them out for itself from the lengths, a request a lane.
+constexpr int LEAST_TILES = 8;
+struct Share { int b, part, parts, slot; };
+
+__device__ __forceinline__ Share share_of(const Call &a, const Pages &p, int slot, int slots, int32_t *spans)
+{
+    if (slots == a.B) return {slot, 0, 1, slot};
+    const int lane = threadIdx.x & 63, width = a.B < 64 ? a.B : 64;        // lanes that have requests
+    const auto tiles_of = [&](int b) {
+        if (b >= a.B) return 0;
+        const int count = count_of(p, b, a.Lq), most = p.slots * p.S, n = length_of(p, b) + count;
+        return count == 0 ? 0 : ((n < most ? n : most) + KT - 1) / KT;
+    };
+    float all = 0.0f;
+    for (int b = lane; b - lane < a.B; b += 64) all += (float)tiles_of(b);
+    for (int x = 1; x < width; x <<= 1) all += __shfl_xor(all, x);
+    all = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, all)));
+    // a little less than the proportion, so that rounding gives out no slot too many
+    const float each = all > 0.0f ? (float)(slots - a.B) / all * (1.0f - 0x1p-18f) : 0.0f;
+    int before = 0;
+    Share s{-1, 0, 0, slot};
+    for (int b = lane; b - lane < a.B; b += 64) {
+        const int tiles = tiles_of(b), most = tiles / LEAST_TILES < 64 ? tiles / LEAST_TILES : 64;
+        int n = 1 + (int)((float)tiles * each);
+        if (n > most) n = most > 1 ? most : 1;
+        if (b >= a.B) n = 0;
+        int until = n;
+        for (int x = 1; x < width; x <<= 1) {
+            const int t = __shfl_up(until, x);
+            if (lane >= x) until += t;
+        }
+        until += before;
+        const uint64_t mine = __ballot(slot < until && slot >= until - n);
+        if (mine) {
+            const int l = __ffsll((unsigned long long)mine) - 1;
+            s.b = uniform(b - lane + l);
+            s.parts = uniform(__shfl(n, l));
+            s.part = uniform(slot - (__shfl(until, l) - s.parts));
+        }
+        before = __shfl(until, 63);
+    }
+    s.b = uniform(s.b);
+    s.part = uniform(s.part);
+    s.parts = uniform(s.parts);
+    if (s.b >= 0 && s.part == 0 && threadIdx.x == 0) {
+        spans[2 * s.b] = slot;
+        spans[2 * s.b + 1] = s.parts;
+    }
+    return s;
 }
 
 template <class T, int PE, bool FAST>
@@ -104,7 +196,8 @@ __device__ __forceinline__ void page_piece(const T *base, uint32_t offset, bool 
 
 template <class T, int D, int DV, bool FAST>
 __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 64) ? 1 : 2) void pages_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks,
-                                                                                                  void *out, float *partial, int splits, int row_tiles)
+                                                                                                            void *out, float *partial, int32_t *spans, int slots,
+                                                                                                            int row_tiles)
 {
     constexpr int TR = ROWS, NK = D / KS<T, TR>, E = DV / 16;           // E: elements of a lane's values
     constexpr int PE = E < FE<T> ? E : FE<T>, PIECES = E / PE, WORDS = E * (int)sizeof(T) / 4, PW = PE * (int)sizeof(T) / 4;
@@ -115,9 +208,11 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
     constexpr bool AHEAD = FAST && !(sizeof(T) == 4 && DV > 128), EARLY = AHEAD && (sizeof(T) == 2 || D <= 64);
     __shared__ float joined[2][ROWS][DV + 4];
     __shared__ float tops[2][4][ROWS], sums[2][4][ROWS];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = a.B * a.Hkv;
-    const int bh = blockIdx.x % heads, rest_id = blockIdx.x / heads, tile = rest_id % row_tiles, split = rest_id / row_tiles;
-    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = blockIdx.x % a.Hkv, rest_id = blockIdx.x / a.Hkv, tile = rest_id / slots;
+    // the slot is the wave's: held a lane each it was kept elsewhere inside a branch of lanes, and came back for those lanes alone
+    const Share share = share_of(a, p, uniform(rest_id - tile * slots), slots, spans);
+    if (share.b < 0) return;            // a slot that no request has
+    const int b = share.b, split = share.part, splits = share.parts;
     const int length = uniform(length_of(p, b)), count = uniform(count_of(p, b, a.Lq)), room = p.slots * p.S;
     const int row = tile * ROWS + lane_row<TR>();
     const int query = row < a.R ? row / a.G : 0;
@@ -336,7 +431,7 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
 #pragma unroll
         for (int w = 0; w < 4; ++w) m_sum[m] += sums[m][w][mine] == 0.0f ? 0.0f : sums[m][w][mine] * __builtin_amdgcn_exp2f(tops[m][w][mine] - m_top[m]);
     }
-    if (splits == 1) {
+    if (!partial) {
         const int i = out_row / a.G, h = hk * a.G + out_row - i * a.G;
         const float lam = lambda_of(a, h, static_cast<const T *>(nullptr));
         const float inv[2] = {m_sum[0] > 0.0f ? 1.0f / m_sum[0] : 0.0f, m_sum[1] > 0.0f ? 1.0f / m_sum[1] : 0.0f};
@@ -348,7 +443,7 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
             store_pack<T, 4>(to + col, a.dv - col, r);
         }
     } else {
-        float *to = partial + (((int64_t)split * a.B * a.Hkv + bh) * a.R + out_row) * (2 * (int64_t)a.dv + 4);
+        float *to = partial + (((int64_t)share.slot * a.Hkv + hk) * a.R + out_row) * (2 * (int64_t)a.dv + 4);
         for (int m = 0; m < 2; ++m)
             for (int col = place; col < a.dv; col += 16) to[m * a.dv + col] = joined[m][mine][col];
         if (place < 2) {
@@ -390,12 +485,12 @@ struct Swizzled {
 typedef __attribute__((address_space(3))) void *lds_pointer;
 typedef const __attribute__((address_space(1))) void *global_pointer;
 
-constexpr int LDS_BYTES = 156 * 1024;
+constexpr int WAVES = 8, LDS_BYTES = 156 * 1024;
 template <class T, int D, int DV>
 constexpr int PAGE_TILE = KT * (2 * D + DV) * (int)sizeof(T);
 // Tiles of a part of the workgroup's keys: one in use, the others on their way.
 template <class T, int D, int DV, int RG>
-constexpr int RING = LDS_BYTES / (8 / RG * PAGE_TILE<T, D, DV>) < 4 ? LDS_BYTES / (8 / RG * PAGE_TILE<T, D, DV>) : 4;
+constexpr int RING = LDS_BYTES / (WAVES / RG * PAGE_TILE<T, D, DV>) < 4 ? LDS_BYTES / (WAVES / RG * PAGE_TILE<T, D, DV>) : 4;
 
 // Waits until at most N of the wave's loads are on their way and all of its reads of LDS are done, then for the other waves.
 template <int N>
@@ -415,7 +510,7 @@ __device__ __forceinline__ uint32_t lds_offset(const unsigned char *p)
 // Fragments of 16 columns each of 32 rows by the transposing read (column_frag): 16 lanes give the addresses of 4 rows x 16 columns and get a column's 4 rows each; the second read's rows
 // stand HIGH bytes on.  Four fragments and their wait in one block: before the builtin the compiler waits for every load from memory to LDS that is on its way.
 template <int HIGH, class F>
-__device__ __forceinline__ void columns_of(const uint32_t (&from)[4], F (&v)[4])
+__device__ __forceinline__ void columns_of(const uint32_t (&from)[4], F *v)
 {
     typedef uint32_t quad __attribute__((ext_vector_type(2)));
     typedef uint32_t octet __attribute__((ext_vector_type(4)));
@@ -439,68 +534,134 @@ __device__ __forceinline__ void columns_of(const uint32_t (&from)[4], F (&v)[4])
     }
 }
 
-// 32 keys of a tile: their scores, probabilities, and the products with their values.
+// A wave's running products and sums; exponentials are relative to `base`, the maximum in powers of two or 0 before there is one.
+template <int DV>
+struct Running {
+    Acc<ROWS> o[2][DV / ROWS];
+    float top[2], base[2], sum[2];
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            top[m] = -INFINITY;
+            base[m] = sum[m] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < DV / ROWS; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[m][b][i] = 0.0f;
+        }
+    }
+};
+
+// 32 keys of a tile: their scores, probabilities, and the products with their values.  The vector units are what bounds it (16 exponentials a lane), so nothing else is done for a tile that
+// need not be: whether a maximum rises is asked of both maps at once and of each lane's own scores; the rows' maxima are formed across lanes where one does.  Values are read behind the
+// products of the scores, which run meanwhile.
 template <bool LIMITED, class T, int D, int DV>
-__device__ __forceinline__ void page_keys(State<T, ROWS, D, DV, true> &state, const Frag<T> (&q)[2][D / KS<T, ROWS>], const unsigned char *tile, float c, int limit,
-                                          uint32_t word)
+__device__ __forceinline__ void page_keys(Running<DV> &state, const Frag<T> (&q)[2][D / KS<T, ROWS>], const unsigned char *tile, float c, int limit, uint32_t word)
 {
-    constexpr int TR = ROWS, NK = D / KS<T, TR>;
+    constexpr int TR = ROWS, NK = D / KS<T, TR>, BLK = DV / TR, WIDE = sizeof(T) == 2, FIRST = WIDE && BLK <= 8 ? BLK : 0;
     typedef Swizzled<T, 2 * D, false> KeyTile;
     typedef Swizzled<T, DV, true> ValueTile;
     const unsigned char *values = tile + KeyTile::BYTES;
     const int lane = threadIdx.x & 63, row = lane_row<TR>(), group = lane_group<TR>();
-    Frag<T> frag[2][FRAGS<T, TR>];
+    Acc<TR> s[2][BLOCKS<TR>];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        Acc<TR> s[BLOCKS<TR>];
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) s[blk][n] = 0.0f;
+            for (int n = 0; n < 4; ++n) s[m][blk][n] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
-                mma<TR>(*reinterpret_cast<const Frag<T> *>(KeyTile::piece(tile, blk * TR + row, m * (D / FE<T>) + kk * GROUPS<TR> + group)), q[m][kk], s[blk]);
+                mma<TR>(*reinterpret_cast<const Frag<T> *>(KeyTile::piece(tile, blk * TR + row, m * (D / FE<T>) + kk * GROUPS<TR> + group)), q[m][kk], s[m][blk]);
         }
-        float x[REGS<TR>];
-        state.template softmax<LIMITED, REGS<TR>>(m, s, c, limit, word, x);
-        to_frags<T, TR>(x, frag[m]);
-    }
-    if constexpr (sizeof(T) == 2) {
-        const int r = 4 * group + lane % 16 / 4, half = lane % 4 / 2;
-        const uint32_t at = lds_offset(values) + r * (DV * 2) + lane % 2 * 8;
+    // column fragments of 16-bit values
+    const int r = 4 * group + lane % 16 / 4, half = lane % 4 / 2;
+    const uint32_t at = lds_offset(values) + r * (DV * 2) + lane % 2 * 8;
+    const auto columns = [&](int blk, Frag<T> *v) __attribute__((always_inline)) {
+        uint32_t from[4];
 #pragma unroll
-        for (int blk = 0; blk < DV / TR; blk += 4) {
-            Frag<T> v[4];
-            uint32_t from[4];
+        for (int n = 0; n < 4; ++n) from[n] = at + ((2 * (blk + n) + half) ^ ValueTile::turn(r)) * 16;
+        columns_of<16 * DV * 2>(from, v);
+    };
+    Frag<T> v[FIRST ? FIRST : 1];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) from[n] = at + ((2 * (blk + n) + half) ^ ValueTile::turn(r)) * 16;
-            columns_of<16 * DV * 2>(from, v);
+    for (int blk = 0; blk < FIRST; blk += 4) columns(blk, v + blk);
+
+    float high[2];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                mma<TR>(v[n], frag[0][0], state.o[0][blk + n]);
-                mma<TR>(v[n], frag[1][0], state.o[1][blk + n]);
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int f = 0; f < REGS<TR>; ++f)
+            if constexpr (LIMITED) {
+                const int key = index_of<TR>(f);
+                s[m][f / 4][f % 4] = key < limit && (word >> key & 1) ? s[m][f / 4][f % 4] : -INFINITY;
             }
+        float x = s[m][0][0];
+#pragma unroll
+        for (int f = 1; f < REGS<TR>; ++f) x = fmaxf(x, s[m][f / 4][f % 4]);
+        high[m] = x * c;
+    }
+    if (__any(high[0] > state.top[0] + SLACK || high[1] > state.top[1] + SLACK)) {
+        asm volatile("; a new maximum");        // kept a branch
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float rise = fmaxf(state.top[m], groups_max<TR>(high[m])), factor = rise == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(state.top[m] - rise);
+            state.top[m] = rise;
+            state.base[m] = rise == -INFINITY ? 0.0f : rise;
+            state.sum[m] *= factor;
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) state.o[m][b][i] *= factor;
+        }
+    }
+    Frag<T> frag[2][FRAGS<T, TR>];
+    const auto exponentials = [&](int m) __attribute__((always_inline)) {
+        float x[REGS<TR>];
+#pragma unroll
+        for (int f = 0; f < REGS<TR>; ++f) x[f] = __builtin_amdgcn_exp2f(fmaf(s[m][f / 4][f % 4], c, -state.base[m]));
+        state.sum[m] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        to_frags<T, TR>(x, frag[m]);
+    };
+    exponentials(0);
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int blk = 0; blk < FIRST; ++blk) mma<TR>(v[blk], frag[0][0], state.o[0][blk]);
+        exponentials(1);
+#pragma unroll
+        for (int blk = 0; blk < FIRST; ++blk) mma<TR>(v[blk], frag[1][0], state.o[1][blk]);
+#pragma unroll
+        for (int blk = FIRST; blk < BLK; blk += 4) {
+            Frag<T> more[4];
+            columns(blk, more);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) mma<TR>(more[n], frag[m][0], state.o[m][blk + n]);
         }
     } else {
+        exponentials(1);
 #pragma unroll
-        for (int blk = 0; blk < DV / TR; ++blk)
+        for (int blk = 0; blk < BLK; ++blk)
 #pragma unroll
             for (int j = 0; j < FRAGS<T, TR>; ++j) {
-                Frag<T> v;
+                Frag<T> x;
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    v[u] = *reinterpret_cast<const float *>(ValueTile::piece(values, 16 * j + 4 * group + u, 4 * blk + lane % 16 / 4) + lane % 4 * 4);
-                mma<TR>(v, frag[0][j], state.o[0][blk]);
-                mma<TR>(v, frag[1][j], state.o[1][blk]);
+                    x[u] = *reinterpret_cast<const float *>(ValueTile::piece(values, 16 * j + 4 * group + u, 4 * blk + lane % 16 / 4) + lane % 4 * 4);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) mma<TR>(x, frag[m][j], state.o[m][blk]);
             }
     }
 }
 
 template <class T, int D, int DV, int RG>
-__global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks, void *out, float *partial,
-                                                            int splits, int row_tiles)
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void page_tiles_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks, void *out, float *partial,
+                                                                   int32_t *spans, int slots, int row_tiles)
 {
-    constexpr int TR = ROWS, PARTS = 8 / RG, NB = RING<T, D, DV, RG>, AHEAD = NB - 1, TILE = PAGE_TILE<T, D, DV>, AR = 4, ACC = DV / TR * AR, NK = D / KS<T, TR>;
+    constexpr int TR = ROWS, PARTS = WAVES / RG, NB = RING<T, D, DV, RG>, AHEAD = NB - 1, TILE = PAGE_TILE<T, D, DV>, AR = 4, ACC = DV / TR * AR, NK = D / KS<T, TR>;
     typedef Swizzled<T, 2 * D, false> KeyTile;
     typedef Swizzled<T, DV, true> ValueTile;
     constexpr int LOADS = (KeyTile::LOADS + ValueTile::LOADS + RG - 1) / RG;            // of a wave, for a tile
@@ -508,9 +669,11 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
     constexpr int TILES_AT = PARTS * NB * TILE, JOIN_AT = (PARTS - 1) * RG * 2 * 64 * ACC * 4;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[TILES_AT > JOIN_AT ? TILES_AT : JOIN_AT];
     __shared__ float tops[PARTS][2][RG][TR], sums[PARTS][2][RG][TR];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave / RG, group = wave % RG, lane = threadIdx.x & 63, heads = a.B * a.Hkv;
-    const int bh = blockIdx.x % heads, rest_id = blockIdx.x / heads, tile = row_tiles - 1 - rest_id % row_tiles, split = rest_id / row_tiles;
-    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave / RG, group = wave % RG, lane = threadIdx.x & 63;
+    const int hk = blockIdx.x % a.Hkv, rest_id = blockIdx.x / a.Hkv, turn = rest_id / slots, tile = row_tiles - 1 - turn;
+    const Share share = share_of(a, p, uniform(rest_id - turn * slots), slots, spans);
+    if (share.b < 0) return;            // a slot that no request has
+    const int b = share.b, split = share.part, splits = share.parts;
     const int length = uniform(length_of(p, b)), count = uniform(count_of(p, b, a.Lq)), room = p.slots * p.S;
     const int first = (tile * RG + group) * TR, row = first + lane_row<TR>();
     const int query = row < a.R ? row / a.G : 0;
@@ -536,68 +699,75 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
 #pragma unroll
     for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
     const float c = a.scale * LOG2E;
-    State<T, TR, D, DV, true> state;
+    Running<DV> state;
     state.clear();
     if (a.d < D || a.dv < DV) {
         typedef uint32_t words __attribute__((ext_vector_type(4)));
-        for (int i = threadIdx.x * 16; i < TILES_AT; i += 512 * 16) *reinterpret_cast<words *>(lds + i) = words{0, 0, 0, 0};
+        for (int i = threadIdx.x * 16; i < TILES_AT; i += WAVES * 64 * 16) *reinterpret_cast<words *>(lds + i) = words{0, 0, 0, 0};
         __syncthreads();
     }
 
     // A tile on its way.  Whole ones take every row as it is; of another one, rows past the last key are the last key's, and a half that is not there is the other one's rows.
     unsigned char *const ring = lds + part * NB * TILE;
-    Walk walk(p, b, hk, begin * KT);
-    uint32_t offset[LOADS];                     // of a lane's piece of a whole tile, in its half's rows
+    PageWalk walk(p, b, hk, begin * KT, (int)sizeof(T));
+    constexpr int ALL = KeyTile::LOADS + ValueTile::LOADS;
+    uint32_t offset[LOADS];                     // bytes from a half's rows to a lane's piece of a whole tile
     bool mine_there[LOADS];
-    const auto place = [&](int i, bool &value, int &second, int &r, int &column) __attribute__((always_inline)) {
-        const int n = (i * RG + group) % (KeyTile::LOADS + ValueTile::LOADS);           // a wave that has none left loads another one's again
-        value = n >= KeyTile::LOADS;
-        const int at = (value ? n - KeyTile::LOADS : n) * 1024, bytes = (value ? DV : 2 * D) * (int)sizeof(T);          // of a row of LDS
-        const int row_of_tile = (at + lane * 16) / bytes, spot = (at + lane * 16) % bytes / 16;
-        const int chunk = spot ^ (value ? ValueTile::turn(row_of_tile) : KeyTile::turn(row_of_tile));
+    const auto number_of = [&](int i) __attribute__((always_inline)) { return (i * RG + group) % ALL; };       // a wave that has none left loads another one's again
+    const auto is_value = [&](int i) __attribute__((always_inline)) { return KeyTile::LOADS % RG == 0 ? i >= KeyTile::LOADS / RG : number_of(i) >= KeyTile::LOADS; };
+    const auto second_of = [&](int i) __attribute__((always_inline)) {
+        const bool value = is_value(i);
+        return (value ? number_of(i) - KeyTile::LOADS : number_of(i)) >= (value ? ValueTile::LOADS : KeyTile::LOADS) / 2;
+    };
+    const auto place = [&](int i, int &r, int &column) __attribute__((always_inline)) {
+        const bool value = is_value(i);
+        const int at = (value ? number_of(i) - KeyTile::LOADS : number_of(i)) * 1024 + lane * 16, bytes = (value ? DV : 2 * D) * (int)sizeof(T);   // of a row of LDS
+        const int chunk = at % bytes / 16 ^ (value ? ValueTile::turn(at / bytes) : KeyTile::turn(at / bytes));
         const int map = value ? 0 : chunk / (D / FE<T>), col = (value ? chunk : chunk % (D / FE<T>)) * FE<T>;
-        second = at / bytes / 16;
-        r = row_of_tile & 15;
+        r = at / bytes & 15;
         column = map * a.d + col;
         return col < (value ? a.dv : a.d);
     };
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        bool value;
-        int second, r, column;
-        mine_there[i] = place(i, value, second, r, column);
-        offset[i] = (uint32_t)(r * (value ? a.dv : 2 * a.d) + column);
+        int r, column;
+        mine_there[i] = place(i, r, column);
+        offset[i] = (uint32_t)(r * (is_value(i) ? a.dv : 2 * a.d) + column) * (uint32_t)sizeof(T);
     }
     uint32_t ways = 0;                          // of the tiles from the one in use on, two bits each: which halves of them there are
     int from_ring = 0, to_ring = 0;             // where the tile in use and the next one to load stand
+    const auto fetch = [&](const unsigned char *base, uint32_t off, unsigned char *to) __attribute__((always_inline)) {
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00027000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_pointer)to, 16, (int)off, 0, 0, 0);
+    };
     const auto load = [&](int t, int ahead) __attribute__((always_inline)) {
-        const int64_t row0 = walk.next(), row1 = walk.next();
+        const unsigned char *k_first, *k_second, *v_first, *v_second;
+        const bool first_there = walk.next(k_first, v_first), second_there = walk.next(k_second, v_second);
         const int left = any - t * KT;          // keys of the tile
-        const uint32_t halves = (row0 < 0 ? 0u : 1u) | (row1 < 0 || left <= 16 ? 0u : 2u);
+        const uint32_t halves = (first_there ? 1u : 0u) | (second_there && left > 16 ? 2u : 0u);
         ways |= halves << 2 * ahead;
-        unsigned char *const to = ring + to_ring * TILE;
-        to_ring = to_ring + 1 < NB ? to_ring + 1 : 0;
+        unsigned char *const to = ring + to_ring;
+        to_ring = to_ring + TILE < NB * TILE ? to_ring + TILE : 0;
         if (halves == 3 && left >= KT) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int n = (i * RG + group) % (KeyTile::LOADS + ValueTile::LOADS);
-                const bool value = n >= KeyTile::LOADS;
-                const int second = (value ? n - KeyTile::LOADS : n) * 1024 / ((value ? DV : 2 * D) * (int)sizeof(T)) / 16;
-                const T *base = static_cast<const T *>(value ? p.v : p.k) + (second ? row1 : row0) * (value ? a.dv : 2 * a.d);
-                if (mine_there[i]) __builtin_amdgcn_global_load_lds((global_pointer)(base + offset[i]), (lds_pointer)(to + n * 1024), 16, 0, 0);
+                const unsigned char *base = is_value(i) ? second_of(i) ? v_second : v_first : second_of(i) ? k_second : k_first;
+                if (mine_there[i]) fetch(base, offset[i], to + number_of(i) * 1024);
             }
         } else {
-            const int64_t rows0 = halves & 1 ? row0 : halves ? row1 : 0, rows1 = halves & 2 ? row1 : rows0;
+            const unsigned char *k0 = static_cast<const unsigned char *>(p.k), *v0 = static_cast<const unsigned char *>(p.v), *k1, *v1;
+            if (halves) k0 = halves & 1 ? k_first : k_second, v0 = halves & 1 ? v_first : v_second;
+            k1 = halves & 2 ? k_second : k0;
+            v1 = halves & 2 ? v_second : v0;
             const int end0 = halves == 2 ? left - 16 : left, end1 = halves & 2 ? left - 16 : left;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                bool value;
-                int second, r, column;
-                const bool there_too = place(i, value, second, r, column);
-                const int n = (i * RG + group) % (KeyTile::LOADS + ValueTile::LOADS), end = second ? end1 : end0;
-                const T *base = static_cast<const T *>(value ? p.v : p.k) + (second ? rows1 : rows0) * (value ? a.dv : 2 * a.d);
-                const uint32_t off = (uint32_t)((r < end ? r : end - 1) * (value ? a.dv : 2 * a.d) + column);
-                if (there_too) __builtin_amdgcn_global_load_lds((global_pointer)(base + off), (lds_pointer)(to + n * 1024), 16, 0, 0);
+                int r, column;
+                const bool there_too = place(i, r, column);
+                const int end = second_of(i) ? end1 : end0;
+                const unsigned char *base = is_value(i) ? second_of(i) ? v1 : v0 : second_of(i) ? k1 : k0;
+                if (there_too)
+                    fetch(base, (uint32_t)((r < end ? r : end - 1) * (is_value(i) ? a.dv : 2 * a.d) + column) * (uint32_t)sizeof(T), to + number_of(i) * 1024);
             }
         }
     };
@@ -612,8 +782,8 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
         const uint32_t halves = ways & 3;
         ways >>= 2;
         if (i + AHEAD < number) load(begin + i + AHEAD, AHEAD - 1);         // where the last tile stood: every wave is past it
-        use((begin + i) * KT, halves, ring + from_ring * TILE);
-        from_ring = from_ring + 1 < NB ? from_ring + 1 : 0;
+        use((begin + i) * KT, halves, ring + from_ring);
+        from_ring = from_ring + TILE < NB * TILE ? from_ring + TILE : 0;
         ++i;
     };
     const int open = (wave_all < wave_any ? wave_all : wave_any) / KT - begin, seen = (wave_any + KT - 1) / KT - begin;
@@ -636,7 +806,7 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
     if constexpr (PARTS > 1) {
         __syncthreads();
         float *cells = reinterpret_cast<float *>(lds) + lane;
-        constexpr int WAVE = 2 * 64 * ACC;
+        constexpr int SIZE = 2 * 64 * ACC;
         if (part) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -645,7 +815,7 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
                     sums[part][m][group][lane_row<TR>()] = total[m];
                 }
 #pragma unroll
-                for (int n = 0; n < ACC; ++n) cells[((part - 1) * RG + group) * WAVE + (m * ACC + n) * 64] = state.o[m][n / AR][n % AR];
+                for (int n = 0; n < ACC; ++n) cells[((part - 1) * RG + group) * SIZE + (m * ACC + n) * 64] = state.o[m][n / AR][n % AR];
             }
         }
         __syncthreads();
@@ -660,7 +830,7 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
 #pragma unroll
                 for (int n = 0; n < ACC; ++n) {
                     const float x = total[m] == 0.0f ? 0.0f : state.o[m][n / AR][n % AR] * old;
-                    const float y = sum == 0.0f ? 0.0f : cells[((other - 1) * RG + group) * WAVE + (m * ACC + n) * 64] * more;
+                    const float y = sum == 0.0f ? 0.0f : cells[((other - 1) * RG + group) * SIZE + (m * ACC + n) * 64] * more;
                     state.o[m][n / AR][n % AR] = x + y;
                 }
                 total[m] = (total[m] == 0.0f ? 0.0f : total[m] * old) + (sum == 0.0f ? 0.0f : sum * more);
@@ -674,7 +844,7 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
                 for (int n = 0; n < ACC; ++n) state.o[m][n / AR][n % AR] = 0.0f;
     }
     if (row >= a.R) return;
-    if (splits == 1) {
+    if (!partial) {
         const int head = hk * a.G + row - query * a.G;
         const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
         float factor[2];
@@ -691,7 +861,7 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
             store_pack<T, 4>(to + col, a.dv - col, r);
         }
     } else {
-        float *to = partial + (((int64_t)split * a.B * a.Hkv + bh) * a.R + row) * (2 * (int64_t)a.dv + 4);
+        float *to = partial + (((int64_t)share.slot * a.Hkv + hk) * a.R + row) * (2 * (int64_t)a.dv + 4);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
@@ -711,44 +881,102 @@ __global__ __launch_bounds__(512, 2) void page_tiles_kernel(const Call a, const 
     }
 }
 
-// How a call runs: row groups of a workgroup's tiles (0: rows are streamed), workgroups that share a row's keys.
-struct Plan { int groups, splits; };
-
-// The fewest row groups whose rings have room, and registers for the widest heads (16 bits: 8 groups; fp32: none, 0).
-template <class T, int D, int DV>
-constexpr int FEWEST_GROUPS = DV > 128 ? sizeof(T) == 2 ? 8 : 0 : RING<T, D, DV, 2> >= 2 ? 2 : RING<T, D, DV, 4> >= 2 ? 4 : 8;
-
+// The slots' parts of a row, a wave a row, in the slots' order.
 template <class T>
-struct Fewest {
+__global__ __launch_bounds__(256) void join_pages_kernel(const Call a, void *out, const float *__restrict__ partial, const int32_t *__restrict__ spans)
+{
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (int64_t)a.B * a.Hkv * a.R) return;
+    const int lane = threadIdx.x & 63, row = (int)(id % a.R), bh = (int)(id / a.R), b = bh / a.Hkv, hk = bh - b * a.Hkv;
+    const int query = row / a.G, head = hk * a.G + row - query * a.G;
+    const int first = uniform(spans[2 * b]), parts = uniform(spans[2 * b + 1]);
+    const int64_t size = 2 * (int64_t)a.dv + 4, step = (int64_t)a.Hkv * a.R * size;
+    const float *p = partial + (((int64_t)first * a.Hkv + hk) * a.R + row) * size;
+    // lane s holds part s's maxima and sums (parts <= 64)
+    float factor[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        float top = -INFINITY, sum = 0.0f;
+        if (lane < parts) {
+            top = p[lane * step + 2 * a.dv + 2 * m];
+            sum = p[lane * step + 2 * a.dv + 2 * m + 1];
+        }
+        float most = top;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) most = fmaxf(most, __shfl_xor(most, x));
+        const float mine = most == -INFINITY ? sum == 0.0f ? 0.0f : 1.0f : __builtin_amdgcn_exp2f(top - most);
+        float total = sum == 0.0f ? 0.0f : sum * mine;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
+        factor[m] = total != 0.0f ? sum == 0.0f ? 0.0f : mine / total : 0.0f;
+    }
+    const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
+    const int left = a.dv - 4 * lane;
+    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int AHEAD = 8;            // parts on their way at once
+    for (int s0 = 0; s0 < parts; s0 += AHEAD) {         // every lane stays to the end: each has a part's factors
+        float p1[AHEAD][4], p2[AHEAD][4];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const float *t = p + (s0 + u < parts ? s0 + u : parts - 1) * step + 4 * lane;
+            load_pack<float, 4>(t, left, p1[u]);
+            load_pack<float, 4>(t + a.dv, left, p2[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int s = s0 + u;
+            const float f0 = s < parts ? __shfl(factor[0], s) : 0.0f, f1 = s < parts ? -lam * __shfl(factor[1], s) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = fmaf(f1, p2[u][e], fmaf(f0, p1[u][e], r[e]));
+        }
+    }
+    if (left > 0) store_pack<T, 4>(static_cast<T *>(out) + (((int64_t)b * a.Lq + query) * a.H + head) * a.dv + 4 * lane, left, r);
+}
+
+// Row groups of a workgroup's tiles for `rows` rows of a key head, as few as hold them and as the ring leaves room for; 0: rows are streamed.  The widest heads have no registers for more
+// than one part (16 bits) and for any (fp32).
+template <class T, int D, int DV>
+constexpr bool FITS(int groups)
+{
+    if (DV > 128) return sizeof(T) == 2 && groups == 8;
+    return (groups == 2 ? RING<T, D, DV, 2> : groups == 4 ? RING<T, D, DV, 4> : RING<T, D, DV, 8>) >= 2;
+}
+template <class T>
+struct GroupsOf {
+    int rows;
     template <int D, int DV>
-    int operator()() const { return FEWEST_GROUPS<T, D, DV>; }
+    int operator()() const
+    {
+        if (rows <= 2 * ROWS && FITS<T, D, DV>(2)) return 2;
+        if (rows <= 4 * ROWS && FITS<T, D, DV>(4)) return 4;
+        return FITS<T, D, DV>(8) ? 8 : 0;
+    }
 };
 
-// Tiles where a key head has more rows than a wave streams: as few row groups as hold them and as the ring's tiles leave room for.  Heads that end inside 16 bytes are streamed.
-inline int row_groups(const Call &a, const Pages &p, int type)
+// How a call runs: row groups, and slots: workgroups that share the keys of a key head's tile of rows over all requests.
+struct Plan {
+    int groups, slots;
+    int64_t row_tiles;
+};
+Plan plan_of(const Call &a, const Pages &p, int type)
 {
-    if (a.R <= FEW || !a.fast || p.P == 0) return 0;
-    const int fewest = type == MAM_F32 ? with_head_sizes(a.d, a.dv, Fewest<float>()) : with_head_sizes(a.d, a.dv, Fewest<bf16>());
-    const int want = a.R <= 2 * ROWS ? 2 : a.R <= 4 * ROWS ? 4 : 8;
-    return fewest == 0 ? 0 : want < fewest ? fewest : want;
+    Plan plan{};
+    if (a.R > FEW && a.fast && p.P > 0)         // heads that end inside 16 bytes are streamed
+        plan.groups = type == MAM_F32 ? with_head_sizes(a.d, a.dv, GroupsOf<float>{a.R}) : with_head_sizes(a.d, a.dv, GroupsOf<bf16>{a.R});
+    plan.row_tiles = ceil_div(a.R, plan.groups ? plan.groups * ROWS : ROWS);
+    // two workgroups of four waves a CU, or one of eight; a request's part is at least as long as the waves have tiles to begin with
+    const int64_t rows = a.Hkv * plan.row_tiles, want = (plan.groups ? 1 : 2) * kNumCU / (rows > 0 ? rows : 1), most = ceil_div(a.Lk, LEAST_TILES * KT) * a.B;
+    int64_t n = want < most ? want : most;
+    if (n > 64 * (int64_t)a.B) n = 64 * (int64_t)a.B;
+    plan.slots = n > a.B ? (int)n : a.B;
+    return plan;
 }
+inline bool parted(const Call &a, const Plan &plan) { return plan.slots > a.B; }
 
-// Workgroups that share a row's keys: two a CU over the whole call, but 64 keys a wave at least of what a request has room for; of the tiles' eight waves one a CU.
-inline Plan plan_of(const Call &a, const Pages &pages, int type)
+// Partial rows of every slot, and each request's first slot and their number.
+size_t pages_workspace(const Call &a, const Plan &plan)
 {
-    Plan p{row_groups(a, pages, type), 1};
-    const int64_t rows = (int64_t)a.B * a.Hkv * ceil_div(a.R, p.groups ? p.groups * ROWS : ROWS), most = ceil_div(a.Lk, 4 * 64);
-    int64_t n = p.groups ? kNumCU / (rows > 0 ? rows : 1) : ceil_div(2 * (int64_t)kNumCU, rows);
-    if (n > 64) n = 64;
-    if (n > most) n = most;
-    p.splits = n < 1 ? 1 : (int)n;
-    return p;
-}
-
-inline size_t pages_workspace(const Call &a, const Pages &p, int type)
-{
-    const int n = plan_of(a, p, type).splits;
-    return n > 1 ? (size_t)n * a.B * a.Hkv * a.R * partial_size(a) * sizeof(float) : 0;
+    return parted(a, plan) ? (size_t)plan.slots * a.Hkv * a.R * partial_size(a) * sizeof(float) + 2 * (size_t)a.B * sizeof(int32_t) : 0;
 }
 
 template <class T>
@@ -757,28 +985,31 @@ struct PagesRun {
     const Pages &p;
     const int64_t *masks;
     void *out;
-    float *partial;
     Plan plan;
+    float *partial;
+    int32_t *spans;
     hipStream_t st;
     template <int D, int DV, int RG>
-    int tiles(dim3 grid, int row_tiles) const
+    void tiles(dim3 grid) const
     {
-        if constexpr (FEWEST_GROUPS<T, D, DV> > 0 && RG >= FEWEST_GROUPS<T, D, DV>)
-            hipLaunchKernelGGL((page_tiles_kernel<T, D, DV, RG>), grid, dim3(512), 0, st, a, p, masks, out, partial, plan.splits, row_tiles);
-        return check_launch("attention::page_tiles_kernel");
+        if constexpr (FITS<T, D, DV>(RG))
+            hipLaunchKernelGGL((page_tiles_kernel<T, D, DV, RG>), grid, dim3(WAVES * 64), 0, st, a, p, masks, out, partial, spans, plan.slots, (int)plan.row_tiles);
     }
     template <int D, int DV>
     int operator()() const
     {
-        const int64_t row_tiles = ceil_div(a.R, plan.groups ? plan.groups * ROWS : ROWS), blocks = row_tiles * a.B * a.Hkv * plan.splits;
+        const int64_t blocks = plan.row_tiles * a.Hkv * plan.slots;
         if (blocks > INT32_MAX) return fail(MAM_ERR_UNSUPPORTED, "too many tiles");
         const dim3 grid((unsigned)blocks);
-        if (plan.groups == 8) return tiles<D, DV, 8>(grid, (int)row_tiles);
-        if (plan.groups == 4) return tiles<D, DV, 4>(grid, (int)row_tiles);
-        if (plan.groups == 2) return tiles<D, DV, 2>(grid, (int)row_tiles);
-        if (a.fast) hipLaunchKernelGGL((pages_kernel<T, D, DV, true>), grid, dim3(256), 0, st, a, p, masks, out, partial, plan.splits, (int)row_tiles);
-        else hipLaunchKernelGGL((pages_kernel<T, D, DV, false>), grid, dim3(256), 0, st, a, p, masks, out, partial, plan.splits, (int)row_tiles);
-        return check_launch("attention::pages_kernel");
+        if (plan.groups == 8) tiles<D, DV, 8>(grid);
+        else if (plan.groups == 4) tiles<D, DV, 4>(grid);
+        else if (plan.groups == 2) tiles<D, DV, 2>(grid);
+        else if (a.fast) hipLaunchKernelGGL((pages_kernel<T, D, DV, true>), grid, dim3(256), 0, st, a, p, masks, out, partial, spans, plan.slots, (int)plan.row_tiles);
+        else hipLaunchKernelGGL((pages_kernel<T, D, DV, false>), grid, dim3(256), 0, st, a, p, masks, out, partial, spans, plan.slots, (int)plan.row_tiles);
+        int rc = check_launch("attention over pages");
+        if (rc != MAM_OK || !partial) return rc;
+        hipLaunchKernelGGL((join_pages_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.B * a.Hkv * a.R, 4)), dim3(256), 0, st, a, out, partial, spans);
+        return check_launch("attention::join_pages_kernel");
     }
 };
 
@@ -804,6 +1035,7 @@ int fill_pages_call(const mam_diff_attention_pages_t *x, Call &c, Pages &p)
     return MAM_OK;
 }
 
+}  // namespace
 }  // namespace attention
 }  // namespace mam
 
@@ -813,7 +1045,7 @@ extern "C" size_t mam_diff_attention_pages_workspace(const mam_diff_attention_pa
     attention::Call a;
     Pages p;
     if (attention::fill_pages_call(args, a, p) != MAM_OK || a.B == 0 || a.R == 0) return 0;
-    return attention::pages_workspace(a, p, args->pages.type);
+    return attention::pages_workspace(a, attention::plan_of(a, p, args->pages.type));
 }
 
 extern "C" int mam_diff_attention_pages(const mam_diff_attention_pages_t *args, void *out, void *workspace, size_t workspace_bytes, void *stream)
@@ -824,15 +1056,14 @@ extern "C" int mam_diff_attention_pages(const mam_diff_attention_pages_t *args, 
     int rc = attention::fill_pages_call(args, a, p);
     if (rc != MAM_OK || a.B == 0 || a.R == 0) return rc;
     if (!a.q || !a.lam || !out || (p.P > 0 && (!p.k || !p.v))) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
-    const size_t need = attention::pages_workspace(a, p, args->pages.type);
+    const attention::Plan plan = attention::plan_of(a, p, args->pages.type);
+    const size_t need = attention::pages_workspace(a, plan);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(MAM_ERR_WORKSPACE, "the attention needs %zu workspace bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);
     hipStream_t st = static_cast<hipStream_t>(stream);
     float *partial = need > 0 ? static_cast<float *>(workspace) : nullptr;
-    const attention::Plan plan = attention::plan_of(a, p, args->pages.type);
-    if (args->pages.type == MAM_F32) rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<float>{a, p, args->masks, out, partial, plan, st});
-    else if (args->pages.type == MAM_BF16) rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<bf16>{a, p, args->masks, out, partial, plan, st});
-    else rc = attention::with_head_sizes(a.d, a.dv, attention::PagesRun<f16>{a, p, args->masks, out, partial, plan, st});
-    if (rc != MAM_OK || need == 0) return rc;
-    return attention::join_parts(a, args->pages.type, out, partial, plan.splits, st);
+    int32_t *spans = need > 0 ? reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + need) - 2 * (int64_t)a.B : nullptr;
+    if (args->pages.type == MAM_F32) return attention::with_head_sizes(a.d, a.dv, attention::PagesRun<float>{a, p, args->masks, out, plan, partial, spans, st});
+    if (args->pages.type == MAM_BF16) return attention::with_head_sizes(a.d, a.dv, attention::PagesRun<bf16>{a, p, args->masks, out, plan, partial, spans, st});
+    return attention::with_head_sizes(a.d, a.dv, attention::PagesRun<f16>{a, p, args->masks, out, plan, partial, spans, st});
 }

@@ -40,6 +40,9 @@ bool use_split(const Call &a, int type, bool keep)
     return a.R <= ROWS || (a.Lk >= 512 && tiles <= (type == MAM_F32 || (a.d <= 64 && a.dv <= 128) ? 2 : 1) * kNumCU);
 }
 
+// A partial row: both maps' products relative to their maxima, then maximum and sum of each.
+inline int64_t partial_size(const Call &a) { return 2 * (int64_t)a.dv + 4; }
+
 size_t split_workspace(const Call &a)
 {
     const int n = split_count(a);
@@ -364,13 +367,6 @@ __global__ __launch_bounds__(256) void join_kernel(const Call a, void *out, cons
 }
 
 template <class T>
-int launch_join(const Call &a, void *out, const float *partial, int splits, hipStream_t st)
-{
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.B * a.Hkv * a.R, 4)), dim3(256), 0, st, a, out, partial, splits);
-    return check_launch("attention::join_kernel");
-}
-
-template <class T>
 struct Split {
     const Call &a;
     void *out;
@@ -387,16 +383,10 @@ struct Split {
         else hipLaunchKernelGGL((split_kernel<T, D, DV, false>), grid, dim3(256), 0, st, a, out, partial, splits, (int)row_tiles);
         int rc = check_launch("attention::split_kernel");
         if (rc != MAM_OK || splits == 1) return rc;
-        return launch_join<T>(a, out, partial, splits, st);
+        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.B * a.Hkv * a.R, 4)), dim3(256), 0, st, a, out, partial, splits);
+        return check_launch("attention::join_kernel");
     }
 };
-
-int join_parts(const Call &a, int type, void *out, const float *partial, int splits, hipStream_t st)
-{
-    if (type == MAM_F32) return launch_join<float>(a, out, partial, splits, st);
-    if (type == MAM_BF16) return launch_join<bf16>(a, out, partial, splits, st);
-    return launch_join<f16>(a, out, partial, splits, st);
-}
 
 int run_split(const Call &a, int type, void *out, void *workspace, size_t workspace_bytes, hipStream_t st)
 {
