@@ -22,6 +22,23 @@ constexpr int FEW = 16;                 // rows of a key head that are streamed
 // A value that all lanes share, where the compiler does not see it: loops over it are branches of the wave, not of lanes.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Quotients of whole numbers below 2^31 by one that the host knows: a multiplication, where a division is 25 instructions in the way of the first load.
+struct Divider {
+    uint32_t factor;
+    int shift;
+
+    explicit Divider(int64_t d) : shift(0)
+    {
+        while (((int64_t)1 << shift) < d) ++shift;
+        factor = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);       // too large by less than 1, so that a quotient is by less than n / 2^(31 + shift) < 1 / d
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)(__umulhi((uint32_t)n << 1, factor) >> shift); }
+};
+struct Grid {
+    int slots, row_tiles;
+    Divider heads, group, page;         // of Hkv, of G, of the steps of 16 tokens of a page
+};
+
 // A request's table, walked in steps of 16 tokens.
 struct Walk {
     const int32_t *row;
@@ -58,42 +75,23 @@ struct Walk {
     }
 };
 
-// The same as pointers to a key head's rows: a page's are found once, and 16 tokens on they are a step on.
-struct PageWalk {
-    Walk walk;
-    const unsigned char *k_pages, *v_pages, *k, *v;
-    int64_t k_row, v_row;               // bytes
-    int left;                           // tokens of the page from the pointers on
-    bool there;
+// 64 steps of 16 tokens from `first` on, one a lane: which step of the pages each is, and those that there are, and that are below `end` tokens as a whole.
+struct Steps {
+    const int32_t *row;
+    int slots, P, per, heads, head;
+    int first, at;
+    uint64_t there, whole;
 
-    __device__ __forceinline__ PageWalk(const Pages &p, int b, int head, int key, int size)
-        : walk(p, b, head, key), k_pages(static_cast<const unsigned char *>(p.k)), v_pages(static_cast<const unsigned char *>(p.v)), k_row(2 * p.d * size), v_row(p.dv * size)
+    __device__ __forceinline__ Steps(const Pages &p, int b, int head) : row(p.table + (int64_t)b * p.slots), slots(p.slots), P(p.P), per(p.S / 16), heads(p.Hkv), head(head) {}
+    __device__ __forceinline__ void read(int from, int end, const Divider &page)
     {
-        find();
-    }
-    __device__ __forceinline__ void find()
-    {
-        left = walk.S - walk.off;
-        const int64_t row = walk.next();
-        there = row >= 0;
-        k = k_pages + (there ? row : 0) * k_row;
-        v = v_pages + (there ? row : 0) * v_row;
-    }
-    __device__ __forceinline__ bool next(const unsigned char *&k_rows, const unsigned char *&v_rows)
-    {
-        const bool was = there;
-        k_rows = k;
-        v_rows = v;
-        left -= 16;
-        if (left == 0) {
-            walk.slot += walk.off > 0;          // the walk has looked at the page's first tokens alone
-            walk.off = 0;
-            find();
-        } else {
-            k += 16 * k_row;
-            v += 16 * v_row;
-        }
-        return was;
+        first = from;
+        const int step = from + (threadIdx.x & 63), slot = page(step), id = slot < slots ? row[slot] : -1;
+        const bool ok = id >= 0 && id < P;
+        at = ok ? (id * heads + head) * per + step - slot * per : 0;
+        there = __ballot(ok);
+        whole = __ballot(ok && (step + 1) * 16 <= end);
+        asm volatile("" : "+v"(at));        // waited for here: behind the branch around this call every use would wait for all loads on their way
     }
 };
 
@@ -110,15 +108,17 @@ __device__ __forceinline__ uint32_t seen_word(int key, int length, uint64_t mask
 // A workgroup's share of a call: a request, and which part of its keys.  The slots go to the requests by their lengths: one each, the others in proportion, as far as a part keeps
 // LEAST_TILES tiles.  Every wave works them out for itself from the lengths, a request a lane.
 constexpr int LEAST_TILES = 8;
-struct Share { int b, part, parts, slot; };
+struct Share { int b, part, parts, slot, length, count; };
 
 __device__ __forceinline__ Share share_of(const Call &a, const Pages &p, int slot, int slots, int32_t *spans)
 {
-    if (slots == a.B) return {slot, 0, 1, slot};
+    if (slots == a.B) return {slot, 0, 1, slot, uniform(length_of(p, slot)), uniform(count_of(p, slot, a.Lq))};
     const int lane = threadIdx.x & 63, width = a.B < 64 ? a.B : 64;        // lanes that have requests
+    int length = 0, count = 0;
     const auto tiles_of = [&](int b) {
-        if (b >= a.B) return 0;
-        const int count = count_of(p, b, a.Lq), most = p.slots * p.S, n = length_of(p, b) + count;
+        length = b < a.B ? length_of(p, b) : 0;
+        count = b < a.B ? count_of(p, b, a.Lq) : 0;
+        const int most = p.slots * p.S, n = length + count;
         return count == 0 ? 0 : ((n < most ? n : most) + KT - 1) / KT;
     };
     float all = 0.0f;
@@ -128,7 +128,7 @@ __device__ __forceinline__ Share share_of(const Call &a, const Pages &p, int slo
     // a little less than the proportion, so that rounding gives out no slot too many
     const float each = all > 0.0f ? (float)(slots - a.B) / all * (1.0f - 0x1p-18f) : 0.0f;
     int before = 0;
-    Share s{-1, 0, 0, slot};
+    Share s{-1, 0, 0, slot, 0, 0};
     for (int b = lane; b - lane < a.B; b += 64) {
         const int tiles = tiles_of(b), most = tiles / LEAST_TILES < 64 ? tiles / LEAST_TILES : 64;
         int n = 1 + (int)((float)tiles * each);
@@ -146,12 +146,16 @@ __device__ __forceinline__ Share share_of(const Call &a, const Pages &p, int slo
             s.b = uniform(b - lane + l);
             s.parts = uniform(__shfl(n, l));
             s.part = uniform(slot - (__shfl(until, l) - s.parts));
+            s.length = uniform(__shfl(length, l));
+            s.count = uniform(__shfl(count, l));
         }
         before = __shfl(until, 63);
     }
     s.b = uniform(s.b);
     s.part = uniform(s.part);
     s.parts = uniform(s.parts);
+    s.length = uniform(s.length);
+    s.count = uniform(s.count);
     if (s.b >= 0 && s.part == 0 && threadIdx.x == 0) {
         spans[2 * s.b] = slot;
         spans[2 * s.b + 1] = s.parts;
@@ -196,8 +200,7 @@ __device__ __forceinline__ void page_piece(const T *base, uint32_t offset, bool 
 
 template <class T, int D, int DV, bool FAST>
 __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 64) ? 1 : 2) void pages_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks,
-                                                                                                            void *out, float *partial, int32_t *spans, int slots,
-                                                                                                            int row_tiles)
+                                                                                                            void *out, float *partial, int32_t *spans, Grid grid)
 {
     constexpr int TR = ROWS, NK = D / KS<T, TR>, E = DV / 16;           // E: elements of a lane's values
     constexpr int PE = E < FE<T> ? E : FE<T>, PIECES = E / PE, WORDS = E * (int)sizeof(T) / 4, PW = PE * (int)sizeof(T) / 4;
@@ -208,21 +211,21 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
     constexpr bool AHEAD = FAST && !(sizeof(T) == 4 && DV > 128), EARLY = AHEAD && (sizeof(T) == 2 || D <= 64);
     __shared__ float joined[2][ROWS][DV + 4];
     __shared__ float tops[2][4][ROWS], sums[2][4][ROWS];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = blockIdx.x % a.Hkv, rest_id = blockIdx.x / a.Hkv, tile = rest_id / slots;
-    // the slot is the wave's: held a lane each it was kept elsewhere inside a branch of lanes, and came back for those lanes alone
-    const Share share = share_of(a, p, uniform(rest_id - tile * slots), slots, spans);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = uniform(grid.heads(blockIdx.x)), hk = blockIdx.x - slot * a.Hkv, tile = blockIdx.y;
+    // (the slot is the wave's: held a lane each it was kept elsewhere inside a branch of lanes, and came back for those lanes alone)
+    const Share share = share_of(a, p, slot, grid.slots, spans);
     if (share.b < 0) return;            // a slot that no request has
     const int b = share.b, split = share.part, splits = share.parts;
-    const int length = uniform(length_of(p, b)), count = uniform(count_of(p, b, a.Lq)), room = p.slots * p.S;
+    const int length = share.length, count = share.count, room = p.slots * p.S;
     const int row = tile * ROWS + lane_row<TR>();
-    const int query = row < a.R ? row / a.G : 0;
+    const int query = row < a.R ? grid.group(row) : 0;
     const bool there = row < a.R && query < count;
     const uint64_t mask = masks && there ? (uint64_t)masks[(int64_t)b * a.Lq + query] : 0;
     const int limit = there ? length + (masks ? count : query + 1) : 0;
-    const int last_row = tile * ROWS + ROWS - 1 < a.R ? tile * ROWS + ROWS - 1 : a.R - 1, last = last_row / a.G;
+    const int last_row = tile * ROWS + ROWS - 1 < a.R ? tile * ROWS + ROWS - 1 : a.R - 1, last = grid.group(last_row);
     int any = length + (masks || last + 1 > count ? count : last + 1);
     if (any > room) any = room;
-    if (tile * ROWS / a.G >= count) any = 0;
+    if (grid.group(tile * ROWS) >= count) any = 0;
     // this wave's keys: whole tiles of 32, as even as they come
     const int per = ((any + 31) / 32 + 4 * splits - 1) / (4 * splits) * 32;
     const int64_t begin64 = (int64_t)per * (split * 4 + wave);
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
         for (int w = 0; w < 4; ++w) m_sum[m] += sums[m][w][mine] == 0.0f ? 0.0f : sums[m][w][mine] * __builtin_amdgcn_exp2f(tops[m][w][mine] - m_top[m]);
     }
     if (!partial) {
-        const int i = out_row / a.G, h = hk * a.G + out_row - i * a.G;
+        const int i = grid.group(out_row), h = hk * a.G + out_row - i * a.G;
         const float lam = lambda_of(a, h, static_cast<const T *>(nullptr));
         const float inv[2] = {m_sum[0] > 0.0f ? 1.0f / m_sum[0] : 0.0f, m_sum[1] > 0.0f ? 1.0f / m_sum[1] : 0.0f};
         T *to = static_cast<T *>(out) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv;
@@ -569,13 +572,15 @@ __device__ __forceinline__ void page_keys(Running<DV> &state, const Frag<T> (&q)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int blk = 0; blk < BLOCKS<TR>; ++blk) {
+        for (int blk = 0; blk < BLOCKS<TR>; ++blk)
 #pragma unroll
             for (int n = 0; n < 4; ++n) s[m][blk][n] = 0.0f;
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk)
-                mma<TR>(*reinterpret_cast<const Frag<T> *>(KeyTile::piece(tile, blk * TR + row, m * (D / FE<T>) + kk * GROUPS<TR> + group)), q[m][kk], s[m][blk]);
-        }
+    for (int n = 0; n < 2 * BLOCKS<TR> * NK; ++n) {
+        // sums that do not wait for each other in turn; one after the other where there are no registers for their keys
+        const int sum = DV > 128 ? n / NK : n % (2 * BLOCKS<TR>), kk = DV > 128 ? n % NK : n / (2 * BLOCKS<TR>), m = sum / BLOCKS<TR>, blk = sum % BLOCKS<TR>;
+        mma<TR>(*reinterpret_cast<const Frag<T> *>(KeyTile::piece(tile, blk * TR + row, m * (D / FE<T>) + kk * GROUPS<TR> + group)), q[m][kk], s[m][blk]);
+    }
     // column fragments of 16-bit values
     const int r = 4 * group + lane % 16 / 4, half = lane % 4 / 2;
     const uint32_t at = lds_offset(values) + r * (DV * 2) + lane % 2 * 8;
@@ -659,7 +664,7 @@ __device__ __forceinline__ void page_keys(Running<DV> &state, const Frag<T> (&q)
 
 template <class T, int D, int DV, int RG>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void page_tiles_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks, void *out, float *partial,
-                                                                   int32_t *spans, int slots, int row_tiles)
+                                                                   int32_t *spans, Grid grid)
 {
     constexpr int TR = ROWS, PARTS = WAVES / RG, NB = RING<T, D, DV, RG>, AHEAD = NB - 1, TILE = PAGE_TILE<T, D, DV>, AR = 4, ACC = DV / TR * AR, NK = D / KS<T, TR>;
     typedef Swizzled<T, 2 * D, false> KeyTile;
@@ -670,25 +675,25 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
     __shared__ __attribute__((aligned(1024))) unsigned char lds[TILES_AT > JOIN_AT ? TILES_AT : JOIN_AT];
     __shared__ float tops[PARTS][2][RG][TR], sums[PARTS][2][RG][TR];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave / RG, group = wave % RG, lane = threadIdx.x & 63;
-    const int hk = blockIdx.x % a.Hkv, rest_id = blockIdx.x / a.Hkv, turn = rest_id / slots, tile = row_tiles - 1 - turn;
-    const Share share = share_of(a, p, uniform(rest_id - turn * slots), slots, spans);
+    const int slot = uniform(grid.heads(blockIdx.x)), hk = blockIdx.x - slot * a.Hkv, tile = grid.row_tiles - 1 - blockIdx.y;
+    const Share share = share_of(a, p, slot, grid.slots, spans);
     if (share.b < 0) return;            // a slot that no request has
     const int b = share.b, split = share.part, splits = share.parts;
-    const int length = uniform(length_of(p, b)), count = uniform(count_of(p, b, a.Lq)), room = p.slots * p.S;
+    const int length = share.length, count = share.count, room = p.slots * p.S;
     const int first = (tile * RG + group) * TR, row = first + lane_row<TR>();
-    const int query = row < a.R ? row / a.G : 0;
+    const int query = row < a.R ? grid.group(row) : 0;
     const bool there = row < a.R && query < count;
     const uint64_t mask = masks && there ? (uint64_t)masks[(int64_t)b * a.Lq + query] : 0;
     const int limit = there ? length + (masks ? count : query + 1) : 0;
     // keys that rows from .. last see at most: none where the first of them is no query
     const auto reach = [&](int from, int last) {
-        const int q = (last < a.R ? last : a.R - 1) / a.G;
+        const int q = grid.group(last < a.R ? last : a.R - 1);
         const int n = length + (masks || q + 1 > count ? count : q + 1);
-        return from >= a.R || from / a.G >= count ? 0 : n < room ? n : room;
+        return from >= a.R || grid.group(from) >= count ? 0 : n < room ? n : room;
     };
     const int wave_any = reach(first, first + TR - 1), any = reach(tile * RG * TR, (tile + 1) * RG * TR - 1);
     // and those that every row of the wave sees (rows that are none see what they like)
-    const int wave_all = masks || wave_any == 0 ? length : length + first / a.G + 1;
+    const int wave_all = masks || wave_any == 0 ? length : length + grid.group(first) + 1;
     // the workgroup's tiles, and this part's; parts differ by one tile at most, the first ones having more
     const int tiles = (any + KT - 1) / KT, per = (tiles + splits - 1) / splits, from = split * per < tiles ? split * per : tiles;
     const int mine = from + per < tiles ? per : tiles - from, most = (mine + PARTS - 1) / PARTS;
@@ -698,6 +703,18 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
     Frag<T> q[2][NK];
 #pragma unroll
     for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
+    Steps steps(p, b, hk);
+    steps.read(2 * begin, any, grid.page);
+    // the queries come with the table: waited for in the loop they would have every tile waited for
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            typedef uint32_t words __attribute__((ext_vector_type(4)));
+            words w = __builtin_bit_cast(words, q[m][kk]);
+            asm volatile("" : "+v"(w));
+            q[m][kk] = __builtin_bit_cast(Frag<T>, w);
+        }
     const float c = a.scale * LOG2E;
     Running<DV> state;
     state.clear();
@@ -707,9 +724,10 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
         __syncthreads();
     }
 
-    // A tile on its way.  Whole ones take every row as it is; of another one, rows past the last key are the last key's, and a half that is not there is the other one's rows.
+    // A tile on its way.
     unsigned char *const ring = lds + part * NB * TILE;
-    PageWalk walk(p, b, hk, begin * KT, (int)sizeof(T));
+    const unsigned char *const keys = static_cast<const unsigned char *>(p.k), *const values = static_cast<const unsigned char *>(p.v);
+    const uint32_t key_step = 16 * 2 * (uint32_t)(a.d * (int)sizeof(T)), value_step = 16 * (uint32_t)(a.dv * (int)sizeof(T));
     constexpr int ALL = KeyTile::LOADS + ValueTile::LOADS;
     uint32_t offset[LOADS];                     // bytes from a half's rows to a lane's piece of a whole tile
     bool mine_there[LOADS];
@@ -719,7 +737,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
         const bool value = is_value(i);
         return (value ? number_of(i) - KeyTile::LOADS : number_of(i)) >= (value ? ValueTile::LOADS : KeyTile::LOADS) / 2;
     };
-    const auto place = [&](int i, int &r, int &column) __attribute__((always_inline)) {
+    const auto place = [&](int i, int lane, int &r, int &column) __attribute__((always_inline)) {
         const bool value = is_value(i);
         const int at = (value ? number_of(i) - KeyTile::LOADS : number_of(i)) * 1024 + lane * 16, bytes = (value ? DV : 2 * D) * (int)sizeof(T);   // of a row of LDS
         const int chunk = at % bytes / 16 ^ (value ? ValueTile::turn(at / bytes) : KeyTile::turn(at / bytes));
@@ -731,7 +749,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         int r, column;
-        mine_there[i] = place(i, r, column);
+        mine_there[i] = place(i, lane, r, column);
         offset[i] = (uint32_t)(r * (is_value(i) ? a.dv : 2 * a.d) + column) * (uint32_t)sizeof(T);
     }
     uint32_t ways = 0;                          // of the tiles from the one in use on, two bits each: which halves of them there are
@@ -741,44 +759,46 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_pointer)to, 16, (int)off, 0, 0, 0);
     };
     const auto load = [&](int t, int ahead) __attribute__((always_inline)) {
-        const unsigned char *k_first, *k_second, *v_first, *v_second;
-        const bool first_there = walk.next(k_first, v_first), second_there = walk.next(k_second, v_second);
+        int j = 2 * t - steps.first;
+        if (j >= 64) {
+            steps.read(2 * t, any, grid.page);
+            j = 0;
+        }
+        // Whole tiles take every row as it is; of another one, rows past the last key are the last key's, and a half that is not there is the other one's rows.
         const int left = any - t * KT;          // keys of the tile
-        const uint32_t halves = (first_there ? 1u : 0u) | (second_there && left > 16 ? 2u : 0u);
+        const bool all = (steps.whole >> j & 3) == 3;
+        const uint32_t halves = all ? 3 : (uint32_t)(steps.there >> j) & (left > 16 ? 3 : 1);
         ways |= halves << 2 * ahead;
-        unsigned char *const to = ring + to_ring;
-        to_ring = to_ring + TILE < NB * TILE ? to_ring + TILE : 0;
-        if (halves == 3 && left >= KT) {
+        uint32_t half[2] = {(uint32_t)__builtin_amdgcn_readlane(steps.at, j), (uint32_t)__builtin_amdgcn_readlane(steps.at, j + 1)};
+        if (halves == 2) half[0] = half[1];
+        if (!(halves & 2)) half[1] = half[0];
+        uint32_t off[LOADS];
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const unsigned char *base = is_value(i) ? second_of(i) ? v_second : v_first : second_of(i) ? k_second : k_first;
-                if (mine_there[i]) fetch(base, offset[i], to + number_of(i) * 1024);
-            }
-        } else {
-            const unsigned char *k0 = static_cast<const unsigned char *>(p.k), *v0 = static_cast<const unsigned char *>(p.v), *k1, *v1;
-            if (halves) k0 = halves & 1 ? k_first : k_second, v0 = halves & 1 ? v_first : v_second;
-            k1 = halves & 2 ? k_second : k0;
-            v1 = halves & 2 ? v_second : v0;
-            const int end0 = halves == 2 ? left - 16 : left, end1 = halves & 2 ? left - 16 : left;
+        for (int i = 0; i < LOADS; ++i) off[i] = offset[i];
+        if (!all) {
+            int here = lane;                    // rows are formed here, not kept for the loop
+            asm volatile("" : "+v"(here));
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 int r, column;
-                const bool there_too = place(i, r, column);
-                const int end = second_of(i) ? end1 : end0;
-                const unsigned char *base = is_value(i) ? second_of(i) ? v1 : v0 : second_of(i) ? k1 : k0;
-                if (there_too)
-                    fetch(base, (uint32_t)((r < end ? r : end - 1) * (is_value(i) ? a.dv : 2 * a.d) + column) * (uint32_t)sizeof(T), to + number_of(i) * 1024);
+                place(i, here, r, column);
+                const int past = r + 1 - ((second_of(i) ? halves & 2 : halves == 2) ? left - 16 : left);
+                if (past > 0) off[i] -= (uint32_t)(past * (is_value(i) ? a.dv : 2 * a.d)) * (uint32_t)sizeof(T);
             }
         }
+        const unsigned char *const k[2] = {keys + (uint64_t)half[0] * key_step, keys + (uint64_t)half[1] * key_step};
+        const unsigned char *const v[2] = {values + (uint64_t)half[0] * value_step, values + (uint64_t)half[1] * value_step};
+        unsigned char *const to = ring + to_ring;
+        to_ring = to_ring + TILE < NB * TILE ? to_ring + TILE : 0;
+        // (a load covers rows as a whole, so that some of its lanes are always there, and it counts)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            if (mine_there[i]) fetch(is_value(i) ? v[second_of(i)] : k[second_of(i)], off[i], to + number_of(i) * 1024);
     };
     for (int i = 0; i < AHEAD && i < number; ++i) load(begin + i, i);
 
-    // A tile's part of the loop, with `use` what a wave does that sees some of its keys.  Waves that are past their keys go on loading for the others, in a loop of its own
-    // (a condition around the products has the accumulators copied in every tile).
     int i = 0;
-    const auto tile_of = [&](const auto &use) __attribute__((always_inline)) {
-        if (i + AHEAD <= number) wait_and_meet<(AHEAD - 1) * LOADS>();
-        else wait_and_meet<0>();
+    const auto next_tile = [&](const auto &use) __attribute__((always_inline)) {
         const uint32_t halves = ways & 3;
         ways >>= 2;
         if (i + AHEAD < number) load(begin + i + AHEAD, AHEAD - 1);         // where the last tile stood: every wave is past it
@@ -787,14 +807,28 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
         ++i;
     };
     const int open = (wave_all < wave_any ? wave_all : wave_any) / KT - begin, seen = (wave_any + KT - 1) / KT - begin;
-    while (i < number && i < open && (ways & 3) == 3)
-        tile_of([&](int, uint32_t, const unsigned char *t) { page_keys<false, T, D, DV>(state, q, t, c, 0, 0); });
-    while (i < number && i < seen)
-        tile_of([&](int key, uint32_t halves, const unsigned char *t) {
+    // as long as there is a tile to load for each that is used, and every row sees all of it
+    const int many = open < number - AHEAD ? open : number - AHEAD;
+    while (i < many && (ways & 3) == 3) {
+        wait_and_meet<(AHEAD - 1) * LOADS>();
+        next_tile([&](int, uint32_t, const unsigned char *t) { page_keys<false, T, D, DV>(state, q, t, c, 0, 0); });
+    }
+    // then the others.  Waves that are past their keys go on loading for those that are not, in a loop of its own (a condition around the products has the accumulators copied in every tile).
+    const auto wait = [&]() __attribute__((always_inline)) {
+        if (i + AHEAD <= number) wait_and_meet<(AHEAD - 1) * LOADS>();
+        else wait_and_meet<0>();
+    };
+    while (i < number && i < seen) {
+        wait();
+        next_tile([&](int key, uint32_t halves, const unsigned char *t) {
             const uint32_t word = (masks ? seen_word(key, length, mask) : 0xffffffffu) & ((halves & 1 ? 0xffffu : 0u) | (halves & 2 ? 0xffff0000u : 0u));
             if (halves) page_keys<true, T, D, DV>(state, q, t, c, limit - key, word);
         });
-    while (i < most) tile_of([](int, uint32_t, const unsigned char *) {});
+    }
+    while (i < most) {
+        wait();
+        next_tile([](int, uint32_t, const unsigned char *) {});
+    }
 
     // the parts: every row's maxima, sums and products but the first part's go to LDS; a row that is no query's has seen nothing
     float total[2];
@@ -843,14 +877,17 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
                 for (int n = 0; n < ACC; ++n) state.o[m][n / AR][n % AR] = 0.0f;
     }
-    if (row >= a.R) return;
+    int late = lane_row<TR>();          // the row and its query once more, not kept for the loop
+    asm volatile("" : "+v"(late));
+    const int out_row = first + late, out_query = grid.group(out_row);
+    if (out_row >= a.R) return;
     if (!partial) {
-        const int head = hk * a.G + row - query * a.G;
+        const int head = hk * a.G + out_row - out_query * a.G;
         const float lam = lambda_of(a, head, static_cast<const T *>(nullptr));
         float factor[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) factor[m] = total[m] > 0.0f ? 1.0f / total[m] : 0.0f;
-        T *to = static_cast<T *>(out) + (((int64_t)b * a.Lq + query) * a.H + head) * a.dv;
+        T *to = static_cast<T *>(out) + (((int64_t)b * a.Lq + out_query) * a.H + head) * a.dv;
 #pragma unroll
         for (int blk = 0; blk < DV / TR; ++blk) {
             const int col = blk * TR + 4 * lane_group<TR>();
@@ -861,7 +898,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
             store_pack<T, 4>(to + col, a.dv - col, r);
         }
     } else {
-        float *to = partial + (((int64_t)share.slot * a.Hkv + hk) * a.R + row) * (2 * (int64_t)a.dv + 4);
+        float *to = partial + (((int64_t)share.slot * a.Hkv + hk) * a.R + out_row) * (2 * (int64_t)a.dv + 4);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
@@ -990,22 +1027,22 @@ struct PagesRun {
     int32_t *spans;
     hipStream_t st;
     template <int D, int DV, int RG>
-    void tiles(dim3 grid) const
+    void tiles(dim3 blocks, const Grid &grid) const
     {
         if constexpr (FITS<T, D, DV>(RG))
-            hipLaunchKernelGGL((page_tiles_kernel<T, D, DV, RG>), grid, dim3(WAVES * 64), 0, st, a, p, masks, out, partial, spans, plan.slots, (int)plan.row_tiles);
+            hipLaunchKernelGGL((page_tiles_kernel<T, D, DV, RG>), blocks, dim3(WAVES * 64), 0, st, a, p, masks, out, partial, spans, grid);
     }
     template <int D, int DV>
     int operator()() const
     {
-        const int64_t blocks = plan.row_tiles * a.Hkv * plan.slots;
-        if (blocks > INT32_MAX) return fail(MAM_ERR_UNSUPPORTED, "too many tiles");
-        const dim3 grid((unsigned)blocks);
-        if (plan.groups == 8) tiles<D, DV, 8>(grid);
-        else if (plan.groups == 4) tiles<D, DV, 4>(grid);
-        else if (plan.groups == 2) tiles<D, DV, 2>(grid);
-        else if (a.fast) hipLaunchKernelGGL((pages_kernel<T, D, DV, true>), grid, dim3(256), 0, st, a, p, masks, out, partial, spans, plan.slots, (int)plan.row_tiles);
-        else hipLaunchKernelGGL((pages_kernel<T, D, DV, false>), grid, dim3(256), 0, st, a, p, masks, out, partial, spans, plan.slots, (int)plan.row_tiles);
+        if ((int64_t)a.Hkv * plan.slots > INT32_MAX || plan.row_tiles > 65535) return fail(MAM_ERR_UNSUPPORTED, "too many requests or rows for a launch");
+        const dim3 blocks((unsigned)(a.Hkv * plan.slots), (unsigned)plan.row_tiles);
+        const Grid grid{plan.slots, (int)plan.row_tiles, Divider(a.Hkv), Divider(a.G), Divider(p.S / 16)};
+        if (plan.groups == 8) tiles<D, DV, 8>(blocks, grid);
+        else if (plan.groups == 4) tiles<D, DV, 4>(blocks, grid);
+        else if (plan.groups == 2) tiles<D, DV, 2>(blocks, grid);
+        else if (a.fast) hipLaunchKernelGGL((pages_kernel<T, D, DV, true>), blocks, dim3(256), 0, st, a, p, masks, out, partial, spans, grid);
+        else hipLaunchKernelGGL((pages_kernel<T, D, DV, false>), blocks, dim3(256), 0, st, a, p, masks, out, partial, spans, grid);
         int rc = check_launch("attention over pages");
         if (rc != MAM_OK || !partial) return rc;
         hipLaunchKernelGGL((join_pages_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.B * a.Hkv * a.R, 4)), dim3(256), 0, st, a, out, partial, spans);
