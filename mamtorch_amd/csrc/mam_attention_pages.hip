@@ -2,8 +2,8 @@
 //
 // Few rows are bound by reading K and V once.  A wave takes 16 rows (queries times the heads that share a key head) and a range of the keys, 32 at a time, straight from
 // the pages as the fragments of both products (as mam_attention_split.hip does from dense keys); no wave waits for another.  A page's size is a multiple of 16 tokens, so the
-// 16 keys of a fragment stand in one page, and what a tile of 32 needs of the table is two numbers that all its lanes share: a wave keeps 64 entries of the table in a
-// register, an entry a lane.
+// 16 keys of a fragment stand in one page, and what a tile of 32 needs of the table is two numbers that all its lanes share: a wave keeps where 64 steps of 16 tokens stand in a
+// register, a step a lane.
 //
 // All tokens of the cache are seen by every row; of the new ones a row sees those that its mask names, or those up to itself.  So only the last tiles are limited.
 #include "mam_attention.h"
@@ -39,43 +39,7 @@ struct Grid {
     Divider heads, group, page;         // of Hkv, of G, of the steps of 16 tokens of a page
 };
 
-// A request's table, walked in steps of 16 tokens.
-struct Walk {
-    const int32_t *row;
-    int slots, P, S, Hkv, hk;
-    int base, ids;                      // 64 entries from `base` on, one a lane
-    int slot, off;
-
-    __device__ __forceinline__ Walk(const Pages &p, int b, int head, int key)
-        : row(p.table + (int64_t)b * p.slots), slots(p.slots), P(p.P), S(p.S), Hkv(p.Hkv), hk(head), base(0), ids(-1)
-    {
-        slot = key / S;
-        off = key - slot * S;
-        read();
-    }
-    __device__ __forceinline__ void read()
-    {
-        base = slot;
-        const int mine = slot + (threadIdx.x & 63);
-        ids = mine < slots ? row[mine] : -1;
-        asm volatile("" : "+v"(ids));       // waited for here: behind the branch around this call every use would wait for all loads on their way
-    }
-    // Row of the pages where the next 16 tokens begin, -1 where the request has none.
-    __device__ __forceinline__ int64_t next()
-    {
-        if (slot - base >= 64) read();
-        const int page = __builtin_amdgcn_readlane(ids, slot - base);
-        const int64_t r = page < 0 || page >= P ? -1 : ((int64_t)page * Hkv + hk) * S + off;
-        off += 16;
-        if (off == S) {
-            off = 0;
-            ++slot;
-        }
-        return r;
-    }
-};
-
-// 64 steps of 16 tokens from `first` on, one a lane: which step of the pages each is, and those that there are, and that are below `end` tokens as a whole.
+// A request's table as steps of 16 tokens, 64 of them from `first` on, one a lane: which step of the pages each is, those that there are, and those that are below `end` tokens as a whole.
 struct Steps {
     const int32_t *row;
     int slots, P, per, heads, head;
@@ -239,7 +203,18 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
     for (int m = 0; m < 2; ++m) load_rows<T, TR, D>(qs, row, there, m, q[m]);
     const float c = a.scale * LOG2E;
 
-    Walk walk(p, b, hk, begin);
+    Steps steps(p, b, hk);
+    steps.read(begin / 16, room, grid.page);
+    // rows of the pages where the 16 keys from key and from key + 16 on begin, -1 where the request has none
+    const auto rows_of = [&](int key, int64_t (&r)[2]) {
+        int j = key / 16 - steps.first;
+        if (j >= 64) {
+            steps.read(key / 16, room, grid.page);
+            j = 0;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) r[n] = steps.there >> (j + n) & 1 ? (int64_t)__builtin_amdgcn_readlane(steps.at, j + n) * 16 : -1;
+    };
     int64_t rows[2], next_rows[2];
     Frag<T> k[2][BLOCKS<TR>][NK];
     // addresses of single elements are formed where they are used, not kept for the loop
@@ -294,8 +269,7 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[m][j][i] = 0.0f;
     if (begin < end) {
-        rows[0] = walk.next();
-        rows[1] = walk.next();
+        rows_of(begin, rows);
         if (AHEAD) load_keys(begin, rows);
     }
     for (int key = begin; key < end; key += 32) {
@@ -313,8 +287,7 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
             }
         const bool pages = rows[0] >= 0 && rows[1] >= 0;
         if (key + 32 < end) {
-            next_rows[0] = walk.next();
-            next_rows[1] = walk.next();
+            rows_of(key + 32, next_rows);
         } else {                // past the range: nothing
             next_rows[0] = next_rows[1] = -1;
         }
