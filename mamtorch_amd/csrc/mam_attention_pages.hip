@@ -5,6 +5,8 @@
 // 16 keys of a fragment stand in one page, and what a tile of 32 needs of the table is two numbers that all its lanes share: a wave keeps where 64 steps of 16 tokens stand in a
 // register, a step a lane.
 //
+// Measured: 16 requests of up to 16384 tokens, 4 key heads of 64/128 for 16, bf16, one token each: 87 us with the join's 7, 4.7 TB/s (a copy reaches 5.4).
+//
 // All tokens of the cache are seen by every row; of the new ones a row sees those that its mask names, or those up to itself.  So only the last tiles are limited.
 #include "mam_attention.h"
 #include "mam_pages.h"
@@ -17,7 +19,9 @@ constexpr int ROWS = 16;                // rows of a wave
 
 // A partial row: both maps' products relative to their maxima, then maximum and sum of each.
 inline int64_t partial_size(const Call &a) { return 2 * (int64_t)a.dv + 4; }
-constexpr int FEW = 16;                 // rows of a key head that are streamed
+// Rows of a key head that are streamed; more share tiles of keys.  Eight requests with 4 key heads of 64/128 behind 16384 tokens, 32 rows: bf16 59 us by tiles, 75 streamed; fp32, which the
+// matrix cores bound, 232 by tiles, 178 streamed (64 rows: 239 by tiles, 303 streamed).
+constexpr int FEW(int type) { return type == MAM_F32 ? 32 : 16; }
 
 // A value that all lanes share, where the compiler does not see it: loops over it are branches of the wave, not of lanes.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -70,8 +74,9 @@ __device__ __forceinline__ uint32_t seen_word(int key, int length, uint64_t mask
 }
 
 // A workgroup's share of a call: a request, and which part of its keys.  The slots go to the requests by their lengths: one each, the others in proportion, as far as a part keeps
-// LEAST_TILES tiles.  Every wave works them out for itself from the lengths, a request a lane.
-constexpr int LEAST_TILES = 8;
+// LEAST_TILES tiles, of which each of a workgroup's waves has one then.  Every wave works them out for itself from the lengths, a request a lane.  (Eight requests behind 1000 tokens, 4 key
+// heads of 64/128, fp32, 4 rows each: 28 us; with 8 tiles at least 32, with 2 37 us.  Parts of equal tiles, found by trying, balance no better: trees of 32 tokens 47.7 us, here 46.6.)
+constexpr int LEAST_TILES = 4;
 struct Share { int b, part, parts, slot, length, count; };
 
 __device__ __forceinline__ Share share_of(const Call &a, const Pages &p, int slot, int slots, int32_t *spans)
@@ -162,8 +167,12 @@ __device__ __forceinline__ void page_piece(const T *base, uint32_t offset, bool 
     }
 }
 
+// Workgroups of a CU that the registers leave room for.  More than fit at once are a second round: eight requests behind 4000 tokens, 4 key heads of 128/256, 4 rows each: bf16 48 us,
+// with two a CU 70; fp32, 128 rows, 331 and 519 us.
+constexpr int STREAMS(int size, int d, int dv, bool fast) { return d > 64 || dv > 128 || ((size == 4 || !fast) && dv > 64) ? 1 : 2; }
+
 template <class T, int D, int DV, bool FAST>
-__global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 64) ? 1 : 2) void pages_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks,
+__global__ __launch_bounds__(256, STREAMS(sizeof(T), D, DV, FAST)) void pages_kernel(const Call a, const Pages p, const int64_t *__restrict__ masks,
                                                                                                             void *out, float *partial, int32_t *spans, Grid grid)
 {
     constexpr int TR = ROWS, NK = D / KS<T, TR>, E = DV / 16;           // E: elements of a lane's values
@@ -440,6 +449,11 @@ __global__ __launch_bounds__(256, D > 64 || ((sizeof(T) == 4 || !FAST) && DV > 6
 // no score counts; heads smaller than the kernel's have zeros behind them that no load touches.
 //
 // In 16-bit types the probabilities are rounded once: what 16 bits leave of the first map's is not kept here, as in mam_attention.hip's kernels for many rows (a third product of the values).
+//
+// Measured: 8 trees of 32 tokens behind up to 8192, 4 key heads of 64/128 for 16, bf16: 47 us, of which this kernel 42 and the join 9 (overlapped by 4): 5 us to the first tile, 25 tiles of 1.2 us,
+// 2 us to store 34 MB of parts.  Per tile and SIMD two waves have 770 cycles of products, 1020 of reads of LDS and 1260 of vector instructions, which hide each other only in part.  Scores of the next
+// tile under the exponentials of this one: 47.0 us; six and eight tiles of LDS instead of four: 50.5 and 51.1 (49.4 at the time); 64 rows and two parts of the keys in a workgroup, which halves
+// the parts' bytes and reads every key twice: 72.  Two chunks of 509 behind up to 4099, 2 key heads of 128/256 for 8, fp16: 83 us, 580 TFLOP/s.
 
 // Places of a tile's pieces: W elements a row, so that 16 rows' pieces of a column (keys), and the 8 rows of 32 bytes (16-bit types) or 4 rows of 64 (fp32) that a read of columns
 // takes at a time (values), are in all banks.
@@ -949,6 +963,7 @@ template <class T, int D, int DV>
 constexpr bool FITS(int groups)
 {
     if (DV > 128) return sizeof(T) == 2 && groups == 8;
+    if (groups == 2 && sizeof(T) == 4) return false;            // as few rows are streamed
     return (groups == 2 ? RING<T, D, DV, 2> : groups == 4 ? RING<T, D, DV, 4> : RING<T, D, DV, 8>) >= 2;
 }
 template <class T>
@@ -971,11 +986,11 @@ struct Plan {
 Plan plan_of(const Call &a, const Pages &p, int type)
 {
     Plan plan{};
-    if (a.R > FEW && a.fast && p.P > 0)         // heads that end inside 16 bytes are streamed
+    if (a.R > FEW(type) && a.fast && p.P > 0)         // heads that end inside 16 bytes are streamed
         plan.groups = type == MAM_F32 ? with_head_sizes(a.d, a.dv, GroupsOf<float>{a.R}) : with_head_sizes(a.d, a.dv, GroupsOf<bf16>{a.R});
     plan.row_tiles = ceil_div(a.R, plan.groups ? plan.groups * ROWS : ROWS);
-    // two workgroups of four waves a CU, or one of eight; a request's part is at least as long as the waves have tiles to begin with
-    const int64_t rows = a.Hkv * plan.row_tiles, want = (plan.groups ? 1 : 2) * kNumCU / (rows > 0 ? rows : 1), most = ceil_div(a.Lk, LEAST_TILES * KT) * a.B;
+    // as many workgroups as there is room for at once
+    const int64_t rows = a.Hkv * plan.row_tiles, want = (plan.groups ? 1 : STREAMS((int)type_size(type), a.d, a.dv, a.fast)) * kNumCU / (rows > 0 ? rows : 1), most = ceil_div(a.Lk, LEAST_TILES * KT) * a.B;
     int64_t n = want < most ? want : most;
     if (n > 64 * (int64_t)a.B) n = 64 * (int64_t)a.B;
     plan.slots = n > a.B ? (int)n : a.B;
