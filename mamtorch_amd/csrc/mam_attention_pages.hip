@@ -719,7 +719,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2
     uint32_t offset[LOADS];                     // bytes from a half's rows to a lane's piece of a whole tile
     bool mine_there[LOADS];
     const auto number_of = [&](int i) __attribute__((always_inline)) { return (i * RG + group) % ALL; };       // a wave that has none left loads another one's again
-    const auto is_value = [&](int i) __attribute__((always_inline)) { return KeyTile::LOADS % RG == 0 ? i >= KeyTile::LOADS / RG : number_of(i) >= KeyTile::LOADS; };
+    const auto is_value = [&](int i) __attribute__((always_inline)) { return KeyTile::LOADS % RG == 0 && ALL % RG == 0 ? i >= KeyTile::LOADS / RG : number_of(i) >= KeyTile::LOADS; };
     const auto second_of = [&](int i) __attribute__((always_inline)) {
         const bool value = is_value(i);
         return (value ? number_of(i) - KeyTile::LOADS : number_of(i)) >= (value ? ValueTile::LOADS : KeyTile::LOADS) / 2;
@@ -1023,7 +1023,7 @@ struct PagesRun {
     template <int D, int DV>
     int operator()() const
     {
-        if ((int64_t)a.Hkv * plan.slots > INT32_MAX || plan.row_tiles > 65535) return fail(MAM_ERR_UNSUPPORTED, "too many requests or rows for a launch");
+        if ((int64_t)a.Hkv * plan.slots > UINT32_MAX / (WAVES * 64) || plan.row_tiles > 65535) return fail(MAM_ERR_UNSUPPORTED, "too many requests or rows for a launch");
         const dim3 blocks((unsigned)(a.Hkv * plan.slots), (unsigned)plan.row_tiles);
         const Grid grid{plan.slots, (int)plan.row_tiles, Divider(a.Hkv), Divider(a.G), Divider(p.S / 16)};
         if (plan.groups == 8) tiles<D, DV, 8>(blocks, grid);
@@ -1054,6 +1054,7 @@ int fill_pages_call(const mam_diff_attention_pages_t *x, Call &c, Pages &p)
     a.lam_type = x->lam_type;
     rc = fill_call(&a, c);
     if (rc != MAM_OK) return rc;
+    if (g.P * g.Hkv > INT32_MAX / (g.S / 16 > 0 ? g.S / 16 : 1)) return fail(MAM_ERR_UNSUPPORTED, "too many pages");      // their steps of 16 tokens are counted in 32 bits
     if (x->masks && x->N > 64) return fail(MAM_ERR_UNSUPPORTED, "a tree has 64 tokens at most, got %lld", (long long)x->N);
     const int64_t pack = 16 / type_size(g.type);
     c.fast = g.D % pack == 0 && g.Dv % pack == 0;

@@ -192,6 +192,41 @@ def test_long_caches(dtype):
     Case([16384], 20, 16, 2, 1, 32, 64, dtype, 160, _tree_masks(1, 20, 9)).check("long tree")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 20])
+def test_requests_of_very_different_lengths(n, dtype):
+    # more requests than a wave has lanes, some of them in several parts
+    rng = random.Random(n)
+    lengths = [rng.choice([0, 1, 3, 40, 333, 900]) for _ in range(130)]
+    counts = [rng.choice([0, 1, n, n]) for _ in range(130)]
+    Case(lengths, n, 16, 1, 1, 32, 64, dtype, 170, counts=counts).check("many requests")
+    Case([12000] + [0] * 7, n, 32, 4, 2, 64, 64, dtype, 180, counts=[n] + [0, 1] * 3 + [n]).check("one long one")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_long_parts_with_holes(n, dtype):
+    # parts of more tiles than a wave reads of the table at once, and pages that are not there among them
+    case = Case([5000, 6100, 4444, 10, 2000, 5999, 17, 3000], n, 16, 32, 8, 64, 64, dtype, 190, spare=0)
+    for request, slot in ((0, 150), (0, 151), (1, 0), (1, 381), (2, 33), (4, 124), (5, 200), (7, 187)):
+        case.table[request, slot] = -1
+    case.check("holes")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [17, 33, 50, 65, 130, 200])
+@pytest.mark.parametrize("d, dv", HEADS + [(24, 40), (40, 48), (40, 96), (72, 24), (72, 136), (24, 200)])
+def test_rows_of_a_key_head(d, dv, n, dtype):
+    # every way to share a tile among waves, for each size of heads and for heads below it
+    Case([700, 33], n, 32, 1, 1, d, dv, dtype, 210).check("%d rows" % n)
+
+
+@pytest.mark.parametrize("d, dv, n", [(128, 256, 9), (128, 256, 33), (64, 128, 17), (128, 128, 12)])
+def test_long_parts_of_wide_heads(d, dv, n):
+    for dtype in TYPES:
+        Case([3001, 4100], n, 48, 4, 1, d, dv, dtype, 200, _tree_masks(2, n, n)).check("tree")
+
+
 def test_offsets_past_32_bits():
     # pages beyond 2^32 bytes and elements: 2^33 bytes of keys
     pages, page, d = 2 ** 33 // (16 * 2 * 128 * 2 * 4), 16, 128

@@ -131,6 +131,11 @@ def test_attention(changes, code, text):
     _refused(l.mam_diff_attention_pages(a, ONE, None, 0, None), code, text)
 
 
+def test_attention_over_more_pages_than_it_counts():
+    l = capi.lib()
+    _refused(l.mam_diff_attention_pages(_attention(_pages(P=1 << 28, Hkv=2, S=128)), ONE, None, 0, None), -2, b"too many pages")
+
+
 def test_attention_needs_its_workspace():
     l = capi.lib()
     a = _attention(_pages(slots=1024, P=1024, S=64))
