@@ -20,6 +20,95 @@ struct ForwardOut {
     float *lse;                 // (2, B, H, Lq): log2 of the sums of exponentials, or NULL
 };
 
+// A wave's running state of TR rows.
+template <class T, int TR, int D, int DV, bool MASKED>
+struct State {
+    Acc<TR> o[2][DV / TR];
+    float top[2], sum[2];       // maximum (powers of two) that the exponentials are relative to; this lane's share of their sum
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            top[m] = -INFINITY;
+            sum[m] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < DV / TR; ++b)
+#pragma unroll
+                for (int i = 0; i < TR * TR / 64; ++i) o[m][b][i] = 0.0f;
+        }
+    }
+
+    // Scores of one map (32 keys x TR rows) to probabilities relative to `top`, which rises first where it has to.
+    template <bool LIMITED, int USED>
+    __device__ __forceinline__ void softmax(int m, const Acc<TR> (&s)[BLOCKS<TR>], float c, int limit, uint32_t word, float (&p)[REGS<TR>])
+    {
+        float most = -INFINITY;
+#pragma unroll
+        for (int f = 0; f < USED; ++f) {
+            float v = s[f / (TR * TR / 64)][f % (TR * TR / 64)];
+            if constexpr (LIMITED) {
+                const int key = index_of<TR>(f);
+                v = key < limit && (!MASKED || (word >> key & 1)) ? v : -INFINITY;
+            }
+            p[f] = v;
+            most = fmaxf(most, v);
+        }
+        most = groups_max<TR>(most) * c;
+        if (__any(most > top[m] + SLACK)) {
+            asm volatile("; a new maximum");       // kept a branch: as selects it is two operations for each accumulator and tile
+            const float rise = fmaxf(top[m], most), factor = rise == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[m] - rise);
+            top[m] = rise;
+            sum[m] *= factor;
+#pragma unroll
+            for (int b = 0; b < DV / TR; ++b)
+#pragma unroll
+                for (int i = 0; i < TR * TR / 64; ++i) o[m][b][i] *= factor;
+        }
+        const float base = top[m] == -INFINITY ? 0.0f : top[m];
+        float add = 0.0f;
+#pragma unroll
+        for (int f = 0; f < USED; ++f) {
+            p[f] = __builtin_amdgcn_exp2f(fmaf(p[f], c, -base));
+            add += p[f];
+        }
+        sum[m] += add;
+    }
+
+    // 32 keys (the first 16: HALF): their scores, probabilities, and the products with their values.
+    template <bool LIMITED, bool HALF>
+    __device__ __forceinline__ void keys(const Frag<T> (&q)[2][D / KS<T, TR>], const T *k_tile, int k_pitch, const T *v_tile, int v_pitch,
+                                         float c, int limit, uint32_t word)
+    {
+        constexpr int PART = HALF ? 2 : 1, USED = REGS<TR> / PART;
+        Frag<T> frag[2][FRAGS<T, TR>];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            Acc<TR> s[BLOCKS<TR>];
+#pragma unroll
+            for (int b = 0; b < BLOCKS<TR> / PART; ++b) {
+#pragma unroll
+                for (int i = 0; i < TR * TR / 64; ++i) s[b][i] = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < D / KS<T, TR>; ++kk)
+                    mma<TR>(row_frag<T, TR>(k_tile + m * D, k_pitch, b * TR + lane_row<TR>(), kk), q[m][kk], s[b]);
+            }
+            float p[REGS<TR>];
+            softmax<LIMITED, USED>(m, s, c, limit, word, p);
+            to_frags<T, TR>(p, frag[m], FRAGS<T, TR> / PART);
+        }
+#pragma unroll
+        for (int b = 0; b < DV / TR; ++b) {
+#pragma unroll
+            for (int j = 0; j < FRAGS<T, TR> / PART; ++j) {
+                const Frag<T> v = column_frag<TR>(v_tile, v_pitch, b * TR, j);
+                mma<TR>(v, frag[0][j], o[0][b]);
+                mma<TR>(v, frag[1][j], o[1][b]);
+            }
+        }
+    }
+};
+
 // Waves of a SIMD that the registers are shared between: accumulators take DV * TR / 32 of a lane's, queries D * TR * size / 128.
 template <class T, int TR, int D, int DV>
 constexpr int WAVES = DV * TR / 32 + D * TR * (int)sizeof(T) / 128 <= 160 ? 2 : 1;
