@@ -134,7 +134,6 @@ class PageTable:
         self.refs = torch.zeros(pages, device=device, dtype=torch.int32)
         self.caches = []
         self.granted = self.masks = self.positions = None       # of the step that has begun
-        self._forked = False
 
     def _vector(self, value) -> Tensor:
         if isinstance(value, Tensor):
@@ -150,11 +149,10 @@ class PageTable:
         self.masks = self.positions = None
         counts = self._vector(parents.shape[1] if counts is None else counts)
         self.granted, copies = K.pages_extend(self.table, self.lengths, self.refs, counts, self.page_size)
-        # pages are in common after a fork alone; a captured step may be replayed after one
-        if self._forked or torch.cuda.is_current_stream_capturing():
-            for cache in self.caches:
-                K.pages_copy(cache.k, cache.v, copies)
-        self._forked = False
+        # whatever the step: how long pages stay in common after a fork, and whether a replayed graph held one, the device alone knows.  (4 to 5 us a layer where there is
+        # nothing to copy: one token of 64 requests through 12 layers of 768 takes 3.20 ms, 3.11 without.)
+        for cache in self.caches:
+            K.pages_copy(cache.k, cache.v, copies)
         if parents is not None:
             self.masks, self.positions = K.draft_tree(parents, self.lengths)
         return self.granted
@@ -180,7 +178,6 @@ class PageTable:
         """Request i goes on from what request ``sources[i]`` (int32) was; -1 frees it."""
         K.pages_fork(self.table, self.lengths, self.refs, sources, self.page_size)
         self.granted = self.masks = self.positions = None
-        self._forked = True
 
 
 class DiffAttentionPages:

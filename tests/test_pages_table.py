@@ -1,0 +1,82 @@
+"""nn.PageTable as a server uses it: after every call each request's pages hold its own tokens, whoever shares them, on the host's operators and on the GPU's."""
+import random
+
+import pytest
+import torch
+
+from pages_server import PAGE, Server, place_on
+
+GPU = pytest.param("cuda:0", marks=pytest.mark.gpu)
+
+
+@pytest.fixture(params=["cpu", GPU])
+def device(request, monkeypatch):
+    return place_on(request.param, monkeypatch)
+
+
+def test_pages_in_common_for_longer_than_one_step(device):
+    s = Server(device, 3, 12)
+    s.step([20, 0, 0])
+    s.fork([0, 0, 0])
+    s.step([1, 0, 0])               # the first one leaves the page; the others still share it
+    s.step([0, 1, 0])
+    s.step([1, 1, 1])
+
+
+def test_a_step_of_no_tokens_after_a_fork(device):
+    s = Server(device, 2, 12)
+    s.step([20, 0])
+    s.fork([0, 0])
+    s.step([0, 0])
+    s.step([1, 1])
+
+
+def test_requests_cut_back_into_a_whole_page_in_common(device):
+    s = Server(device, 2, 12)
+    s.step([32, 0])
+    s.fork([0, 0])
+    s.step([1, 1])
+    s.trim([26, 30])
+    s.step([1, 1])
+
+
+def test_a_refused_request_has_its_page_copied_when_there_is_room_again(device):
+    s = Server(device, 3, 4)
+    s.step([20, 0, 30])
+    s.fork([0, 0, 2])
+    assert s.step([1, 0, 0]) == [0, 0, 0]
+    s.trim([20, 20, 0])
+    assert s.step([1, 1, 0]) == [1, 1, 0]
+
+
+@pytest.mark.gpu
+def test_eager_steps_beside_captured_ones():
+    s = Server("cuda:0", 3, 30)
+    s.step([20, 0, 0])
+    one, none = s.ints([1, 0, 0]), s.ints([0, 0, 0])
+
+    def capture(what):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            what()
+        return graph
+
+    def step(counts):
+        s.table.begin(counts)
+        s.table.accept(counts=none)
+
+    s.fork([0, 0, 0])
+    capture(lambda: step(one))                      # nothing has run: the page is shared still
+    s.check("captured begin")
+    s.step([0, 1, 1])
+    sources = s.ints([2, 2, 2])
+    graph = capture(lambda: s.table.fork(sources))
+    for turn in range(3):                           # forks that the host did not see
+        s.step([1, 0, 1])
+        s.step([1, 1, 1])
+        graph.replay()
+        s.tokens = [list(s.tokens[2]) for _ in range(3)]
+        s.check(("replayed fork", turn))
+        s.step([0, 1, 0])
+        s.step([1, 1, 1])
