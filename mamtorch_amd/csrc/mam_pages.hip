@@ -84,7 +84,7 @@ __device__ __forceinline__ int before(int v, int *waves, int &total)
 
 // Room for counts[b] tokens behind each request's, by one workgroup.  What a request takes: pages for slots that have none, and one for a begun last page that others
 // hold too, unless they all come before it and take one themselves.  The requests' needs are added up, the free pages are ranked, and rank r goes to the request
-// whose needs reach past r.  A request whose needs go beyond what is free gets nothing, and so do those behind it that need any.
+// whose needs reach past r.  A request whose needs go beyond what is free gets nothing, and so do those behind it that need any, or that could have gone without if it had been served.
 //
 // Bound by latency: a request a thread (four where there are more than 1024), its few loads side by side, those of the first 16384 pages' counts before all.  Measured:
 // 256 requests of up to 1021 tokens, all of them beams of four that write to pages in common, 1507 pages, 10 us (four requests a thread from the start on: 24 us).
@@ -186,6 +186,19 @@ __global__ __launch_bounds__(EXTEND) void extend_kernel(const Book k, const int3
     }
     __threadfence_block();
     __syncthreads();
+    // Where pages run out, an earlier request that was to give up a page keeps it: the one that counted on that needs a copy, for which there is no page either.  All
+    // that write to the page before it were to give it up, and needs are met up to some request, so the last of them tells.
+    if (total > have) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int b = u * EXTEND + t, page = b < k.B && copy[u] < 0 && want[u] == 0 ? last[b] : -1;
+            if (page < 0) continue;
+            int i = b - 1;
+            while (i >= 0 && last[i] != page) --i;
+            if (i >= 0 && until[i] > have) c_of[u] = 0;
+        }
+        __syncthreads();
+    }
     // requests whose needs are met are the first ones, and of those behind them the ones without needs
 #pragma unroll
     for (int u = 0; u < PER; ++u) {

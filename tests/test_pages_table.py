@@ -80,3 +80,31 @@ def test_eager_steps_beside_captured_ones():
         s.check(("replayed fork", turn))
         s.step([0, 1, 0])
         s.step([1, 1, 1])
+
+
+def test_a_request_that_is_refused_keeps_the_page_that_it_would_have_left(device):
+    s = Server(device, 2, 2)
+    s.step([20, 0])
+    s.fork([0, 0])
+    s.trim([20, 18])
+    assert s.step([1, 1]) == [0, 0]         # the first finds no page for its copy and holds on to the one in common: the second cannot write there
+    s.trim([20, 0])
+    assert s.step([1, 0]) == [1, 0]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_a_server_with_few_pages_at_random(device, seed):
+    rng = random.Random(seed)
+    batch = rng.choice([2, 3, 5])
+    s = Server(device, batch, rng.choice([batch, 2 * batch, 3 * batch]), 5 * PAGE)
+    for _ in range(30):
+        what = rng.random()
+        if what < 0.5:
+            s.step([rng.choice([0, 1, 1, rng.randint(1, 20)]) for _ in range(batch)], rng.choice([None, [rng.randint(-1, 20) for _ in range(batch)]]))
+        elif what < 0.7:
+            s.fork([rng.choice([b, rng.randint(-1, batch), rng.randrange(batch)]) for b in range(batch)])
+        elif what < 0.85:
+            s.trim([rng.choice([len(t), rng.randint(0, len(t)), 0]) for t in s.tokens])
+        else:
+            n = rng.choice([1, 4, 9])
+            s.draft([[rng.randint(-1, i - 1) for i in range(n)] for _ in range(batch)], [sorted(rng.sample(range(n), n)) for _ in range(batch)], [rng.randint(0, n) for _ in range(batch)])
