@@ -159,15 +159,25 @@ class PageTable:
 
     def accept(self, path: Tensor = None, counts=None) -> None:
         """Takes over the new tokens of the step: the first ``counts`` of each request (a number, or int32 (batch); by default all that it had room for) or, with ``path``
-        (batch, n), int32, those that it names, in ascending order.  No more than there was room for; other new tokens are forgotten."""
+        (batch, n), int32, those that it names, in ascending order, up to an entry that does not ascend or names none of them.  No more than there was room for; other new
+        tokens are forgotten."""
         if self.granted is None:
             raise ValueError("no step has begun")
         counts = self.granted if counts is None else torch.minimum(self._vector(counts).clamp(min=0), self.granted)
         if path is not None:
-            counts = counts.clamp(max=path.shape[1])
+            counts = torch.minimum(counts, self._named(path))
             for cache in self.caches:
                 K.pages_compact(cache.k, cache.v, self.table, self.lengths, path, counts)
         self.trim(self.lengths + counts)
+
+    def _named(self, path: Tensor) -> Tensor:
+        """How many entries of each request's path name tokens that it had room for, in ascending order."""
+        n = path.shape[1]
+        if n == 0:
+            return torch.zeros_like(self.granted)
+        ok = (path > nn.functional.pad(path, (1, 0), value=-1)[:, :-1]) & (path < self.granted[:, None])
+        # a running minimum, not a reduction: one over many blocks would clear its memory by a node that a graph must not hold
+        return torch.where(ok, n, torch.arange(n, device=path.device, dtype=torch.int32)).cummin(1).values[:, -1]
 
     def trim(self, ends) -> None:
         """Requests end at ``ends`` (a number, or int32 (batch)); 0 frees a request."""

@@ -108,3 +108,48 @@ def test_a_server_with_few_pages_at_random(device, seed):
         else:
             n = rng.choice([1, 4, 9])
             s.draft([[rng.randint(-1, i - 1) for i in range(n)] for _ in range(batch)], [sorted(rng.sample(range(n), n)) for _ in range(batch)], [rng.randint(0, n) for _ in range(batch)])
+
+
+LINE = [[i - 1 for i in range(6)]] * 4
+
+
+@pytest.mark.parametrize("counts", [None, [6, 6, 6, 6], [2, 3, 1, 0]])
+def test_a_path_names_tokens_of_the_step_alone(device, counts):
+    s = Server(device, 4, 24)
+    s.step([20, 3, 16, 0])
+    # padded trees of 4, 6, 2 and no tokens
+    s.draft(LINE, [[0, 2, 5, 5, 5, 5], [1, 2, 4, 5, 0, 0], [0, 1, 2, 3, 4, 5], [0, 1, 2, 3, 4, 5]], counts, drafted=[4, 6, 2, 0])
+    # names that are none, and that do not ascend
+    s.draft(LINE, [[-1, 0, 1, 2, 3, 4], [0, 0, 1, 2, 3, 4], [3, 2, 4, 5, 5, 5], [0, 1, 6, 7, 8, 9]], counts)
+    s.draft(LINE, [[], [], [], []], counts)
+    s.draft(LINE, [[0, 1, 2, 3, 4, 5, 6, 7]] * 4, counts)
+
+
+def test_a_path_of_a_request_without_room(device):
+    s = Server(device, 2, 3)
+    s.step([16, 16])
+    assert s.draft(LINE[:2], [[0, 1, 2, 3, 4, 5]] * 2) == [6, 0]
+
+
+@pytest.mark.gpu
+def test_a_captured_path_ends_where_the_eager_one_does():
+    servers = [Server("cuda:0", 3, 40) for _ in range(2)]
+    path, drafted = servers[0].ints([[0, 1, 2]] * 3), servers[0].ints([0] * 3)
+    parents = servers[0].ints([[-1, 0, 1]] * 3)
+
+    def step(s):
+        s.table.begin(drafted, parents)
+        s.table.accept(path)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(servers[0])
+    for turn, rows in enumerate([[[0, 1, 2]] * 3, [[2, 1, 0], [1, 2, 0], [-1, 0, 1]], [[0, 2, 3], [3, 0, 1], [1, 2, 3]], [[0, 0, 0]] * 3]):
+        path.copy_(servers[0].ints(rows))
+        drafted.copy_(servers[0].ints([3, turn, 2]))
+        graph.replay()
+        step(servers[1])
+        torch.cuda.synchronize()
+        assert servers[0].table.lengths.tolist() == servers[1].table.lengths.tolist()
+        assert torch.equal(servers[0].table.table, servers[1].table.table)
