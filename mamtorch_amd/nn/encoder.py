@@ -216,6 +216,11 @@ class DiffAttentionPages:
         return self.table
 
 
+def _place_after_load(module: "DiffAttention", keys) -> None:
+    # parameters that are assigned may stand on another device than the ones before
+    module._place_frequencies()
+
+
 class DiffAttention(nn.Module):
     """Differential attention after T. Ye et al., "Differential Transformer", 2024: each head's map is the difference of two softmaxes, the second one weighted
     with lambda = exp(q1 . k1) - exp(q2 . k2) + lambda_init from learned vectors, each head's output is normalised by itself and scaled with
@@ -255,6 +260,7 @@ class DiffAttention(nn.Module):
             self.query_norm = nn.Parameter(torch.ones(self.head_size, device=device, dtype=dtype))
             self.key_norm = nn.Parameter(torch.ones(self.head_size, device=device, dtype=dtype))
         self._place_frequencies()
+        self.register_load_state_dict_post_hook(_place_after_load)
 
     def _place_frequencies(self) -> None:
         # no buffer: .half() and its like would round it
@@ -266,6 +272,12 @@ class DiffAttention(nn.Module):
         super()._apply(*args, **kwargs)
         self._place_frequencies()
         return self
+
+    def _frequencies_on(self, device: torch.device) -> Tensor:
+        # a replica on another device shares the attribute
+        if self.frequencies is None or self.frequencies.device == device:
+            return self.frequencies
+        return K.rotary_frequencies(self.rotary, self.base, device)
 
     def lambdas(self) -> Tensor:
         q1, k1, q2, k2 = self.lambda_vectors.float()
@@ -296,16 +308,16 @@ class DiffAttention(nn.Module):
         k = self.key(x).view(b, n, self.kv_heads, 2, self.head_size)
         v = self.value(x).view(b, n, self.kv_heads, self.value_size)
         weights = (self.query_norm, self.key_norm) if self.qk_norm else (None, None)
-        eps = self.qk_eps if self.qk_norm else 0.0
+        eps, frequencies = self.qk_eps if self.qk_norm else 0.0, self._frequencies_on(x.device)
         if paged:
-            q = cache.append(q, k, v, *weights, self.frequencies, eps, self.qk_norm)
+            q = cache.append(q, k, v, *weights, frequencies, eps, self.qk_norm)
             out = cache.attend(q, self.lambdas())
         else:
             if self.qk_norm or self.rotary:
                 places = None
                 if self.rotary and cache is not None:
                     places = cache.lengths[:, None] + torch.arange(n, device=x.device, dtype=torch.int32)
-                q, k = K.norm_rotate(q, k, *weights, self.frequencies, places, eps, self.qk_norm)
+                q, k = K.norm_rotate(q, k, *weights, frequencies, places, eps, self.qk_norm)
             starts = None
             if cache is not None:
                 starts = cache.append(k, v)
