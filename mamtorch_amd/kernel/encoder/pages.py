@@ -8,7 +8,7 @@ requests.  One table may serve the pages of many layers.
 import torch
 from torch import Tensor
 
-from .rotary import check_rotation
+from .rotary import TYPES, check_rotation
 
 __all__ = ["pages_extend", "pages_fork", "pages_trim", "pages_copy", "pages_compact", "draft_tree", "norm_rotate_append", "diff_attention_pages"]
 
@@ -73,55 +73,74 @@ def diff_attention_pages(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Ten
     return K.diff_attention_pages.default(q, k_pages, v_pages, table, lengths, lam, float(q.shape[-1] ** -0.5 if scale is None else scale), counts, masks)
 
 
+# What the operators refuse by shapes and types is refused under tracing too.
+def _check_vector(t, n):
+    torch._check(t is None or (t.dim() == 1 and t.size(0) == n and t.dtype == torch.int32))
+
+
 def _check_pages(k_pages, v_pages):
-    torch._check(k_pages.dim() == 5 and v_pages.dim() == 4 and k_pages.size(3) == 2 and k_pages.dtype == v_pages.dtype)
+    torch._check(k_pages.dim() == 5 and v_pages.dim() == 4 and k_pages.size(3) == 2 and k_pages.dtype == v_pages.dtype and k_pages.dtype in TYPES)
     torch._check(k_pages.shape[:3] == v_pages.shape[:3])
+    torch._check(k_pages.size(2) >= 16 and k_pages.size(2) % 16 == 0)
+    torch._check(1 <= k_pages.size(4) <= 128 and 1 <= v_pages.size(3) <= 256)
 
 
 def _check_table(table, *vectors):
     torch._check(table.dim() == 2 and table.dtype == torch.int32)
     for t in vectors:
-        torch._check(t is None or (t.dim() == 1 and t.size(0) == table.size(0) and t.dtype == torch.int32))
+        _check_vector(t, table.size(0))
+
+
+def _check_book(table, lengths, refs, more, page_size):
+    _check_table(table, lengths, more)
+    torch._check(refs.dim() == 1 and refs.dtype == torch.int32)
+    torch._check(page_size >= 16 and page_size % 16 == 0 and table.size(0) <= 4096)
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::pages_extend")
 def _(table, lengths, refs, counts, page_size):
-    _check_table(table, lengths, counts)
+    _check_book(table, lengths, refs, counts, page_size)
     return table.new_empty((table.size(0),)), table.new_empty((table.size(0), 2))
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::pages_fork")
 def _(table, lengths, refs, sources, page_size):
-    _check_table(table, lengths, sources)
+    _check_book(table, lengths, refs, sources, page_size)
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::pages_trim")
 def _(table, lengths, refs, ends, page_size):
-    _check_table(table, lengths, ends)
+    _check_book(table, lengths, refs, ends, page_size)
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::pages_copy")
 def _(k_pages, v_pages, copies):
     _check_pages(k_pages, v_pages)
+    torch._check(copies.dim() == 2 and copies.size(1) == 2 and copies.dtype == torch.int32)
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::pages_compact")
 def _(k_pages, v_pages, table, lengths, path, counts):
     _check_pages(k_pages, v_pages)
     _check_table(table, lengths, counts)
+    torch._check(path.dim() == 2 and path.size(0) == table.size(0) and path.dtype == torch.int32)
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::draft_tree")
 def _(parents, lengths):
-    torch._check(parents.dim() == 2)
+    torch._check(parents.dim() == 2 and parents.size(1) <= 64 and parents.dtype == torch.int32)
+    _check_vector(lengths, parents.size(0))
     return parents.new_empty(parents.shape, dtype=torch.long), parents.new_empty(parents.shape)
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::norm_rotate_append")
 def _(q, k, v, k_pages, v_pages, table, lengths, counts, q_weight, k_weight, frequencies, positions, eps, norm, interleaved):
-    check_rotation(q, k, q_weight, k_weight, frequencies, positions)
+    check_rotation(q, k, q_weight, k_weight, frequencies, positions, norm)
     _check_pages(k_pages, v_pages)
     _check_table(table, lengths, counts)
+    torch._check(q.size(3) == 2 and q.size(0) == table.size(0) and v.dtype == q.dtype and k_pages.dtype == q.dtype)
+    torch._check(v.dim() == 4 and v.shape[:3] == k.shape[:3])
+    torch._check(k_pages.size(1) == k.size(2) and k_pages.size(4) == k.size(4) and v_pages.size(3) == v.size(3))
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
@@ -129,4 +148,9 @@ def _(q, k, v, k_pages, v_pages, table, lengths, counts, q_weight, k_weight, fre
 def _(q, k_pages, v_pages, table, lengths, lam, scale, counts, masks):
     _check_pages(k_pages, v_pages)
     _check_table(table, lengths, counts)
+    torch._check(q.dim() == 5 and q.size(3) == 2 and q.size(4) == k_pages.size(4) and q.size(0) == table.size(0) and q.dtype == k_pages.dtype)
+    torch._check(q.size(2) == 0 or (k_pages.size(1) > 0 and q.size(2) % k_pages.size(1) == 0))
+    torch._check(lam.dim() == 1 and lam.size(0) == q.size(2) and lam.dtype in (q.dtype, torch.float))
+    torch._check(0 < scale <= 1e30)
+    torch._check(masks is None or (q.size(1) <= 64 and masks.shape == q.shape[:2] and masks.dtype == torch.long))
     return torch.empty((*q.shape[:3], v_pages.size(3)), dtype=q.dtype, device=q.device)

@@ -30,24 +30,29 @@ def norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor = None, k_weight: Tensor 
     return K.norm_rotate.default(q, k, q_weight, k_weight, frequencies, positions, float(eps), bool(norm), bool(interleaved))
 
 
-def check_rotation(q, k, q_weight, k_weight, frequencies, positions):
-    torch._check(q.dim() == 5 and k.dim() == 5 and q.dtype == k.dtype)
+TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def check_rotation(q, k, q_weight, k_weight, frequencies, positions, norm):
+    torch._check(q.dim() == 5 and k.dim() == 5 and q.dtype == k.dtype and q.dtype in TYPES)
     torch._check(k.size(0) == q.size(0) and k.size(1) == q.size(1) and k.size(3) == q.size(3) and k.size(4) == q.size(4))
+    torch._check(1 <= q.size(4) <= 128)
     for w in (q_weight, k_weight):
-        torch._check(w is None or (w.dim() == 1 and w.size(0) == q.size(4) and w.dtype in (q.dtype, torch.float)))
-    torch._check(frequencies is None or (frequencies.dim() == 1 and frequencies.dtype == torch.double))
+        torch._check(w is None or (norm and w.dim() == 1 and w.size(0) == q.size(4) and w.dtype in (q.dtype, torch.float)))
+    torch._check(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype)
+    torch._check(frequencies is None or (frequencies.dim() == 1 and 2 * frequencies.size(0) <= q.size(4) and frequencies.dtype == torch.double))
     torch._check(positions is None or (positions.shape == q.shape[:2] and positions.dtype == torch.int32))
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::norm_rotate")
 def _(q, k, q_weight, k_weight, frequencies, positions, eps, norm, interleaved):
-    check_rotation(q, k, q_weight, k_weight, frequencies, positions)
+    check_rotation(q, k, q_weight, k_weight, frequencies, positions, norm)
     return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
 
 
 @torch.library.register_fake("mamtorch_kernel_encoder::norm_rotate_backward")
 def _(q_grad, k_grad, q, k, q_weight, k_weight, frequencies, positions, eps, norm, interleaved, want_q, want_k, want_q_weight, want_k_weight):
-    check_rotation(q, k, q_weight, k_weight, frequencies, positions)
+    check_rotation(q, k, q_weight, k_weight, frequencies, positions, norm)
     weight = q_weight if q_weight is not None else k_weight
     dtype = q.dtype if weight is None else weight.dtype
     like = [torch.empty(t.shape if w else (0,), dtype=q.dtype, device=q.device) for t, w in ((q, want_q), (k, want_k))]
