@@ -570,7 +570,7 @@ extern "C" int mam_norm_rotate_append(const mam_norm_rotate_t *args, const void 
     if (pages->type != args->type || pages->B != args->B || pages->Hkv != args->Hkv || pages->D != args->D || args->M != 2)
         return fail(MAM_ERR_INVALID_ARGUMENT, "the pages are for other keys");
     if (c.all == 0) return MAM_OK;
-    if ((c.side[0].heads && !q_out) || (c.side[1].heads && (!v || !v_stride || !to.to.k || !to.to.v))) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((c.side[0].heads && !q_out) || (c.side[1].heads && (!v || !v_stride || (to.to.P > 0 && (!to.to.k || !to.to.v))))) return fail(MAM_ERR_INVALID_ARGUMENT, "null pointer");
     to.v = v;
     if (v_stride) {
         to.vb = v_stride[0]; to.vl = v_stride[1]; to.vh = v_stride[2];

@@ -2,10 +2,13 @@
 import random
 
 import pytest
+import torch
 
+import mamtorch_amd as mt
 from test_gpu_pages import Both
 
 pytestmark = pytest.mark.gpu
+enc = mt.kernel.encoder
 
 
 def test_a_page_stays_with_a_holder_that_is_refused():
@@ -69,3 +72,21 @@ def test_many_requests_on_few_pages():
         k.extend([rng.choice([0, 1, 1]) if b > 2900 else 0 for b in range(3000)])
     k.trim([n if b > 2990 else 0 for b, n in enumerate(k.host.lengths)])
     k.extend([1] * 3000)
+
+
+@torch.no_grad()
+def test_a_cache_of_no_pages_takes_and_shows_nothing():
+    make = lambda *s: torch.randn(*s, device="cuda:0")           # noqa: E731
+    q, k, v, kp, vp = make(2, 3, 4, 2, 16), make(2, 3, 2, 2, 16), make(2, 3, 2, 8), make(0, 2, 16, 2, 16), make(0, 2, 16, 8)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda:0")       # noqa: E731
+    table, lengths = ints([-1, 0], [5, -1]), ints(0, 20)
+    assert torch.equal(enc.norm_rotate_append(q, k, v, kp, vp, table, lengths, norm=False), q)
+    assert not enc.diff_attention_pages(q, kp, vp, table, lengths, make(4)).any()
+    server = mt.nn.PageTable(2, 0, 16, most=64, device="cuda:0")
+    module = mt.nn.DiffAttention(96, 3, causal=True, qk_norm=True, rotary=12).to("cuda:0")
+    cache = module.pages(server)
+    assert server.begin(3).tolist() == [0, 0]
+    assert torch.isfinite(module(make(2, 3, 96), cache=cache)).all()
+    server.accept()
+    server.fork(ints(1, 0))
+    assert server.lengths.tolist() == [0, 0]
