@@ -300,3 +300,20 @@ def test_same_bits_on_every_call():
     first = case.run()
     for _ in range(3):
         assert torch.equal(case.run(), first)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("d, dv", HEADS)
+@pytest.mark.parametrize("n, h", [(4, 8), (5, 8), (9, 8), (19, 8), (40, 8), (70, 8)])
+def test_the_first_maps_probabilities_at_any_number_of_rows(n, h, d, dv, dtype):
+    # Without the second map a result errs by its own rounding, by what 32 bits cost (the same operands in fp32) and by what two parts of 8 or 11 bits leave of a probability: 2^-16 or 2^-22 of it,
+    # of fp16 half the spacing of its smallest numbers.  One part alone would leave 2^-8 or 2^-11.
+    case = Case([300, 37, 0], n, 16, h, 2, d, dv, dtype, seed=n)
+    lam = torch.zeros(h)
+    args = case.table, case.lengths, lam, None, None, case.masks
+    want = pref.PagesAttention(case.q.float(), case.k.float(), case.v.float(), *args)
+    sizes = pref.PagesAttention(case.q.float(), case.k.float(), case.v.abs().float(), *args).out
+    bound = want.out_bound + ref.UNIT[dtype] * want.out.abs() + ref.UNIT[dtype] ** 2 * sizes + ref.TINY[dtype]
+    if dtype == torch.float16:
+        bound = bound + 2.0 ** -25 * want.seen.sum(-1)[:, :, None, None] * case.v.abs().max().double()
+    ref.assert_within(case.run(lam=lam.to(DEV)), want.out, bound, "one map")
