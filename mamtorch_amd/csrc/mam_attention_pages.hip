@@ -19,8 +19,8 @@ constexpr int ROWS = 16;                // rows of a wave
 
 // A partial row: both maps' products relative to their maxima, then maximum and sum of each.
 inline int64_t partial_size(const Call &a) { return 2 * (int64_t)a.dv + 4; }
-// Rows of a key head that are streamed; more share tiles of keys.  Eight requests with 4 key heads of 64/128 behind 16384 tokens, 32 rows: bf16 59 us by tiles, 75 streamed; fp32, which the
-// matrix cores bound, 232 by tiles, 178 streamed (64 rows: 239 by tiles, 303 streamed).
+// Rows of a key head that are streamed; more share tiles of keys.  Eight requests with 4 key heads of 64/128 behind 16384 tokens, 32 rows: bf16 55 us by tiles, 72 streamed (four requests 43
+// and 45, one 41 and 37); fp32, which the matrix cores bound, 232 by tiles, 178 streamed (64 rows: 239 by tiles, 303 streamed).
 constexpr int FEW(int type) { return type == MAM_F32 ? 32 : 16; }
 
 // A value that all lanes share, where the compiler does not see it: loops over it are branches of the wave, not of lanes.
@@ -75,7 +75,8 @@ __device__ __forceinline__ uint32_t seen_word(int key, int length, uint64_t mask
 
 // A workgroup's share of a call: a request, and which part of its keys.  The slots go to the requests by their lengths: one each, the others in proportion, as far as a part keeps
 // LEAST_TILES tiles, of which each of a workgroup's waves has one then.  Every wave works them out for itself from the lengths, a request a lane.  (Eight requests behind 1000 tokens, 4 key
-// heads of 64/128, fp32, 4 rows each: 28 us; with 8 tiles at least 32, with 2 37 us.  Parts of equal tiles, found by trying, balance no better: trees of 32 tokens 47.7 us, here 46.6.)
+// heads of 64/128, fp32, 4 rows each: 28 us; with 8 tiles at least 32, with 2 37 us.  Parts of equal tiles, found by trying, balance no better: trees of 32 tokens 47.7 us, so 46.6,
+// both before probabilities had two parts there.)
 constexpr int LEAST_TILES = 4;
 struct Share { int b, part, parts, slot, length, count; };
 
@@ -449,13 +450,14 @@ __global__ __launch_bounds__(256, STREAMS(sizeof(T), D, DV, FAST)) void pages_ke
 // no score counts; heads smaller than the kernel's have zeros behind them that no load touches.
 //
 // In 16-bit types what 16 bits leave of the first map's probabilities is a product of its own, as where rows are streamed: a drafted token more or less does not change how exact the others
-// are.  Without it 47 us for the trees below and 82 for the chunks, 51 and 94 with it; their errors against 64 bits 0.0025 and 0.00032, 0.0019 and 0.00024 with it (results rounded
-// once from 64 bits: 0.0017 and 0.00021).
+// are.  Without it 47 us for the trees below and 82 for the chunks; their errors against 64 bits 0.0025 and 0.00032, with it 0.0019 and 0.00024 (results rounded once from 64 bits: 0.0017 and
+// 0.00021).
 //
-// Measured: 8 trees of 32 tokens behind up to 8192, 4 key heads of 64/128 for 16, bf16: 47 us, of which this kernel 42 and the join 9 (overlapped by 4): 5 us to the first tile, 25 tiles of 1.2 us,
-// 2 us to store 34 MB of parts.  Per tile and SIMD two waves have 770 cycles of products, 1020 of reads of LDS and 1260 of vector instructions, which hide each other only in part.  Scores of the next
-// tile under the exponentials of this one: 47.0 us; six and eight tiles of LDS instead of four: 50.5 and 51.1 (49.4 at the time); 64 rows and two parts of the keys in a workgroup, which halves
-// the parts' bytes and reads every key twice: 72.  Two chunks of 509 behind up to 4099, 2 key heads of 128/256 for 8, fp16: 83 us, 580 TFLOP/s.
+// Measured: 8 trees of 32 tokens behind up to 8192, 4 key heads of 64/128 for 16, bf16: 51 us, of which this kernel 46 and the join 9 (overlapped by 4): 5 us to the first tile, 25 tiles of 1.6 us,
+// 2 us to store 34 MB of parts.  By counters the kernel's 90000 cycles, 3600 a tile, hold for each tile 1020 of products and 1600 of vector instructions of a SIMD's two waves, which hide each
+// other only in part, and 530 of reads of the CU's LDS, without conflicts.  Two chunks of 509 behind up to 4099, 2 key heads of 128/256 for 8, fp16: 94 us, 511 TFLOP/s.  Tried before the probabilities had two parts, beside 47 us:
+// scores of the next tile under the exponentials of this one 47.0; six and eight tiles of LDS instead of four 50.5 and 51.1 (49.4 at the time); 64 rows and two parts of the keys in a workgroup, which
+// halves the parts' bytes and reads every key twice, 72.
 
 // Places of a tile's pieces: W elements a row, so that 16 rows' pieces of a column (keys), and the 8 rows of 32 bytes (16-bit types) or 4 rows of 64 (fp32) that a read of columns
 // takes at a time (values), are in all banks.

@@ -68,7 +68,8 @@ def diff_attention_pages(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Ten
     cache and, of the new ones, those up to itself or, where there are masks (batch, n <= 64; int64), those whose bits are set.
 
     counts (batch, int32): how many of the n tokens a request has, all by default.  A token beyond, or one that sees nothing, gives zeros.  Tokens for which a request has no
-    page are not seen.  What pages hold behind a request's tokens may be anything; NaN or infinities among the new tokens' values may reach those before them, and beside
+    page are not seen.  Softmaxes and sums are float32; in 16-bit types the probabilities beside v are rounded to the type, those of the first map in two parts, whatever the number of tokens.
+    What pages hold behind a request's tokens may be anything; NaN or infinities among the new tokens' values may reach those before them, and beside
     them in the tree.  No gradient."""
     return K.diff_attention_pages.default(q, k_pages, v_pages, table, lengths, lam, float(q.shape[-1] ** -0.5 if scale is None else scale), counts, masks)
 
