@@ -604,7 +604,8 @@ int mam_norm_rotate_append(const mam_norm_rotate_t *args, const void *v, const i
  * tokens are its own.
  *   extend: room for counts[b] tokens behind each request's, from the free pages of lowest number, in the requests' order.  A begun last page that other requests hold as well is
  *           given up for a new one, but by the last request that holds it: copies (B, 2) gets (page, new page), which mam_pages_copy takes, or -1, -1.  granted (B): counts[b], or 0 where the
- *           free pages or the slots do not reach; such a request is left as it was, and those behind it that need pages are too.
+ *           free pages or the slots do not reach; such a request is left as it was, and those behind it that need pages, or that would write to a page
+ *           which it was to give up, are too.
  *   fork:   request b goes on from request sources[b] as it was before the call; one that goes on from none (a number that is no request) is left empty.
  *   trim:   requests have ends[b] tokens (no more than their pages hold); pages behind are given back.
  */

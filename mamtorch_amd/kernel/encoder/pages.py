@@ -20,7 +20,8 @@ def pages_extend(table: Tensor, lengths: Tensor, refs: Tensor, counts: Tensor, p
 
     Pages are the free ones of lowest number, in the requests' order.  A begun last page that other requests hold too is given up for a new one, but by the last request that
     holds it; copies (batch, 2) names the page and the new one, for ``pages_copy``, or is -1.  granted (batch): a request's count, or 0 where the free pages or the table's slots do
-    not reach: that request is left as it was, and so are those behind it that need pages."""
+    not reach: that request is left as it was, and so are those behind it that need pages,
+    or that would write to a page which it was to give up."""
     return K.pages_extend.default(table, lengths, refs, counts, int(page_size))
 
 
