@@ -142,12 +142,16 @@ class PageTable:
 
     def begin(self, counts=None, parents: Tensor = None) -> Tensor:
         """Room for ``counts`` new tokens behind each request's (a number, or int32 (batch)), or for trees of drafted tokens, ``parents`` (batch, n) as
-        ``kernel.encoder.draft_tree`` takes them.  Returns how many tokens each request has room for: its count or, where the pages do not reach, 0, and then its tokens
+        ``kernel.encoder.draft_tree`` takes them, or for the first ``counts`` tokens of those.  Returns how many tokens each request has room for: its count or, where the pages do not reach, 0, and then its tokens
         are not written and give zeros."""
         if (counts is None) and (parents is None):
             raise ValueError("a step has counts or parents")
         self.masks = self.positions = None
-        counts = self._vector(parents.shape[1] if counts is None else counts)
+        if parents is None:
+            counts = self._vector(counts)
+        else:
+            n = parents.shape[1]
+            counts = self._vector(n) if counts is None else self._vector(counts).clamp(max=n)
         self.granted, copies = K.pages_extend(self.table, self.lengths, self.refs, counts, self.page_size)
         # whatever the step: how long pages stay in common after a fork, and whether a replayed graph held one, the device alone knows.  (4 to 5 us a layer where there is
         # nothing to copy: one token of 64 requests through 12 layers of 768 takes 3.20 ms, 3.11 without.)

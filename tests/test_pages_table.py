@@ -153,3 +153,21 @@ def test_a_captured_path_ends_where_the_eager_one_does():
         torch.cuda.synchronize()
         assert servers[0].table.lengths.tolist() == servers[1].table.lengths.tolist()
         assert torch.equal(servers[0].table.table, servers[1].table.table)
+
+
+def test_a_tree_has_no_more_tokens_than_it_names(device):
+    s = Server(device, 2, 12)
+    s.step([20, 3])
+    granted = s.table.begin(s.ints([9, 2]), s.ints([[-1, 0, 1]] * 2))
+    assert granted.tolist() == [3, 2]
+    ids, k, v = s.new(3)
+    s.append(k, v)
+    s.table.accept(s.ints([[0, 2, 5, 7]] * 2))
+    s.tokens = [s.tokens[0] + [ids[0][0], ids[0][2]], s.tokens[1] + [ids[1][0]]]
+    s.check("a path past the tree")
+    s.table.begin(s.ints([40, 40]), s.ints([[-1]] * 2))
+    ids, k, v = s.new(1)
+    s.append(k, v)
+    s.table.accept()
+    s.tokens = [t + row for t, row in zip(s.tokens, ids)]
+    s.check("trees of one token")
